@@ -46,6 +46,15 @@ extern "C" {
 #define REMORA_B200_B_KN 0 /* B is [K, N], N contiguous (dot_general rhs [K,N]) */
 #define REMORA_B200_B_NK 1 /* B is [N, K], K contiguous (transposed rhs)        */
 
+/* Element types of the entry points that take one. */
+#define REMORA_B200_BF16 0
+#define REMORA_B200_F16 1
+#define REMORA_B200_F32 2
+#define REMORA_B200_E4M3 3 /* 8-bit float, 4 exponent and 3 mantissa bits, no infinities */
+
+/* new_tokens value of remora_b200_kv_block_table that releases a request. */
+#define REMORA_B200_KV_RELEASE (-1)
+
 /* Text of the last error raised on the calling thread ("" if none). */
 const char* remora_b200_last_error(void);
 
@@ -55,7 +64,8 @@ int remora_b200_version(void);
 /* Synchronises the current device and reports (then clears) an error a
  * kernel recorded on the device since the last check: REMORA_B200_ERR_TIMEOUT
  * for a bounded device wait that expired, REMORA_B200_ERR_INVALID for a bad
- * value seen by a kernel (an expert id outside [0, E)). */
+ * value seen by a kernel (an expert id outside [0, E); a block id, slot or
+ * length outside its paged cache). */
 int remora_b200_device_status(void);
 
 /* ------------------------------------------------------------------------
@@ -164,6 +174,112 @@ int remora_b200_gemm_f32_exact(const float* A, const float* B, float* C, int64_t
 int remora_b200_attention_fwd_bf16(const void* q, const void* k, const void* v, void* out,
                                    int64_t batch, int64_t heads, int64_t seq, int64_t head_dim,
                                    int causal, float scale, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Decoding: attention of one new token per request over a paged key-value
+ * cache, the tables and slots of that cache, and rotary positions (no
+ * counterpart program in the reference, which has no cache).  One step of a
+ * serving loop is kv_block_table, then per layer rope_kv_append and
+ * paged_attention.
+ *
+ * A cache holds num_blocks blocks of block_size tokens; slot s is token
+ * s % block_size of block s / block_size.  Key and value caches are
+ * addressed by element strides of block, token and head (the head_dim
+ * elements of a row are adjacent), so [block][token][head][dim] and
+ * [block][head][token][dim] are both taken as they lie.  An E4M3 cache
+ * stores x / scale, rounded to nearest even and saturated at +-448.
+ * Values that only the device sees (block ids, slots, lengths) are checked
+ * there: a bad one is skipped and reported by remora_b200_device_status()
+ * as REMORA_B200_ERR_INVALID.
+ * --------------------------------------------------------------------- */
+
+/* Block tables, slots and positions of one step, from the requests' lengths.
+ * Request r (r < R <= 8192) holds lens[r] tokens in the first
+ * ceil(lens[r] / block_size) blocks of block_table[r * ld_table ...]
+ * (max_blocks entries); free_blocks (num_blocks entries) is a stack of the
+ * *free_count free block ids.  new_tokens[r] >= 0 appends that many tokens,
+ * REMORA_B200_KV_RELEASE gives the request's blocks back (its table row is
+ * left as it is, its length becomes 0).  Released blocks are pushed first, in
+ * (request, page) order; then blocks are popped in the same order.
+ *
+ * A request whose blocks would not be free, counting those of the requests
+ * before it, is refused whole (status 1), and so are later ones that need a
+ * block; status 2 marks a bad length or count, tokens past max_blocks blocks
+ * or past max_tokens.  A refused request keeps its length and blocks.
+ *
+ * Written: lens_out[R] and free_count_out[1] (either may be its input),
+ * cu_tokens[R+1] (first token of each request; refused ones keep their
+ * place), the new entries of block_table, and for each token t < max_tokens
+ * its slot, position and request: -1, 0, r for a token of a refused request
+ * and -1, 0, -1 behind the last token.  Deterministic; the same call on the
+ * same lens and free_count gives the same result again. */
+int remora_b200_kv_block_table(const int32_t* lens, const int32_t* new_tokens, int64_t R,
+                               int32_t* block_table, int64_t ld_table, int64_t max_blocks,
+                               int32_t* free_blocks, const int32_t* free_count,
+                               int64_t num_blocks, int64_t block_size, int32_t* lens_out,
+                               int32_t* free_count_out, int32_t* cu_tokens, int32_t* slots,
+                               int32_t* positions, int32_t* requests, int64_t max_tokens,
+                               int32_t* status, void* stream);
+
+/* Rotary positions: pair i < rot / 2 of each head turns by the angle
+ * p * freq[i], p = positions[axis_of[i] * ld_pos + b * S + s], so that
+ * a' = a cos - b sin, b' = a sin + b cos; inverse != 0 negates the angle,
+ * which is also the gradient of the forward form.  Pairs are (i, i + rot/2),
+ * or (2i, 2i + 1) if interleaved != 0; elements from rot on are copied.
+ * x and out: dtype BF16, F16 or F32, [B][S][H][D] by the strides x_b, x_s,
+ * x_h (elements; out may be x).  positions: n_axes rows of B * S int32 on the
+ * device.  freq (rot / 2 doubles) and axis_of (rot / 2 ints, NULL = all 0)
+ * are HOST arrays, read before the call returns.  rot even, <= min(D, 256);
+ * D <= 1024; n_axes <= 8.  Angles are exact to 2^-25 of a quarter turn at
+ * every 32-bit position.  Any strides; sizes, strides and bases that are
+ * multiples of 8 elements (and 16 bytes) move 8 pairs at a time. */
+int remora_b200_rope(const void* x, void* out, int dtype, int64_t B, int64_t S, int64_t H,
+                     int64_t D, int64_t x_b, int64_t x_s, int64_t x_h, int64_t out_b,
+                     int64_t out_s, int64_t out_h, const int32_t* positions, int64_t ld_pos,
+                     int n_axes, const double* freq, const int32_t* axis_of, int64_t rot,
+                     int interleaved, int inverse, void* stream);
+
+/* The same rotation of q and k, and the append of k and v to the cache, in
+ * one pass: q_out[t] = rope(q[t]), cache row of slots[t] = rope(k[t]) and
+ * v[t].  q [T][Hq][D], k and v [T][Hkv][D] by token and head strides (slices
+ * of one projection are taken as they lie; q_out may be q); dtype BF16 or
+ * F16; cache_dtype is dtype or E4M3 (then with the scales k_scale and
+ * v_scale, else both must be 1).  A token whose slot is -1 writes no cache
+ * row.  The rest as remora_b200_rope. */
+int remora_b200_rope_kv_append(
+    const void* q, const void* k, const void* v, void* q_out, int dtype, int64_t T, int64_t Hq,
+    int64_t Hkv, int64_t D, int64_t q_t, int64_t q_h, int64_t k_t, int64_t k_h, int64_t v_t,
+    int64_t v_h, int64_t qo_t, int64_t qo_h, const int32_t* positions, int64_t ld_pos, int n_axes,
+    const double* freq, const int32_t* axis_of, int64_t rot, int interleaved,
+    const int32_t* slots, void* k_cache, void* v_cache, int cache_dtype, int64_t num_blocks,
+    int64_t block_size, int64_t kc_block, int64_t kc_token, int64_t kc_head, int64_t vc_block,
+    int64_t vc_token, int64_t vc_head, float k_scale, float v_scale, void* stream);
+
+/* Bytes of device workspace remora_b200_paged_attention needs (0 for sizes
+ * it rejects).  Calls that may overlap on the GPU need one each. */
+size_t remora_b200_paged_attention_workspace_bytes(int64_t R, int64_t Hq, int64_t Hkv,
+                                                   int64_t D);
+
+/* out[r][h] = sum_j softmax_j(scale * q[r][h] . k_j) v_j over the keys
+ * j < lens[r] of request r (the last `window` of them if window > 0), key j
+ * in block block_table[r * ld_table + j / block_size] of the caches, kv head
+ * h / (Hq / Hkv).  One token per request; fp32 statistics.  lse (f32
+ * [R][Hq], may be NULL) = the natural logarithm of the softmax's sum.  A
+ * request without keys, or whose every score is -infinity, gives zeros and
+ * lse = -infinity.  Cache rows past a request's length are never used,
+ * whatever they hold.  q and out: dtype BF16 or F16, [R][Hq][D] by strides
+ * (out must not be q); caches: dtype, or E4M3 with scales.  D in {64, 128,
+ * 256}, Hq % Hkv == 0, R <= 8192; 16-byte aligned bases, strides of whole 16
+ * bytes.  The call is two launches: the split over the keys, then the join
+ * of what was split. */
+int remora_b200_paged_attention(
+    const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table,
+    const int32_t* lens, void* out, float* lse, int dtype, int cache_dtype, int64_t R, int64_t Hq,
+    int64_t Hkv, int64_t D, int64_t q_t, int64_t q_h, int64_t out_t, int64_t out_h,
+    int64_t num_blocks, int64_t block_size, int64_t kc_block, int64_t kc_token, int64_t kc_head,
+    int64_t vc_block, int64_t vc_token, int64_t vc_head, int64_t ld_table, int64_t max_blocks,
+    float scale, int64_t window, float k_scale, float v_scale, void* workspace,
+    size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------
  * MoE layer (mlir/stablehlo/mixtral_moe_layer.mlir:8-68; simple_moe.mlir:16-35)

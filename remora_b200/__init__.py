@@ -14,8 +14,10 @@ dispatcher that replaces its body.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
+from typing import NamedTuple
 
 import torch
 
@@ -33,6 +35,13 @@ ERR_UNSUPPORTED = -6
 
 B_KN = 0
 B_NK = 1
+
+BF16 = 0
+F16 = 1
+F32 = 2
+E4M3 = 3
+
+KV_RELEASE = -1
 
 
 class RemoraError(RuntimeError):
@@ -70,6 +79,17 @@ _SIGNATURES = {
     "remora_b200_gemm_bf16": ([P, P, P, I64, I64, I64, I64, I64, I64, I64, I64, I64, I64, I, P], I),
     "remora_b200_gemm_f32_exact": ([P, P, P, I64, I64, I64, I64, I64, I64, I, P], I),
     "remora_b200_attention_fwd_bf16": ([P, P, P, P, I64, I64, I64, I64, I, F, P], I),
+    "remora_b200_kv_block_table": ([P, P, I64, P, I64, I64, P, P, I64, I64, P, P, P, P, P, P, I64,
+                                    P, P], I),
+    "remora_b200_rope": ([P, P, I, I64, I64, I64, I64, I64, I64, I64, I64, I64, I64, P, I64, I, P,
+                          P, I64, I, I, P], I),
+    "remora_b200_rope_kv_append": ([P, P, P, P, I, I64, I64, I64, I64, I64, I64, I64, I64, I64,
+                                    I64, I64, I64, P, I64, I, P, P, I64, I, P, P, P, I, I64, I64,
+                                    I64, I64, I64, I64, I64, I64, F, F, P], I),
+    "remora_b200_paged_attention_workspace_bytes": ([I64, I64, I64, I64], ctypes.c_size_t),
+    "remora_b200_paged_attention": ([P, P, P, P, P, P, P, I, I, I64, I64, I64, I64, I64, I64, I64,
+                                     I64, I64, I64, I64, I64, I64, I64, I64, I64, I64, I64, F,
+                                     I64, F, F, P, ctypes.c_size_t, P], I),
     "remora_b200_moe_router_topk_bf16": ([P, P, I64, I64, I, I, P, P, P], I),
     "remora_b200_moe_dispatch_workspace_bytes": ([I64, I, I], ctypes.c_size_t),
     "remora_b200_moe_dispatch": ([P, I64, I, I, P, P, P, P, P, ctypes.c_size_t, P], I),
@@ -278,6 +298,258 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, causal: bool = 
     _check(lib().remora_b200_attention_fwd_bf16(q.data_ptr(), k.data_ptr(), v.data_ptr(),
                                                 out.data_ptr(), B, H, S, Dh, int(causal),
                                                 float(scale), _stream(q)))
+    return out
+
+
+# ----------------------------------------------------------------- decoding
+_DTYPES = {torch.bfloat16: BF16, torch.float16: F16, torch.float32: F32,
+           torch.float8_e4m3fn: E4M3}
+
+
+def _on(*ts: torch.Tensor):
+    """Checks that all tensors are on one CUDA device and makes it current for
+    the launch (a context manager; no cost where it is current already)."""
+    dev = ts[0].device
+    for t in ts:
+        if not t.is_cuda:
+            raise ValueError("remora_b200 operates on CUDA tensors only (no CPU fallback)")
+        if t.device != dev:
+            raise ValueError(f"tensors are on different devices: {dev} and {t.device}")
+    if dev.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(dev)
+
+
+def _ints(name: str, t: torch.Tensor, shape: tuple) -> None:
+    if t.dtype != torch.int32 or not t.is_contiguous() or tuple(t.shape) != shape:
+        raise ValueError(f"{name} must be a contiguous int32 tensor of shape {list(shape)}, got "
+                         f"{t.dtype} {list(t.shape)}")
+
+
+class KvStep(NamedTuple):
+    """What kv_block_table gives: the step's lengths, free-block count and, for
+    each new token, its slot, position and request."""
+    lens: torch.Tensor
+    free_count: torch.Tensor
+    cu_tokens: torch.Tensor
+    slots: torch.Tensor
+    positions: torch.Tensor
+    requests: torch.Tensor
+    status: torch.Tensor
+
+
+def kv_block_table(lens: torch.Tensor, new_tokens: torch.Tensor, block_table: torch.Tensor,
+                   free_blocks: torch.Tensor, free_count: torch.Tensor, block_size: int,
+                   max_tokens: int, out: KvStep | None = None) -> KvStep:
+    """Block tables, slots and positions of one serving step.
+
+    lens int32 [R], new_tokens int32 [R] (n >= 0 appends n tokens, KV_RELEASE
+    gives the request's blocks back), block_table int32 [R, max_blocks] and
+    free_blocks int32 [num_blocks] (a stack of free_count[0] free ids), both
+    updated in place.  max_tokens >= the step's tokens: the length of slots,
+    positions and requests (-1, 0, -1 behind the last token).  status[r]: 0
+    done, 1 refused for want of free blocks, 2 refused for a bad length or
+    count or no room in the table or in max_tokens; a refused request keeps
+    its length and its tokens get slot -1.  `out` may hold lens and free_count
+    themselves (updated in place)."""
+    if block_table.dim() != 2 or lens.dim() != 1 or free_blocks.dim() != 1:
+        raise ValueError("kv_block_table takes lens [R], block_table [R, max_blocks] and "
+                         "free_blocks [num_blocks]")
+    R, N = lens.shape[0], max_tokens
+    if block_table.shape[0] != R or block_table.shape[1] < 1 or free_blocks.shape[0] < 1:
+        raise ValueError("block_table must have a row of at least one block per request and "
+                         "free_blocks at least one entry")
+    _ints("lens", lens, (R,))
+    _ints("new_tokens", new_tokens, (R,))
+    _ints("free_blocks", free_blocks, (free_blocks.shape[0],))
+    _ints("free_count", free_count, (1,))
+    if block_table.dtype != torch.int32 or block_table.stride(1) != 1:
+        raise ValueError("block_table must be int32 with adjacent entries of a row")
+    if N < 0:
+        raise ValueError("max_tokens must not be negative")
+    guard = _on(lens, new_tokens, block_table, free_blocks, free_count)
+    if out is None:
+        # one allocation, cut up: lens, cu_tokens, status, count and the tokens' rows
+        sizes = (R, 1, R + 1, N, N, N, R)
+        out = KvStep(*torch.empty(sum(sizes), dtype=torch.int32, device=lens.device).split(sizes))
+    else:
+        for name, n in zip(KvStep._fields, (R, 1, R + 1, N, N, N, R)):
+            _ints(name, getattr(out, name), (n,))
+        _on(lens, *out)
+    with guard:
+        _check(lib().remora_b200_kv_block_table(
+            lens.data_ptr(), new_tokens.data_ptr(), R, block_table.data_ptr(),
+            block_table.stride(0) if R > 1 else block_table.shape[1], block_table.shape[1],
+            free_blocks.data_ptr(), free_count.data_ptr(), free_blocks.shape[0], block_size,
+            *(t.data_ptr() for t in out[:6]), N, out.status.data_ptr(), _stream(lens)))
+    return out
+
+
+def _rope_plan(freq, axis_of, positions, tokens: tuple):
+    """(n_axes, freq, axis_of, positions, rot) as the C ABI takes them."""
+    if freq.is_cuda or freq.dtype != torch.float64 or freq.dim() != 1:
+        raise ValueError("freq must be a host float64 tensor [rot / 2]")
+    if positions.dtype != torch.int32:
+        raise TypeError("positions must be int32")
+    if tuple(positions.shape) == tokens:
+        n_axes = 1
+    elif positions.dim() == len(tokens) + 1 and tuple(positions.shape[1:]) == tokens:
+        n_axes = positions.shape[0]
+    else:
+        raise ValueError(f"positions must be [axes, *{list(tokens)}] or {list(tokens)}, got "
+                         f"{list(positions.shape)}")
+    if axis_of is not None:
+        if axis_of.is_cuda or axis_of.dtype != torch.int32 or axis_of.shape != freq.shape:
+            raise ValueError("axis_of must be a host int32 tensor with an axis per frequency")
+        axis_of = axis_of.contiguous()
+    elif n_axes != 1:
+        raise ValueError("several axes of positions need axis_of")
+    return n_axes, freq.contiguous(), axis_of, positions.contiguous(), 2 * freq.shape[0]
+
+
+def rope(x: torch.Tensor, positions: torch.Tensor, freq: torch.Tensor,
+         axis_of: torch.Tensor | None = None, interleaved: bool = False, inverse: bool = False,
+         out: torch.Tensor | None = None) -> torch.Tensor:
+    """Rotary positions: pair i of each head turns by positions[axis_of[i]] * freq[i].
+
+    x bf16, f16 or f32, [B, S, H, D] or [T, H, D] with any strides but adjacent
+    head elements (for [B, H, S, D] pass x.transpose(1, 2)).  positions int32
+    [axes, B, S] / [axes, T], or without the axes for one.  freq: host float64
+    [rot / 2], rot <= D; axis_of: host int32 [rot / 2], the axis that each
+    frequency follows.  Pairs are (i, i + rot / 2), or neighbours if
+    interleaved.  inverse=True turns the other way: the gradient with respect
+    to x of the forward form.  out may be x; by default it has x's layout."""
+    if x.dim() not in (3, 4):
+        raise ValueError("rope takes x as [B, S, H, D] or [T, H, D]")
+    if x.dtype not in (torch.bfloat16, torch.float16, torch.float32):
+        raise TypeError(f"rope takes bf16, f16 or f32, got {x.dtype}")
+    n_axes, freq, axis_of, positions, rot = _rope_plan(freq, axis_of, positions,
+                                                       tuple(x.shape[:-2]))
+    guard = _on(x, positions) if out is None else _on(x, positions, out)
+    if out is None:
+        out = torch.empty_like(x)
+    elif out.shape != x.shape or out.dtype != x.dtype:
+        raise ValueError("out must have x's shape and type")
+    if x.stride(-1) != 1 or out.stride(-1) != 1:
+        raise ValueError("the elements of a head must be adjacent")
+    B, S = (x.shape[0], x.shape[1]) if x.dim() == 4 else (1, x.shape[0])
+    xs, os_ = ((t.stride() if t.dim() == 4 else (0,) + t.stride()) for t in (x, out))
+    with guard:
+        _check(lib().remora_b200_rope(
+            x.data_ptr(), out.data_ptr(), _DTYPES[x.dtype], B, S, x.shape[-2], x.shape[-1], *xs[:3],
+            *os_[:3], positions.data_ptr(), B * S, n_axes, freq.data_ptr(),
+            None if axis_of is None else axis_of.data_ptr(), rot, int(interleaved), int(inverse),
+            _stream(x)))
+    return out
+
+
+def _cache(q, k_cache, v_cache, Hkv: int, D: int) -> int:
+    """Checks a pair of caches against q and gives their element type."""
+    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.shape[2:] != (Hkv, D):
+        raise ValueError(f"the caches must be [num_blocks, block_size, {Hkv}, {D}] of one shape, "
+                         f"got {list(k_cache.shape)} and {list(v_cache.shape)}")
+    if k_cache.dtype != v_cache.dtype or k_cache.dtype not in (q.dtype, torch.float8_e4m3fn):
+        raise TypeError(f"the caches must be {q.dtype} or float8_e4m3fn, got {k_cache.dtype} and "
+                        f"{v_cache.dtype}")
+    if k_cache.stride(3) != 1 or v_cache.stride(3) != 1:
+        raise ValueError("the elements of a cache row must be adjacent")
+    return _DTYPES[k_cache.dtype]
+
+
+def rope_kv_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
+                   slots: torch.Tensor, freq: torch.Tensor, k_cache: torch.Tensor,
+                   v_cache: torch.Tensor, axis_of: torch.Tensor | None = None,
+                   interleaved: bool = False, k_scale: float = 1.0, v_scale: float = 1.0,
+                   q_out: torch.Tensor | None = None) -> torch.Tensor:
+    """Rotates q and k as rope() does and writes k and v to the paged cache.
+
+    q [T, Hq, D], k and v [T, Hkv, D], bf16 or f16, with any strides but
+    adjacent head elements (slices of one projection are taken as they lie).
+    k_cache and v_cache [num_blocks, block_size, Hkv, D] of q's type or
+    float8_e4m3fn (x / scale is stored), any strides but adjacent row
+    elements; row slots[t] of each is written, slot -1 writes none.  Returns
+    the rotated q (q_out may be q)."""
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[0] != k.shape[0] or \
+            q.shape[2] != k.shape[2]:
+        raise ValueError("rope_kv_append takes q [T, Hq, D] and k, v [T, Hkv, D]")
+    if q.dtype not in (torch.bfloat16, torch.float16) or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError("rope_kv_append takes q, k and v in bf16 or all in f16")
+    T, Hq, D = q.shape
+    Hkv = k.shape[1]
+    cdt = _cache(q, k_cache, v_cache, Hkv, D)
+    n_axes, freq, axis_of, positions, rot = _rope_plan(freq, axis_of, positions, (T,))
+    _ints("slots", slots, (T,))
+    guard = _on(q, k, v, positions, slots, k_cache, v_cache)
+    if q_out is None:
+        q_out = torch.empty((T, Hq, D), dtype=q.dtype, device=q.device)
+    elif q_out.shape != q.shape or q_out.dtype != q.dtype or q_out.device != q.device:
+        raise ValueError("q_out must have q's shape, type and device")
+    if any(t.stride(2) != 1 for t in (q, k, v, q_out)):
+        raise ValueError("the elements of a head must be adjacent")
+    with guard:
+        _check(lib().remora_b200_rope_kv_append(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), q_out.data_ptr(), _DTYPES[q.dtype], T, Hq,
+            Hkv, D, q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+            q_out.stride(0), q_out.stride(1), positions.data_ptr(), T, n_axes, freq.data_ptr(),
+            None if axis_of is None else axis_of.data_ptr(), rot, int(interleaved),
+            slots.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), cdt, k_cache.shape[0],
+            k_cache.shape[1], *k_cache.stride()[:3], *v_cache.stride()[:3], k_scale, v_scale,
+            _stream(q)))
+    return q_out
+
+
+def paged_attention_workspace_bytes(R: int, Hq: int, Hkv: int, D: int) -> int:
+    return int(lib().remora_b200_paged_attention_workspace_bytes(R, Hq, Hkv, D))
+
+
+def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                    block_table: torch.Tensor, lens: torch.Tensor, scale: float | None = None,
+                    window: int = 0, k_scale: float = 1.0, v_scale: float = 1.0,
+                    out: torch.Tensor | None = None, lse: torch.Tensor | None = None,
+                    workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Softmax attention of one new token per request over its cached keys.
+
+    q bf16 or f16 [R, Hq, D], D 64, 128 or 256; caches as rope_kv_append
+    writes them; block_table int32 [R, max_blocks]; lens int32 [R], the keys of
+    each request (0: its rows of out are zero).  window > 0: the last `window`
+    keys only.  lse f32 [R, Hq], if given, takes the natural logarithm of each
+    softmax's sum (-inf without keys).  Calls that may run at the same time
+    need a workspace each (by default every call has its own)."""
+    if q.dim() != 3 or block_table.dim() != 2:
+        raise ValueError("paged_attention takes q [R, Hq, D] and block_table [R, max_blocks]")
+    if q.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"paged_attention takes q in bf16 or f16, got {q.dtype}")
+    R, Hq, D = q.shape
+    Hkv = k_cache.shape[2] if k_cache.dim() == 4 else 0
+    cdt = _cache(q, k_cache, v_cache, Hkv, D)
+    _ints("lens", lens, (R,))
+    if block_table.dtype != torch.int32 or block_table.shape[0] != R or \
+            block_table.stride(1) != 1:
+        raise ValueError("block_table must be int32 [R, max_blocks] with adjacent entries")
+    guard = _on(q, k_cache, v_cache, block_table, lens)
+    if out is None:
+        out = torch.empty((R, Hq, D), dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
+        raise ValueError("out must have q's shape, type and device")
+    if q.stride(2) != 1 or out.stride(2) != 1:
+        raise ValueError("the elements of a head must be adjacent")
+    if lse is not None and (lse.dtype != torch.float32 or tuple(lse.shape) != (R, Hq) or
+                            not lse.is_contiguous() or lse.device != q.device):
+        raise ValueError("lse must be a contiguous float32 tensor [R, Hq]")
+    if workspace is None:
+        need = paged_attention_workspace_bytes(R, Hq, Hkv, D)
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    elif workspace.device != q.device or not workspace.is_contiguous():
+        raise ValueError("workspace must be a contiguous tensor on q's device")
+    with guard:
+        _check(lib().remora_b200_paged_attention(
+            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
+            lens.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(),
+            _DTYPES[q.dtype], cdt, R, Hq, Hkv, D, q.stride(0), q.stride(1), out.stride(0),
+            out.stride(1), k_cache.shape[0], k_cache.shape[1], *k_cache.stride()[:3],
+            *v_cache.stride()[:3], block_table.stride(0) if R > 1 else block_table.shape[1],
+            block_table.shape[1], D ** -0.5 if scale is None else scale, window, k_scale, v_scale,
+            workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream(q)))
     return out
 
 

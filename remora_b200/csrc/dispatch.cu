@@ -473,6 +473,9 @@ extern "C" int remora_b200_device_status(void) {
   RB_CUDA(cudaMemcpyToSymbol(rb::g_device_error, &zero, sizeof(int)));
   if (v == 1) return rb::fail(REMORA_B200_ERR_TIMEOUT, "a device-side wait timed out");
   if (v == 2) return rb::fail(REMORA_B200_ERR_INVALID, "an expert index was outside [0, E)");
+  if (v == 3)
+    return rb::fail(REMORA_B200_ERR_INVALID,
+                    "a block id, slot or length was outside its paged cache");
   return rb::fail(REMORA_B200_ERR_INVALID, "device reported error %d", v);
 }
 

@@ -1,0 +1,281 @@
+// kv_tables.cu -- block tables and slot maps of a paged key-value cache, built
+// on the GPU from the requests' lengths (no counterpart in the reference,
+// which has no cache; it serves the attention beside it).
+//
+// One step of a serving loop appends n_r tokens to each request r (or releases
+// it).  With bs tokens per block, request r owns ceil(len_r / bs) blocks and
+// needs ceil((len_r + n_r) / bs) - ceil(len_r / bs) more.  The free blocks are
+// a stack; released blocks are pushed on it in (request, page) order, then the
+// needed ones are popped in the same order: the j-th block of the step is
+// entry have - 1 - j of the stack, so every token finds its own block from
+// three prefix sums (tokens, blocks needed, blocks released) and no block is
+// handed out by an atomic whose order could change the result.
+//
+// The call is latency bound (a few KB per thousand tokens).  It is therefore
+// one launch of one cluster: every CTA scans the requests by itself (at most
+// 8192 lengths), the CTAs meet at a cluster barrier before anything is written,
+// and tokens are then spread over all threads, each finding its request by
+// binary search in the shared-memory prefix sums.
+#include "runtime.cuh"
+
+namespace rb {
+namespace kv {
+
+constexpr int kMaxRequests = 8192;
+
+struct TableArgs {
+  const int32_t *lens, *fresh;
+  int32_t* table;
+  int64_t ld_table;
+  int32_t *free_blocks, *lens_out, *free_out, *cu, *slots, *positions, *requests, *status;
+  const int32_t* free_count;
+  int32_t R, max_blocks, num_blocks, bs, max_tokens;
+};
+
+__device__ __forceinline__ void cluster_barrier() {
+  asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+
+__device__ __forceinline__ uint32_t cluster_size() {
+  uint32_t n;
+  asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(n));
+  return n;
+}
+
+__device__ __forceinline__ int32_t sat32(int64_t v) {
+  return v > 0x7fffffffll ? 0x7fffffff : (int32_t)v;
+}
+
+// What one request asks for: tokens, blocks needed, blocks released.
+struct Ask {
+  int64_t tokens, need, back;
+  bool bad;
+};
+
+__device__ __forceinline__ Ask ask_of(const TableArgs& a, int32_t len, int32_t n) {
+  Ask q{0, 0, 0, false};
+  const int64_t room = (int64_t)a.max_blocks * a.bs;
+  const bool held = len >= 0 && len <= room;
+  const int32_t own = held ? (int32_t)(((int64_t)len + a.bs - 1) / a.bs) : 0;
+  if (n >= 0) {
+    q.tokens = n;
+    q.bad = !held || (int64_t)len + n > room;
+    if (!q.bad) q.need = ((int64_t)len + n + a.bs - 1) / a.bs - own;
+  } else {
+    q.bad = n != REMORA_B200_KV_RELEASE || !held;
+    if (!q.bad) q.back = own;
+  }
+  return q;
+}
+
+// Largest i with prefix[i] <= v, over prefix[0..n] (prefix[0] = 0, v >= 0).
+__device__ __forceinline__ int find_le(const int32_t* prefix, int n, int32_t v) {
+  int lo = 0, hi = n + 1;  // prefix[lo] <= v < prefix[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (prefix[mid] <= v) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+__global__ void __launch_bounds__(1024) k_block_table(const TableArgs a) {
+  extern __shared__ int32_t sm[];
+  int32_t* cu = sm;                    // [R + 1] tokens before request r
+  int32_t* need = cu + a.R + 1;        // [R + 1] blocks needed before request r
+  int32_t* back = need + a.R + 1;      // [R + 1] blocks released before request r
+  int32_t* len0 = back + a.R + 1;      // [R] length before the step; bit 31: refused
+  __shared__ int64_t part[3][32];
+  __shared__ int32_t taken;
+  const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5;
+  const int nw = nt >> 5;
+  if (tid == 0) taken = 0;
+
+  // prefix sums: each thread sums a run of requests, then warps, then the block
+  const int c = (a.R + nt - 1) / nt;
+  const int r0 = min(tid * c, a.R), r1 = min(r0 + c, a.R);
+  int64_t s0 = 0, s1 = 0, s2 = 0;
+  int64_t before = 0;  // tokens: a request whose tokens pass max_tokens is refused, so its
+                       // blocks are not counted; that needs the token sum first
+  for (int r = r0; r < r1; ++r) {
+    const Ask q = ask_of(a, a.lens[r], a.fresh[r]);
+    s0 += q.tokens;
+  }
+  int64_t x = s0;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t y = __shfl_up_sync(~0u, x, o);
+    if (lane >= o) x += y;
+  }
+  if (lane == 31) part[0][warp] = x;
+  __syncthreads();
+  int64_t base = 0;
+  for (int w = 0; w < warp; ++w) base += part[0][w];
+  before = base + x - s0;
+  {
+    int64_t t = before;
+    for (int r = r0; r < r1; ++r) {
+      const Ask q = ask_of(a, a.lens[r], a.fresh[r]);
+      t += q.tokens;
+      if (t <= a.max_tokens) s1 += q.need;
+      s2 += q.back;
+    }
+  }
+  int64_t x1 = s1, x2 = s2;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t y1 = __shfl_up_sync(~0u, x1, o), y2 = __shfl_up_sync(~0u, x2, o);
+    if (lane >= o) { x1 += y1; x2 += y2; }
+  }
+  if (lane == 31) { part[1][warp] = x1; part[2][warp] = x2; }
+  __syncthreads();
+  int64_t b1 = 0, b2 = 0, all2 = 0;
+  for (int w = 0; w < nw; ++w) {
+    if (w < warp) { b1 += part[1][w]; b2 += part[2][w]; }
+    all2 += part[2][w];
+  }
+  const int32_t count_in = *a.free_count;
+  const int32_t count0 = min(max(count_in, 0), a.num_blocks);
+  const int32_t have = (int32_t)min((int64_t)count0 + all2, (int64_t)a.num_blocks);
+  {
+    int64_t t = before, p1 = b1 + x1 - s1, p2 = b2 + x2 - s2;
+    for (int r = r0; r < r1; ++r) {
+      const int32_t len = a.lens[r];
+      const Ask q = ask_of(a, len, a.fresh[r]);
+      cu[r] = sat32(t);
+      need[r] = sat32(p1);
+      back[r] = sat32(p2);
+      t += q.tokens;
+      const bool bad = q.bad || t > a.max_tokens;
+      if (t <= a.max_tokens) p1 += q.need;
+      p2 += q.back;
+      const bool dry = !bad && q.need > 0 && p1 > have;
+      if (!bad && !dry && q.need > 0) atomicMax(&taken, (int32_t)p1);
+      len0[r] = (len & 0x7fffffff) | (bad || dry ? 0x80000000 : 0);
+    }
+    if (r1 == a.R) {  // several threads when R is short of the block: the same values
+      cu[a.R] = sat32(t);
+      need[a.R] = sat32(p1);
+      back[a.R] = sat32(p2);
+    }
+  }
+  const uint32_t rank = cluster_rank(), ctas = cluster_size();
+  const int me = rank * nt + tid, step = ctas * nt;
+  cluster_barrier();  // every CTA has read the lengths and the count: they may be overwritten
+
+  if (me == 0 && (count_in != count0 || (int64_t)count0 + all2 > a.num_blocks))
+    atomicExch(&g_device_error, 3);
+
+  // push the released blocks
+  const int32_t n_back = back[a.R];
+  if (n_back > 0) {  // the same in every CTA of the cluster
+    const int room = min(n_back, a.num_blocks - count0);
+    for (int64_t i = me; i < room; i += step) {
+      const int j = (int)i, r = find_le(back, a.R, j);
+      a.free_blocks[count0 + j] = a.table[(int64_t)r * a.ld_table + (j - back[r])];
+    }
+    cluster_barrier();
+  }
+
+  // each token's slot; the token that opens a block enters it into the table
+  const int32_t total = cu[a.R];
+  for (int64_t i = me; i < a.max_tokens; i += step) {
+    const int32_t t = (int32_t)i;
+    int32_t slot = -1, pos = 0, req = -1;
+    if (t < total) {
+      req = find_le(cu, a.R, t);
+      const int32_t l = len0[req];
+      if (l >= 0) {
+        pos = l + (t - cu[req]);
+        const int32_t page = pos / a.bs, off = pos - page * a.bs;
+        const int32_t own = (int32_t)(((int64_t)l + a.bs - 1) / a.bs);
+        int32_t id;
+        if (page < own) {
+          id = a.table[(int64_t)req * a.ld_table + page];
+        } else {
+          id = __ldcg(a.free_blocks + (have - 1 - (need[req] + page - own)));
+          if (off == 0) a.table[(int64_t)req * a.ld_table + page] = id;
+        }
+        if (id >= 0 && id < a.num_blocks) slot = id * a.bs + off;
+        else atomicExch(&g_device_error, 3);
+      }
+    }
+    a.slots[t] = slot;
+    a.positions[t] = pos;
+    a.requests[t] = req;
+  }
+
+  for (int r = me; r < a.R; r += step) {
+    const int32_t n = a.fresh[r], l = len0[r];
+    const bool no = l < 0;
+    // a refused request keeps its length, whatever it is
+    if (!no) a.lens_out[r] = n >= 0 ? l + n : 0;
+    else if (a.lens_out != a.lens) a.lens_out[r] = a.lens[r];
+    const bool dry = no && n >= 0 && cu[r + 1] <= a.max_tokens &&
+                     !ask_of(a, a.lens[r], n).bad;
+    a.status[r] = !no ? 0 : dry ? 1 : 2;
+    a.cu[r] = cu[r];
+  }
+  if (me == 0) {
+    a.cu[a.R] = total;
+    *a.free_out = have - taken;
+  }
+}
+
+}  // namespace kv
+}  // namespace rb
+
+extern "C" int remora_b200_kv_block_table(
+    const int32_t* lens, const int32_t* new_tokens, int64_t R, int32_t* block_table,
+    int64_t ld_table, int64_t max_blocks, int32_t* free_blocks, const int32_t* free_count,
+    int64_t num_blocks, int64_t block_size, int32_t* lens_out, int32_t* free_count_out,
+    int32_t* cu_tokens, int32_t* slots, int32_t* positions, int32_t* requests,
+    int64_t max_tokens, int32_t* status, void* stream) {
+  using namespace rb;
+  using namespace rb::kv;
+  clear_error();
+  RB_CHECK_ARG(R >= 0 && R <= kMaxRequests, "kv_block_table: R must be in [0, %d], got %lld",
+               kMaxRequests, (long long)R);
+  RB_CHECK_ARG(max_tokens >= 0 && max_tokens < 0x7fffffff,
+               "kv_block_table: max_tokens must be in [0, 2^31 - 1)");
+  RB_CHECK_ARG(block_size >= 1 && num_blocks >= 1 && num_blocks < 0x7fffffff &&
+                   block_size <= 0x7fffffff && num_blocks <= 0x7fffffff / block_size,
+               "kv_block_table: num_blocks * block_size must be in [1, 2^31)");
+  RB_CHECK_ARG(max_blocks >= 1 && max_blocks <= 0x7fffffff / block_size,
+               "kv_block_table: max_blocks * block_size must be in [1, 2^31)");
+  RB_CHECK_ARG(ld_table >= max_blocks, "kv_block_table: ld_table must be at least max_blocks");
+  RB_CHECK_ARG(free_blocks && free_count && free_count_out && cu_tokens,
+               "kv_block_table: null pointer");
+  RB_CHECK_ARG(R == 0 || (lens && new_tokens && block_table && lens_out && status),
+               "kv_block_table: null pointer");
+  RB_CHECK_ARG(max_tokens == 0 || (slots && positions && requests),
+               "kv_block_table: null pointer");
+  TableArgs a{lens, new_tokens, block_table, ld_table, free_blocks, lens_out, free_count_out,
+              cu_tokens, slots, positions, requests, status, free_count, (int32_t)R,
+              (int32_t)max_blocks, (int32_t)num_blocks, (int32_t)block_size,
+              (int32_t)max_tokens};
+  const size_t smem = (4 * (size_t)R + 3) * sizeof(int32_t);
+  if (smem > 48 * 1024)
+    RB_CUDA(cudaFuncSetAttribute(k_block_table, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 (4 * kMaxRequests + 3) * (int)sizeof(int32_t)));
+  const int threads = 1024, ctas = max_tokens > 4096 ? 8 : 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = as_stream(stream);
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim = {(unsigned)ctas, 1, 1};
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  RB_CUDA(cudaLaunchKernelEx(&cfg, k_block_table, a));
+  return REMORA_B200_OK;
+}

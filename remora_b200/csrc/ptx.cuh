@@ -13,7 +13,8 @@
 namespace rb {
 
 // Device-side error word, read back by the host after launches that can fail.
-// Codes: 1 = mbarrier wait timed out, 2 = bad argument seen on device.
+// Codes: 1 = mbarrier wait timed out, 2 = bad argument seen on device (an expert
+// id), 3 = a block id, slot or length outside its paged cache.
 __device__ int g_device_error = 0;
 
 constexpr uint64_t kWaitLimitNs = 2000000000ull;  // 2 s per wait
