@@ -10,7 +10,9 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
+#include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "runtime.cuh"
 
@@ -18,6 +20,8 @@ namespace rb {
 namespace paged {
 
 constexpr int kMaxRequests = 8192;
+constexpr int kRingBytes = 196608;  // shared memory of a CTA's rings
+constexpr int kMinTiles = 2;        // tiles of a warp at least
 
 struct Args {
   const void *q, *kc, *vc;
@@ -28,59 +32,800 @@ struct Args {
   int64_t kc_b, kc_t, kc_h, vc_b, vc_t, vc_h;
   int64_t ld_table, window;
   int32_t R, Hq, Hkv, D, num_blocks, bs, max_blocks;
-  float scale2, k_scale, v_scale;  // scale2 = scale * log2(e)
+  float scale2, v_scale;  // scale2 = scale * log2(e) * the keys' scale
 };
 
-template <typename T> __device__ __forceinline__ float up(T v);
-template <> __device__ __forceinline__ float up(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <> __device__ __forceinline__ float up(__half v) { return __half2float(v); }
-template <> __device__ __forceinline__ float up(__nv_fp8_e4m3 v) { return float(v); }
-template <typename T> __device__ __forceinline__ T down(float v);
-template <> __device__ __forceinline__ __nv_bfloat16 down(float v) { return __float2bfloat16_rn(v); }
-template <> __device__ __forceinline__ __half down(float v) { return __float2half_rn(v); }
+// ------------------------------------------------------------- fragments
+__device__ __forceinline__ void ldm_x4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldm_x4_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+// c += a (16 x 16) . b (16 x 8), M the 16-bit type of both.
+template <typename M>
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                         uint32_t a3, uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<M, __half>::value)
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+        "{%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Two values of the 8-bit type (the low or high half of x) as two of f16: exact.
+__device__ __forceinline__ uint32_t f16x2_lo(uint32_t x) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\t}"
+      : "=r"(r)
+      : "r"(x));
+  return r;
+}
+__device__ __forceinline__ uint32_t f16x2_hi(uint32_t x) {
+  uint32_t r;
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}"
+      : "=r"(r)
+      : "r"(x));
+  return r;
+}
+template <typename M>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  if constexpr (std::is_same<M, __half>::value) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+  } else {
+    return pack_bf16x2(lo, hi);
+  }
+}
 
-// One warp per (request, query head), one key at a time.
-template <typename T, typename C>
-__global__ void __launch_bounds__(128) k_paged_simple(const __grid_constant__ Args a) {
-  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31;
-  if (w >= (int64_t)a.R * a.Hq) return;
-  const int r = (int)(w / a.Hq), h = (int)(w - (int64_t)r * a.Hq);
-  const int hk = h / (a.Hq / a.Hkv);
+template <typename M>
+__device__ __forceinline__ float2 unpack2(uint32_t x) {
+  if constexpr (std::is_same<M, __half>::value) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&x));
+  } else {
+    return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xffff0000u));
+  }
+}
+
+// ------------------------------------------------------------------ shapes
+template <typename C, int D>
+struct Shape {
+  static constexpr int RB = D * (int)sizeof(C);     // bytes of a row
+  static constexpr int CH = RB / 16;                // 16-byte pieces of a row
+  static constexpr int KT = RB <= 128 ? 32 : 16;    // keys of a tile
+  static constexpr int SB = 2 * KT * RB;            // a tile's keys and values
+  static constexpr int W = SB > 8192 ? 4 : 8;       // warps
+  static constexpr int S = kRingBytes / (W * SB) > 6 ? 6 : kRingBytes / (W * SB);
+  static constexpr size_t kSmem = (size_t)W * S * SB;
+  static_assert(S >= 2 && kSmem <= kRingBytes, "ring");
+};
+
+// Piece c of row `row` lies at piece c ^ swz(row): the eight rows of an ldmatrix
+// fall into eight different banks' groups (two rows to a 128-byte line if RB is 64).
+template <int RB>
+__device__ __forceinline__ int swz(int row) {
+  return RB >= 128 ? (row & 7) : ((row >> 1) & 3);
+}
+
+// The tiles [first, end) of request length `len`: whole tiles of the keys it uses.
+__device__ __forceinline__ void tiles_of(const Args& a, int32_t len, int KT, int& t0, int& t1) {
   const int64_t room = (int64_t)a.max_blocks * a.bs;
-  int64_t len = a.lens[r];
-  if (len < 0 || len > room) {
-    atomicExch(&g_device_error, 3);
-    len = len < 0 ? 0 : room;
+  const int32_t n = (int32_t)min((int64_t)max(len, 0), room);
+  const int32_t start = a.window > 0 && n > a.window ? n - (int32_t)a.window : 0;
+  t0 = start / KT;
+  t1 = (int)(((int64_t)n + KT - 1) / KT);
+}
+
+struct Stage {  // what the reader of a tile needs to know
+  uint32_t mask;   // keys that count
+  int32_t r, h;    // the item
+  uint32_t flags;  // 1: first tile of this worker's part, 2: first of the item, 4: last of the
+                   // item; the item's tiles behind this one << 3
+};
+
+// A warp's walk over its tiles, as it fetches them.
+template <typename C, int D>
+struct Walk {
+  using X = Shape<C, D>;
+  int64_t left;        // tiles not fetched yet
+  int32_t g, r, h;     // group of 32 requests, request, item of the request
+  int32_t t, t0, t1;   // tile, and the request's
+  int32_t n, start;    // the request's keys [start, n)
+  int32_t glen;        // this lane's request of the group: its length
+  int32_t id;          // this lane's key of the tile to come: its block, and its place there
+  int32_t off;
+  bool ok, fresh;
+
+  __device__ __forceinline__ void load_group(const Args& a, int lane) {
+    const int i = g * 32 + lane;
+    glen = i < a.R ? a.lens[i] : 0;
   }
-  const T* q = (const T*)a.q + r * a.q_t + h * a.q_h;
-  const int n = a.D / 32;
-  float x[8], o[8] = {}, m = -INFINITY, l = 0;
-  for (int i = 0; i < n; ++i) x[i] = up(q[lane + 32 * i]);
-  for (int64_t j = a.window > 0 && len > a.window ? len - a.window : 0; j < len; ++j) {
-    const int page = (int)(j / a.bs), off = (int)(j - (int64_t)page * a.bs);
-    const int id = a.table[r * a.ld_table + page];
-    if (id < 0 || id >= a.num_blocks) {
-      atomicExch(&g_device_error, 3);
-      continue;
+  __device__ __forceinline__ void set_request(const Args& a) {
+    const int32_t len = __shfl_sync(~0u, glen, r & 31);
+    tiles_of(a, len, X::KT, t0, t1);
+    n = (int32_t)min((int64_t)max(len, 0), (int64_t)a.max_blocks * a.bs);
+    start = a.window > 0 && n > a.window ? n - (int32_t)a.window : 0;
+  }
+  // The block of this lane's key of tile t: fetched a tile ahead of its use.
+  __device__ __forceinline__ void look_up(const Args& a, int lane) {
+    const int32_t key = t * X::KT + (lane & (X::KT - 1));
+    ok = key >= start && key < n;
+    id = -1;
+    off = 0;
+    if (ok) {
+      const int32_t page = key / a.bs;
+      off = key - page * a.bs;
+      id = __ldg(a.table + (int64_t)r * a.ld_table + page);
     }
-    const C* k = (const C*)a.kc + id * a.kc_b + off * a.kc_t + hk * a.kc_h;
-    const C* v = (const C*)a.vc + id * a.vc_b + off * a.vc_t + hk * a.vc_h;
-    float s = 0;
-    for (int i = 0; i < n; ++i) s += x[i] * up(k[lane + 32 * i]);
-    for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(~0u, s, d);
-    s *= a.scale2 * a.k_scale;
-    const float m1 = fmaxf(m, s), base = m1 == -INFINITY ? 0.0f : m1;
-    const float c = exp2f(m - base), p = exp2f(s - base);
-    l = l * c + p;
-    m = m1;
-    for (int i = 0; i < n; ++i) o[i] = o[i] * c + p * up(v[lane + 32 * i]);
   }
-  T* out = (T*)a.out + r * a.o_t + h * a.o_h;
-  const float inv = l == 0.0f ? 0.0f : a.v_scale / l;
-  for (int i = 0; i < n; ++i) out[lane + 32 * i] = down<T>(o[i] * inv);
-  if (a.lse && lane == 0)
-    a.lse[(int64_t)r * a.Hq + h] = l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+  __device__ __forceinline__ void next(const Args& a, int Hg, int lane) {
+    ++t;
+    fresh = false;
+    if (t == t1) {
+      fresh = true;
+      if (++h == Hg) {
+        h = 0;
+        do {
+          if (++r >= a.R) {  // only if the lengths changed under the call: end, do not spin
+            left = 0;
+            return;
+          }
+          if ((r & 31) == 0) {
+            ++g;
+            load_group(a, lane);
+          }
+          set_request(a);
+        } while (t0 >= t1);
+      }
+      t = t0;
+    }
+  }
+  // Starts the copies of the next tile into `ring` (a stage), or commits nothing.
+  __device__ __forceinline__ void fetch(const Args& a, int Hg, int ngr, char* ring, Stage* st,
+                                        int lane) {
+    if (left > 0) {
+      const bool in = ok && id >= 0 && id < a.num_blocks;
+      if (ok && !in) atomicExch(&g_device_error, 3);
+      const uint32_t mask = __ballot_sync(~0u, in) & (X::KT == 32 ? ~0u : 0xffffu);
+      const int hk = h / ngr;
+      int64_t ko = 0, vo = 0;
+      if (in) {
+        ko = id * a.kc_b + off * a.kc_t + hk * a.kc_h;
+        vo = id * a.vc_b + off * a.vc_t + hk * a.vc_h;
+      }
+      if (lane == 0) {
+        const uint32_t f = (fresh ? 1u : 0u) | (t == t0 ? 2u : 0u) | (t == t1 - 1 ? 4u : 0u);
+        *st = Stage{mask, r, h, f | (uint32_t)(t1 - 1 - t) << 3};
+      }
+      char* kd = ring;
+      char* vd = ring + X::KT * X::RB;
+#pragma unroll
+      for (int i = 0; i < X::KT * X::CH / 32; ++i) {
+        const int p = i * 32 + lane, row = p / X::CH, c = p % X::CH;
+        const int64_t k1 = __shfl_sync(~0u, ko, row), v1 = __shfl_sync(~0u, vo, row);
+        const bool there = mask >> row & 1;
+        const int at = row * X::RB + ((c ^ swz<X::RB>(row)) << 4);
+        cp_async16(kd + at, (const char*)a.kc + k1 * (int64_t)sizeof(C) + c * 16, there);
+        cp_async16(vd + at, (const char*)a.vc + v1 * (int64_t)sizeof(C) + c * 16, there);
+      }
+      if (--left > 0) {
+        next(a, Hg, lane);
+        if (left > 0) look_up(a, lane);
+      }
+    } else if (lane == 0) {
+      st->r = -1;
+    }
+    cp_async_commit();
+  }
+};
+
+// ------------------------------------------------------------------ results
+// One 16 x 8 fragment of an item's output: lane (g, t) = (lane / 4, lane % 4)
+// holds heads 2t and 2t+1 of group nt at two d's: 16j + g and that + 8 (16-bit
+// caches), or 16j + 2g and that + 1 (8-bit).  All lanes of a warp call it.
+template <typename T, typename C>
+__device__ __forceinline__ void store_fragment(T* out, int64_t o_h, int heads, int nt, int j,
+                                               int lane, float4 c) {
+  const int g = lane >> 2, t = lane & 3;
+  if constexpr (sizeof(C) == 1) {
+    const int h = nt * 8 + 2 * t;
+    uint32_t* p = reinterpret_cast<uint32_t*>(out + h * o_h + 16 * j + 2 * g);
+    if (h < heads) *p = pack2<T>(c.x, c.z);
+    if (h + 1 < heads) *reinterpret_cast<uint32_t*>(reinterpret_cast<T*>(p) + o_h) =
+        pack2<T>(c.y, c.w);
+  } else {
+    const uint32_t lo = transpose8x8(pack2<T>(c.x, c.y));
+    const uint32_t hi = transpose8x8(pack2<T>(c.z, c.w));
+    const int h = nt * 8 + g;
+    if (h < heads) {
+      T* p = out + h * o_h + 16 * j + 2 * t;
+      *reinterpret_cast<uint32_t*>(p) = lo;
+      *reinterpret_cast<uint32_t*>(p + 8) = hi;
+    }
+  }
+}
+
+__device__ __forceinline__ float lse_of(float m, float l) {
+  return l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+}
+// 2^(m - top), where top may be -inf (then so is m: nothing was seen).
+__device__ __forceinline__ float weight(float m, float top) {
+  return exp2f(m - (top == -INFINITY ? 0.0f : top));
+}
+
+// A partial result: fragments [nt][j][lane] as float4, then m[8 NT], l[8 NT].
+template <int D, int NT>
+constexpr int kPartFloats = NT * 8 * (D + 2);
+
+// The CTA's share of the join: what crosses into the next CTA.
+struct Cross {
+  int32_t item, last;  // an item that goes on (-1: none), and the last CTA that has a part
+  int32_t pad[2];
+};
+
+// Workspace: [workers] first parts | [CTAs][2] parts that cross CTAs | [CTAs] Cross.
+struct Room {
+  float* first;
+  float* cross;
+  Cross* about;
+};
+
+template <typename T, typename C, int D, int NT>
+__global__ void __launch_bounds__(Shape<C, D>::W * 32, 1)
+    k_paged_split(const __grid_constant__ Args a, const Room room) {
+  using X = Shape<C, D>;
+  using M = typename std::conditional<sizeof(C) == 1, __half, T>::type;  // the product's type
+  constexpr int W = X::W, S = X::S, KT = X::KT, PF = kPartFloats<D, NT>;
+  constexpr bool F8 = sizeof(C) == 1;
+  extern __shared__ __align__(128) char ring_all[];
+  __shared__ int64_t before[kMaxRequests / 32 + 1];
+  __shared__ Stage stages[W][S];
+  __shared__ int32_t p_item[2 * W], p_flag[2 * W];
+  __shared__ uint32_t p_rest;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int g = lane >> 2, t4 = lane & 3;
+  const int gq = a.Hq / a.Hkv, ngr = (gq + 8 * NT - 1) / (8 * NT), Hg = a.Hkv * ngr;
+
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  // tiles before each group of 32 requests
+  const int groups = (a.R + 31) / 32;
+  for (int i = warp; i < groups; i += W) {
+    const int r = i * 32 + lane;
+    int t0 = 0, t1 = 0;
+    if (r < a.R) tiles_of(a, a.lens[r], KT, t0, t1);
+    int64_t c = (int64_t)max(t1 - t0, 0) * Hg;
+#pragma unroll
+    for (int o = 16; o; o >>= 1) c += __shfl_xor_sync(~0u, c, o);
+    if (lane == 0) before[i + 1] = c;
+  }
+  if (threadIdx.x < 2 * W) p_item[threadIdx.x] = -1;
+  if (threadIdx.x == 0) { before[0] = 0; p_rest = 0; }
+  __syncthreads();
+  if (warp == 0) {
+    int64_t sum = 0;
+    for (int i = 0; i < groups; i += 32) {
+      int64_t c = i + lane < groups ? before[i + lane + 1] : 0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t y = __shfl_up_sync(~0u, c, o);
+        if (lane >= o) c += y;
+      }
+      if (i + lane < groups) before[i + lane + 1] = sum + c;
+      sum += __shfl_sync(~0u, c, 31);
+    }
+  }
+  __syncthreads();
+  const int64_t total = before[groups];
+  const int64_t workers = (int64_t)gridDim.x * W, worker = (int64_t)blockIdx.x * W + warp;
+  const int64_t quota = max((total + workers - 1) / workers, (int64_t)kMinTiles);
+  const int64_t begin = min(worker * quota, total), tiles = min(begin + quota, total) - begin;
+
+  // requests without keys; lengths that are out of range
+  for (int64_t r = worker; r < a.R; r += workers) {
+    const int32_t len = a.lens[r];
+    int t0, t1;
+    tiles_of(a, len, KT, t0, t1);
+    if (lane == 0 && (len < 0 || len > (int64_t)a.max_blocks * a.bs))
+      atomicExch(&g_device_error, 3);
+    if (t0 >= t1) {
+      for (int i = lane; i < a.Hq * (D / 8); i += 32) {
+        const int h = i / (D / 8), d = i % (D / 8);
+        *reinterpret_cast<uint4*>((T*)a.out + r * a.o_t + h * a.o_h + d * 8) =
+            make_uint4(0, 0, 0, 0);
+      }
+      if (a.lse)
+        for (int i = lane; i < a.Hq; i += 32) a.lse[r * a.Hq + i] = -INFINITY;
+    }
+  }
+
+  char* ring = ring_all + (size_t)warp * S * X::SB;
+  if (tiles > 0) {
+    Walk<C, D> w;
+    w.left = tiles;
+    {
+      int lo = 0, hi = groups;  // before[lo] <= begin < before[hi]
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (before[mid] <= begin) lo = mid;
+        else hi = mid;
+      }
+      w.g = lo;
+      w.load_group(a, lane);
+      int t0, t1;
+      tiles_of(a, w.glen, KT, t0, t1);
+      int64_t c = (int64_t)max(t1 - t0, 0) * Hg;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t y = __shfl_up_sync(~0u, c, o);
+        if (lane >= o) c += y;
+      }
+      const int64_t at = begin - before[lo];
+      // (a request that covers the tile: there is one unless the lengths change under the call)
+      const int l = max(__ffs(__ballot_sync(~0u, c > at)) - 1, 0);
+      const int64_t prev = __shfl_sync(~0u, c, l > 0 ? l - 1 : 0);
+      w.r = lo * 32 + l;
+      w.set_request(a);
+      const int64_t in = at - (l > 0 ? prev : 0), each = max(w.t1 - w.t0, 1);
+      w.h = (int)(in / each);
+      w.t = w.t0 + (int)(in - w.h * each);
+      w.fresh = true;
+      if (w.r < a.R && w.t < w.t1 && in >= 0 && w.h < Hg) w.look_up(a, lane);
+      else w.left = 0;
+    }
+#pragma unroll
+    for (int s = 0; s < S - 1; ++s) w.fetch(a, Hg, ngr, ring + s * X::SB, &stages[warp][s], lane);
+
+    uint32_t q[D / 16][2 * NT];
+    float o[NT][D / 16][4];
+    float m[NT], l[NT], sc[NT];
+    bool began = false;
+    const int lrow = lane & 7, lhalf = (lane >> 3) & 1, lsec = lane >> 4;
+    // where this lane points ldmatrix: 16-bit rows (keys by lsec, d's by lhalf), 8-bit the reverse
+    const int frow = (F8 ? lhalf : lsec) * 8 + lrow, fpiece = F8 ? lsec : lhalf;
+    const int fswz = swz<X::RB>(lrow);
+    int rs = 0, ws = S - 1;  // stage to read, stage to fill
+    for (int64_t i = 0; i < tiles; ++i) {
+      cp_async_wait<S - 2>();
+      __syncwarp();
+      w.fetch(a, Hg, ngr, ring + ws * X::SB, &stages[warp][ws], lane);
+      ws = ws + 1 == S ? 0 : ws + 1;
+      const Stage st = stages[warp][rs];
+      const uint32_t kb = smem_u32(ring + rs * X::SB), vb = kb + KT * X::RB;
+      rs = rs + 1 == S ? 0 : rs + 1;
+      if (st.r < 0) break;
+      const int sub = st.h % ngr, head0 = st.h / ngr * gq + sub * 8 * NT;
+      const int heads = min(8 * NT, gq - sub * 8 * NT);
+
+      if (st.flags & 1) {  // a new item: its queries, and nothing seen
+        began = st.flags & 2;
+        const T* qp = (const T*)a.q + st.r * a.q_t + head0 * a.q_h;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const int row = g + 8 * n;
+          const bool on = row < heads;
+          const T* qr = qp + (on ? row : 0) * a.q_h;
+          float fac = 1.0f;
+#pragma unroll
+          for (int j = 0; j < D / 16; ++j) {
+            if constexpr (F8) {  // pairs in the order of the keys' 8-bit pieces
+              const uint2 v = *reinterpret_cast<const uint2*>(qr + 16 * j + 4 * t4);
+              q[j][2 * n] = on ? v.x : 0;
+              q[j][2 * n + 1] = on ? v.y : 0;
+            } else {
+              const uint32_t* p = reinterpret_cast<const uint32_t*>(qr + 16 * j + 2 * t4);
+              q[j][2 * n] = on ? p[0] : 0;
+              q[j][2 * n + 1] = on ? p[4] : 0;
+            }
+          }
+          if constexpr (F8 && !std::is_same<T, __half>::value) {
+            // bf16 queries against keys widened to f16: the row is brought to [1, 2) by a
+            // power of two (put back on the scores), so that f16 holds all of a bf16's 8 bits
+            uint32_t top = 0;
+#pragma unroll
+            for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const uint32_t v = q[j][2 * n + e] & 0x7fff7fffu;
+                top = max(top, max(v & 0xffffu, v >> 16));
+              }
+            top = max(top, __shfl_xor_sync(~0u, top, 1));
+            top = max(top, __shfl_xor_sync(~0u, top, 2));
+            const uint32_t ex = min(max(top << 16 & 0x7f800000u, 0x00800000u), 0x7e800000u);
+            fac = __uint_as_float(ex);
+            const float inv = __uint_as_float(0x7f000000u - ex);
+#pragma unroll
+            for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const uint32_t v = q[j][2 * n + e];
+                q[j][2 * n + e] = pack2<__half>(__uint_as_float(v << 16) * inv,
+                                                __uint_as_float(v & 0xffff0000u) * inv);
+              }
+          }
+          sc[n] = a.scale2 * fac;
+          m[n] = -INFINITY;
+          l[n] = 0.0f;
+#pragma unroll
+          for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[n][j][e] = 0.0f;
+        }
+      }
+
+      // scores: rows = heads, columns = keys
+      float s[KT / 8][4];
+#pragma unroll
+      for (int n = 0; n < KT / 8; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[n][e] = 0.0f;
+#pragma unroll
+      for (int k2 = 0; k2 < KT / 16; ++k2) {
+        const uint32_t rowp = kb + (k2 * 16 + frow) * X::RB;
+#pragma unroll
+        for (int j = 0; j < D / 16; j += F8 ? 2 : 1) {
+          uint32_t b[4];
+          if constexpr (F8) {
+            ldm_x4(b, rowp + (((j + fpiece) ^ fswz) << 4));
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              const uint32_t* aq = q[j + (u >> 1)];
+              mma16816<M>(s[2 * k2 + (u & 1)], aq[0], NT == 2 ? aq[2 * NT - 2] : 0u, aq[1],
+                          NT == 2 ? aq[2 * NT - 1] : 0u, f16x2_lo(b[u]), f16x2_hi(b[u]));
+            }
+          } else {
+            ldm_x4(b, rowp + (((2 * j + fpiece) ^ fswz) << 4));
+            const uint32_t* aq = q[j];
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+              mma16816<M>(s[2 * k2 + u], aq[0], NT == 2 ? aq[2 * NT - 2] : 0u, aq[1],
+                          NT == 2 ? aq[2 * NT - 1] : 0u, b[2 * u], b[2 * u + 1]);
+          }
+        }
+      }
+
+      // softmax over the keys, per head
+      const bool all = st.mask == (KT == 32 ? ~0u : 0xffffu);
+      bool grew = false;
+      float base[NT], c[NT];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float top = m[n];
+#pragma unroll
+        for (int k = 0; k < KT / 8; ++k)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float v = s[k][2 * n + e] * sc[n];
+            if (!all && !(st.mask >> (8 * k + 2 * t4 + e) & 1)) v = -INFINITY;
+            s[k][2 * n + e] = v;
+            top = fmaxf(top, v);
+          }
+        top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
+        base[n] = top == -INFINITY ? 0.0f : top;
+        c[n] = exp2f(m[n] - base[n]);
+        grew |= top > m[n];
+        m[n] = top;
+      }
+      if (__any_sync(~0u, grew)) {  // a maximum rose: what was summed shrinks
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          l[n] *= c[n];
+          const float c0 = __shfl_sync(~0u, c[n], 8 * t4), c1 = __shfl_sync(~0u, c[n], 8 * t4 + 4);
+#pragma unroll
+          for (int j = 0; j < D / 16; ++j) {
+            o[n][j][0] *= c0;
+            o[n][j][1] *= c1;
+            o[n][j][2] *= c0;
+            o[n][j][3] *= c1;
+          }
+        }
+      }
+      // the weights enter the second product as two pieces of the 16-bit type: one piece
+      // alone would be off by as much as the output's own rounding (2^-9 for bf16, 2^-12 for
+      // f16), and the tensor pipe is idle most of the time
+      uint32_t ph[NT][KT / 8], pl[NT][KT / 8];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int k = 0; k < KT / 8; ++k) {
+          const float x = exp2f(s[k][2 * n] - base[n]), y = exp2f(s[k][2 * n + 1] - base[n]);
+          l[n] += x + y;
+          ph[n][k] = pack2<M>(x, y);
+          const float2 w = unpack2<M>(ph[n][k]);
+          pl[n][k] = pack2<M>(x - w.x, y - w.y);
+        }
+
+      // values: rows = d's, columns = heads
+#pragma unroll
+      for (int k2 = 0; k2 < KT / 16; ++k2) {
+        const uint32_t rowp = vb + (k2 * 16 + frow) * X::RB;
+#pragma unroll
+        for (int j = 0; j < D / 16; j += F8 ? 2 : 1) {
+          uint32_t v[4];
+          if constexpr (F8) {
+            ldm_x4_t(v, rowp + (((j + fpiece) ^ fswz) << 4));
+#pragma unroll
+            for (int u = 0; u < 4; ++u) v[u] = __byte_perm(v[u], 0, 0x3120);
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+#pragma unroll
+              for (int n = 0; n < NT; ++n) {
+                const uint32_t a0 = f16x2_lo(v[2 * u]), a1 = f16x2_hi(v[2 * u]);
+                const uint32_t a2 = f16x2_lo(v[2 * u + 1]), a3 = f16x2_hi(v[2 * u + 1]);
+                mma16816<M>(o[n][j + u], a0, a1, a2, a3, ph[n][2 * k2], ph[n][2 * k2 + 1]);
+                mma16816<M>(o[n][j + u], a0, a1, a2, a3, pl[n][2 * k2], pl[n][2 * k2 + 1]);
+              }
+          } else {
+            ldm_x4_t(v, rowp + (((2 * j + fpiece) ^ fswz) << 4));
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              mma16816<M>(o[n][j], v[0], v[1], v[2], v[3], ph[n][2 * k2], ph[n][2 * k2 + 1]);
+              mma16816<M>(o[n][j], v[0], v[1], v[2], v[3], pl[n][2 * k2], pl[n][2 * k2 + 1]);
+            }
+          }
+        }
+      }
+
+      const bool ends = st.flags & 4;
+      if (ends || i == tiles - 1) {  // the end of this warp's part of the item
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          l[n] += __shfl_xor_sync(~0u, l[n], 1);
+          l[n] += __shfl_xor_sync(~0u, l[n], 2);
+        }
+        if (began && ends) {
+          T* out = (T*)a.out + st.r * a.o_t + head0 * a.o_h;
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const float inv = l[n] == 0.0f ? 0.0f : a.v_scale / l[n];
+            const float i0 = __shfl_sync(~0u, inv, 8 * t4), i1 = __shfl_sync(~0u, inv, 8 * t4 + 4);
+#pragma unroll
+            for (int j = 0; j < D / 16; ++j)
+              store_fragment<T, C>(out, a.o_h, heads, n, j, lane,
+                                   make_float4(o[n][j][0] * i0, o[n][j][1] * i1, o[n][j][2] * i0,
+                                               o[n][j][3] * i1));
+            if (a.lse && t4 == 0 && g + 8 * n < heads)
+              a.lse[(int64_t)st.r * a.Hq + head0 + g + 8 * n] = lse_of(m[n], l[n]);
+          }
+        } else {
+          // a part: the first of several is put aside in the workspace, the last one in this
+          // warp's ring, which is then free
+          const bool last = i == tiles - 1;
+          if (last) {
+            cp_async_wait<0>();
+            __syncwarp();
+          }
+          float* to = last ? reinterpret_cast<float*>(ring) : room.first + worker * PF;
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int j = 0; j < D / 16; ++j)
+              reinterpret_cast<float4*>(to)[(n * (D / 16) + j) * 32 + lane] =
+                  make_float4(o[n][j][0], o[n][j][1], o[n][j][2], o[n][j][3]);
+            if (t4 == 0) {
+              to[NT * 8 * D + g + 8 * n] = m[n];
+              to[NT * 8 * (D + 1) + g + 8 * n] = l[n];
+            }
+          }
+          if (lane == 0) {
+            const int e = 2 * warp + (last ? 1 : 0);
+            p_item[e] = st.r * Hg + st.h;
+            p_flag[e] = (began ? 1 : 0) | (ends ? 2 : 0);
+            if (last && !ends && warp == W - 1) p_rest = st.flags >> 3;
+          }
+        }
+      }
+    }
+  }
+  cp_async_wait<0>();
+  __syncthreads();
+
+  // Join the CTA's own parts.  Parts of one item are neighbours in the order of the warps; a
+  // run that lacks the item's first or last tile crosses into another CTA.
+  Cross cross{-1, 0, {0, 0}};
+  for (int e0 = 0; e0 < 2 * W;) {
+    const int item = p_item[e0];
+    if (item < 0) { ++e0; continue; }
+    int e1 = e0, tail = e0;
+    for (int e = e0; e < 2 * W && (p_item[e] == item || p_item[e] < 0); ++e)
+      if (p_item[e] == item) { tail = e; e1 = e + 1; }
+    const bool has0 = p_flag[e0] & 1, has1 = p_flag[tail] & 2;
+    const int r = item / Hg, h = item - r * Hg, sub = h % ngr, head0 = h / ngr * gq + sub * 8 * NT;
+    const int heads = min(8 * NT, gq - sub * 8 * NT);
+    auto part = [&](int e) {
+      return e & 1 ? reinterpret_cast<const float*>(ring_all + (size_t)(e >> 1) * S * X::SB)
+                   : room.first + ((int64_t)blockIdx.x * W + (e >> 1)) * PF;
+    };
+    float* to = room.cross + ((int64_t)blockIdx.x * 2 + (has0 ? 1 : 0)) * PF;
+    for (int f = warp; f < NT * (D / 16); f += W) {
+      const int n = f / (D / 16), j = f % (D / 16), hh = n * 8 + 2 * t4;
+      float m0 = -INFINITY, m1 = -INFINITY;
+      for (int e = e0; e < e1; ++e)
+        if (p_item[e] == item) {
+          const float* p = part(e) + NT * 8 * D;
+          m0 = fmaxf(m0, p[hh]);
+          m1 = fmaxf(m1, p[hh + 1]);
+        }
+      float4 c = make_float4(0, 0, 0, 0);
+      float l0 = 0, l1 = 0;
+      for (int e = e0; e < e1; ++e)
+        if (p_item[e] == item) {
+          const float* p = part(e);
+          const float w0 = weight(p[NT * 8 * D + hh], m0), w1 = weight(p[NT * 8 * D + hh + 1], m1);
+          const float4 v = reinterpret_cast<const float4*>(p)[f * 32 + lane];
+          c.x += w0 * v.x;
+          c.y += w1 * v.y;
+          c.z += w0 * v.z;
+          c.w += w1 * v.w;
+          l0 += w0 * p[NT * 8 * (D + 1) + hh];
+          l1 += w1 * p[NT * 8 * (D + 1) + hh + 1];
+        }
+      if (has0 && has1) {
+        const float i0 = l0 == 0.0f ? 0.0f : a.v_scale / l0;
+        const float i1 = l1 == 0.0f ? 0.0f : a.v_scale / l1;
+        store_fragment<T, C>((T*)a.out + r * a.o_t + head0 * a.o_h, a.o_h, heads, n, j, lane,
+                             make_float4(c.x * i0, c.y * i1, c.z * i0, c.w * i1));
+        if (a.lse && j == 0 && g == 0) {
+          if (hh < heads) a.lse[(int64_t)r * a.Hq + head0 + hh] = lse_of(m0, l0);
+          if (hh + 1 < heads) a.lse[(int64_t)r * a.Hq + head0 + hh + 1] = lse_of(m1, l1);
+        }
+      } else {
+        reinterpret_cast<float4*>(to)[f * 32 + lane] = c;
+        if (j == 0 && g == 0) {
+          to[NT * 8 * D + hh] = m0;
+          to[NT * 8 * D + hh + 1] = m1;
+          to[NT * 8 * (D + 1) + hh] = l0;
+          to[NT * 8 * (D + 1) + hh + 1] = l1;
+        }
+      }
+    }
+    if (has0 && !has1) {
+      const int64_t end = min(total, (int64_t)(blockIdx.x + 1) * W * quota);
+      cross.item = item;
+      cross.last = (int)((end + p_rest - 1) / (W * quota));
+    }
+    e0 = e1;
+  }
+  if (threadIdx.x == 0) room.about[blockIdx.x] = cross;
+}
+
+// Joins the items whose parts lie in several CTAs.  Block (c, f): the item that
+// starts in CTA c and goes on, its fragment f; the warps share the parts.
+constexpr int kJoinWarps = 8;
+
+template <typename T, typename C, int D, int NT>
+__global__ void __launch_bounds__(kJoinWarps * 32)
+    k_paged_join(const __grid_constant__ Args a, const Room room) {
+  constexpr int PF = kPartFloats<D, NT>;
+  __shared__ float4 sc[kJoinWarps][32];
+  __shared__ float sm[kJoinWarps][32][2], sl[kJoinWarps][32][2];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int gq = a.Hq / a.Hkv, ngr = (gq + 8 * NT - 1) / (8 * NT), Hg = a.Hkv * ngr;
+  const int cta = blockIdx.x, f = blockIdx.y;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int item = __ldcg(&room.about[cta].item), last = __ldcg(&room.about[cta].last);
+  if (item < 0) return;
+  const int n = f / (D / 16), j = f % (D / 16), hh = n * 8 + 2 * (lane & 3);
+  float4 c = make_float4(0, 0, 0, 0);
+  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0, l1 = 0;
+#pragma unroll 4
+  for (int b = cta + warp; b <= last; b += kJoinWarps) {
+    const float* p = room.cross + ((int64_t)b * 2 + (b == cta ? 1 : 0)) * PF;
+    const float2 pm = __ldcg(reinterpret_cast<const float2*>(p + NT * 8 * D + hh));
+    const float2 pl = __ldcg(reinterpret_cast<const float2*>(p + NT * 8 * (D + 1) + hh));
+    const float4 v = __ldcg(reinterpret_cast<const float4*>(p) + f * 32 + lane);
+    const float t0 = fmaxf(m0, pm.x), t1 = fmaxf(m1, pm.y);
+    const float a0 = weight(m0, t0), a1 = weight(m1, t1);
+    const float b0 = weight(pm.x, t0), b1 = weight(pm.y, t1);
+    c.x = c.x * a0 + v.x * b0;
+    c.y = c.y * a1 + v.y * b1;
+    c.z = c.z * a0 + v.z * b0;
+    c.w = c.w * a1 + v.w * b1;
+    l0 = l0 * a0 + pl.x * b0;
+    l1 = l1 * a1 + pl.y * b1;
+    m0 = t0;
+    m1 = t1;
+  }
+  sc[warp][lane] = c;
+  sm[warp][lane][0] = m0;
+  sm[warp][lane][1] = m1;
+  sl[warp][lane][0] = l0;
+  sl[warp][lane][1] = l1;
+  __syncthreads();
+  if (warp) return;
+  for (int w = 1; w < kJoinWarps; ++w) {
+    m0 = fmaxf(m0, sm[w][lane][0]);
+    m1 = fmaxf(m1, sm[w][lane][1]);
+  }
+  c = make_float4(0, 0, 0, 0);
+  l0 = l1 = 0;
+  for (int w = 0; w < kJoinWarps; ++w) {
+    const float w0 = weight(sm[w][lane][0], m0), w1 = weight(sm[w][lane][1], m1);
+    const float4 v = sc[w][lane];
+    c.x += w0 * v.x;
+    c.y += w1 * v.y;
+    c.z += w0 * v.z;
+    c.w += w1 * v.w;
+    l0 += w0 * sl[w][lane][0];
+    l1 += w1 * sl[w][lane][1];
+  }
+  const int r = item / Hg, h = item - r * Hg, sub = h % ngr, head0 = h / ngr * gq + sub * 8 * NT;
+  const int heads = min(8 * NT, gq - sub * 8 * NT);
+  const float i0 = l0 == 0.0f ? 0.0f : a.v_scale / l0, i1 = l1 == 0.0f ? 0.0f : a.v_scale / l1;
+  store_fragment<T, C>((T*)a.out + r * a.o_t + head0 * a.o_h, a.o_h, heads, n, j, lane,
+                       make_float4(c.x * i0, c.y * i1, c.z * i0, c.w * i1));
+  if (a.lse && j == 0 && (lane >> 2) == 0) {
+    if (hh < heads) a.lse[(int64_t)r * a.Hq + head0 + hh] = lse_of(m0, l0);
+    if (hh + 1 < heads) a.lse[(int64_t)r * a.Hq + head0 + hh + 1] = lse_of(m1, l1);
+  }
+}
+
+inline int head_tiles(int64_t Hq, int64_t Hkv, int64_t D) { return Hq / Hkv > 8 && D <= 128 ? 2 : 1; }
+
+// Floats of one partial result.
+inline int64_t part_floats(int64_t Hq, int64_t Hkv, int64_t D) {
+  return head_tiles(Hq, Hkv, D) * 8 * (D + 2);
+}
+
+template <typename T, typename C, int D, int NT>
+int launch(const Args& a, void* workspace, cudaStream_t st) {
+  using X = Shape<C, D>;
+  constexpr int PF = kPartFloats<D, NT>;
+  auto split = k_paged_split<T, C, D, NT>;
+  RB_CUDA(cudaFuncSetAttribute(split, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               (int)X::kSmem));
+  // no more CTAs than the tables' room has tiles for
+  const int ngr = (a.Hq / a.Hkv + 8 * NT - 1) / (8 * NT);
+  const int64_t room_tiles = ((int64_t)a.max_blocks * a.bs + X::KT - 1) / X::KT + 1;
+  const int64_t most = (room_tiles * a.R * a.Hkv * ngr + kMinTiles * X::W - 1) / (kMinTiles * X::W);
+  const int sms = num_sms();
+  const int grid = (int)std::min<int64_t>(sms, std::max<int64_t>(most, 1));
+  Room room;
+  room.first = static_cast<float*>(workspace);
+  room.cross = room.first + (int64_t)sms * X::W * PF;
+  room.about = reinterpret_cast<Cross*>(room.cross + (int64_t)sms * 2 * PF);
+  split<<<grid, X::W * 32, X::kSmem, st>>>(a, room);
+  RB_LAUNCH_CHECK();
+  if (grid == 1) return REMORA_B200_OK;  // nothing crosses
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid, NT * (D / 16));
+  cfg.blockDim = dim3(kJoinWarps * 32);
+  cfg.stream = st;
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  RB_CUDA(cudaLaunchKernelEx(&cfg, k_paged_join<T, C, D, NT>, a, room));
+  return REMORA_B200_OK;
+}
+
+template <typename T, typename C>
+int launch_shape(const Args& a, void* ws, cudaStream_t st) {
+  const int nt = head_tiles(a.Hq, a.Hkv, a.D);
+  if (a.D == 64) return nt == 2 ? launch<T, C, 64, 2>(a, ws, st) : launch<T, C, 64, 1>(a, ws, st);
+  if (a.D == 128)
+    return nt == 2 ? launch<T, C, 128, 2>(a, ws, st) : launch<T, C, 128, 1>(a, ws, st);
+  return launch<T, C, 256, 1>(a, ws, st);
 }
 
 inline bool shape_ok(int64_t R, int64_t Hq, int64_t Hkv, int64_t D) {
@@ -93,7 +838,10 @@ inline bool shape_ok(int64_t R, int64_t Hq, int64_t Hkv, int64_t D) {
 
 extern "C" size_t remora_b200_paged_attention_workspace_bytes(int64_t R, int64_t Hq, int64_t Hkv,
                                                               int64_t D) {
-  return rb::paged::shape_ok(R, Hq, Hkv, D) ? 16 : 0;
+  using namespace rb::paged;
+  if (!shape_ok(R, Hq, Hkv, D)) return 0;
+  const int64_t sms = rb::num_sms();
+  return (size_t)(sms * (8 + 2) * part_floats(Hq, Hkv, D) * 4 + sms * (int64_t)sizeof(Cross));
 }
 
 extern "C" int remora_b200_paged_attention(
@@ -143,17 +891,12 @@ extern "C" int remora_b200_paged_attention(
   Args a{q, k_cache, v_cache, block_table, lens, out, lse, q_t, q_h, out_t, out_h, kc_block,
          kc_token, kc_head, vc_block, vc_token, vc_head, ld_table, window, (int32_t)R, (int32_t)Hq,
          (int32_t)Hkv, (int32_t)D, (int32_t)num_blocks, (int32_t)block_size, (int32_t)max_blocks,
-         scale * 1.4426950408889634f, k_scale, v_scale};
-  const int grid = (int)((R * Hq + 3) / 4);
+         scale * 1.4426950408889634f * k_scale, v_scale};
   cudaStream_t st = as_stream(stream);
   const bool f8 = cache_dtype == REMORA_B200_E4M3;
-  if (dtype == REMORA_B200_BF16) {
-    if (f8) k_paged_simple<__nv_bfloat16, __nv_fp8_e4m3><<<grid, 128, 0, st>>>(a);
-    else k_paged_simple<__nv_bfloat16, __nv_bfloat16><<<grid, 128, 0, st>>>(a);
-  } else {
-    if (f8) k_paged_simple<__half, __nv_fp8_e4m3><<<grid, 128, 0, st>>>(a);
-    else k_paged_simple<__half, __half><<<grid, 128, 0, st>>>(a);
-  }
-  RB_LAUNCH_CHECK();
-  return REMORA_B200_OK;
+  if (dtype == REMORA_B200_BF16)
+    return f8 ? launch_shape<__nv_bfloat16, __nv_fp8_e4m3>(a, workspace, st)
+              : launch_shape<__nv_bfloat16, __nv_bfloat16>(a, workspace, st);
+  return f8 ? launch_shape<__half, __nv_fp8_e4m3>(a, workspace, st)
+            : launch_shape<__half, __half>(a, workspace, st);
 }

@@ -13,7 +13,7 @@ def half_step(dtype):
 # ------------------------------------------------------------- block tables
 def block_table(lens, new, table, free, count, bs, max_tokens):
     """The step of kv_block_table, request by request."""
-    lens, new, table, free = (np.array(x, dtype=np.int64) for x in (lens, new, table, free))
+    lens, new, table, free = (np.array(np.asarray(x), dtype=np.int64) for x in (lens, new, table, free))
     R, max_blocks = table.shape
     room = max_blocks * bs
     need_blocks = lambda n: -(-n // bs)  # noqa: E731
