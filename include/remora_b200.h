@@ -213,13 +213,22 @@ int remora_b200_attention_fwd_bf16(const void* q, const void* k, const void* v, 
  * its slot, position and request: -1, 0, r for a token of a refused request
  * and -1, 0, -1 behind the last token.  Deterministic; the same call on the
  * same lens and free_count gives the same result again. */
-int remora_b200_kv_block_table(const int32_t* lens, const int32_t* new_tokens, int64_t R,
-                               int32_t* block_table, int64_t ld_table, int64_t max_blocks,
-                               int32_t* free_blocks, const int32_t* free_count,
-                               int64_t num_blocks, int64_t block_size, int32_t* lens_out,
-                               int32_t* free_count_out, int32_t* cu_tokens, int32_t* slots,
-                               int32_t* positions, int32_t* requests, int64_t max_tokens,
-                               int32_t* status, void* stream);
+typedef struct remora_b200_kv_block_table_args {
+  const int32_t* lens;
+  const int32_t* new_tokens;
+  int32_t* block_table;
+  int32_t* free_blocks;
+  const int32_t* free_count;
+  int32_t* lens_out;
+  int32_t* free_count_out;
+  int32_t* cu_tokens;
+  int32_t* slots;
+  int32_t* positions;
+  int32_t* requests;
+  int32_t* status;
+  int64_t R, ld_table, max_blocks, num_blocks, block_size, max_tokens;
+} remora_b200_kv_block_table_args;
+int remora_b200_kv_block_table(const remora_b200_kv_block_table_args* args, void* stream);
 
 /* Rotary positions: pair i < rot / 2 of each head turns by the angle
  * p * freq[i], p = positions[axis_of[i] * ld_pos + b * S + s], so that
@@ -233,11 +242,17 @@ int remora_b200_kv_block_table(const int32_t* lens, const int32_t* new_tokens, i
  * D <= 1024; n_axes <= 8.  Angles are exact to 2^-25 of a quarter turn at
  * every 32-bit position.  Any strides; sizes, strides and bases that are
  * multiples of 8 elements (and 16 bytes) move 8 pairs at a time. */
-int remora_b200_rope(const void* x, void* out, int dtype, int64_t B, int64_t S, int64_t H,
-                     int64_t D, int64_t x_b, int64_t x_s, int64_t x_h, int64_t out_b,
-                     int64_t out_s, int64_t out_h, const int32_t* positions, int64_t ld_pos,
-                     int n_axes, const double* freq, const int32_t* axis_of, int64_t rot,
-                     int interleaved, int inverse, void* stream);
+typedef struct remora_b200_rope_args {
+  const void* x;
+  void* out;
+  const int32_t* positions;
+  const double* freq;
+  const int32_t* axis_of;
+  int64_t B, S, H, D, rot;
+  int64_t x_b, x_s, x_h, out_b, out_s, out_h, ld_pos;
+  int dtype, n_axes, interleaved, inverse;
+} remora_b200_rope_args;
+int remora_b200_rope(const remora_b200_rope_args* args, void* stream);
 
 /* The same rotation of q and k, and the append of k and v to the cache, in
  * one pass: q_out[t] = rope(q[t]), cache row of slots[t] = rope(k[t]) and
@@ -245,18 +260,32 @@ int remora_b200_rope(const void* x, void* out, int dtype, int64_t B, int64_t S, 
  * of one projection are taken as they lie; q_out may be q); dtype BF16 or
  * F16; cache_dtype is dtype or E4M3 (then with the scales k_scale and
  * v_scale, else both must be 1).  A token whose slot is -1 writes no cache
- * row.  The rest as remora_b200_rope. */
-int remora_b200_rope_kv_append(
-    const void* q, const void* k, const void* v, void* q_out, int dtype, int64_t T, int64_t Hq,
-    int64_t Hkv, int64_t D, int64_t q_t, int64_t q_h, int64_t k_t, int64_t k_h, int64_t v_t,
-    int64_t v_h, int64_t qo_t, int64_t qo_h, const int32_t* positions, int64_t ld_pos, int n_axes,
-    const double* freq, const int32_t* axis_of, int64_t rot, int interleaved,
-    const int32_t* slots, void* k_cache, void* v_cache, int cache_dtype, int64_t num_blocks,
-    int64_t block_size, int64_t kc_block, int64_t kc_token, int64_t kc_head, int64_t vc_block,
-    int64_t vc_token, int64_t vc_head, float k_scale, float v_scale, void* stream);
+ * row.  Two tokens of one slot leave one row or the other in each element.
+ * kc_* and vc_*: the caches' strides of block, token and head.  The rest as
+ * remora_b200_rope. */
+typedef struct remora_b200_rope_kv_append_args {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* q_out;
+  void* k_cache;
+  void* v_cache;
+  const int32_t* positions;
+  const int32_t* slots;
+  const double* freq;
+  const int32_t* axis_of;
+  int64_t T, Hq, Hkv, D, rot;
+  int64_t q_t, q_h, k_t, k_h, v_t, v_h, q_out_t, q_out_h, ld_pos;
+  int64_t num_blocks, block_size;
+  int64_t kc_block, kc_token, kc_head, vc_block, vc_token, vc_head;
+  float k_scale, v_scale;
+  int dtype, cache_dtype, n_axes, interleaved;
+} remora_b200_rope_kv_append_args;
+int remora_b200_rope_kv_append(const remora_b200_rope_kv_append_args* args, void* stream);
 
-/* Bytes of device workspace remora_b200_paged_attention needs (0 for sizes
- * it rejects).  Calls that may overlap on the GPU need one each. */
+/* Bytes of device workspace remora_b200_paged_attention needs on the current
+ * device (0 for sizes it rejects).  Calls that may overlap on the GPU need
+ * one each; what it holds before a call does not matter. */
 size_t remora_b200_paged_attention_workspace_bytes(int64_t R, int64_t Hq, int64_t Hkv,
                                                    int64_t D);
 
@@ -267,19 +296,31 @@ size_t remora_b200_paged_attention_workspace_bytes(int64_t R, int64_t Hq, int64_
  * [R][Hq], may be NULL) = the natural logarithm of the softmax's sum.  A
  * request without keys, or whose every score is -infinity, gives zeros and
  * lse = -infinity.  Cache rows past a request's length are never used,
- * whatever they hold.  q and out: dtype BF16 or F16, [R][Hq][D] by strides
- * (out must not be q); caches: dtype, or E4M3 with scales.  D in {64, 128,
- * 256}, Hq % Hkv == 0, R <= 8192; 16-byte aligned bases, strides of whole 16
+ * whatever they hold; an infinity or NaN in a used row of values makes its
+ * column NaN.  q and out: dtype BF16 or F16, [R][Hq][D] by strides (out must
+ * not be q); caches: dtype, or E4M3 with scales.  D in {64, 128, 256},
+ * Hq % Hkv == 0, R <= 8192; 16-byte aligned bases, strides of whole 16
  * bytes.  The call is two launches: the split over the keys, then the join
  * of what was split. */
-int remora_b200_paged_attention(
-    const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table,
-    const int32_t* lens, void* out, float* lse, int dtype, int cache_dtype, int64_t R, int64_t Hq,
-    int64_t Hkv, int64_t D, int64_t q_t, int64_t q_h, int64_t out_t, int64_t out_h,
-    int64_t num_blocks, int64_t block_size, int64_t kc_block, int64_t kc_token, int64_t kc_head,
-    int64_t vc_block, int64_t vc_token, int64_t vc_head, int64_t ld_table, int64_t max_blocks,
-    float scale, int64_t window, float k_scale, float v_scale, void* workspace,
-    size_t workspace_bytes, void* stream);
+typedef struct remora_b200_paged_attention_args {
+  const void* q;
+  const void* k_cache;
+  const void* v_cache;
+  const int32_t* block_table;
+  const int32_t* lens;
+  void* out;
+  float* lse;
+  void* workspace;
+  size_t workspace_bytes;
+  int64_t R, Hq, Hkv, D;
+  int64_t q_t, q_h, out_t, out_h;
+  int64_t num_blocks, block_size;
+  int64_t kc_block, kc_token, kc_head, vc_block, vc_token, vc_head;
+  int64_t ld_table, max_blocks, window;
+  float scale, k_scale, v_scale;
+  int dtype, cache_dtype;
+} remora_b200_paged_attention_args;
+int remora_b200_paged_attention(const remora_b200_paged_attention_args* args, void* stream);
 
 /* ------------------------------------------------------------------------
  * MoE layer (mlir/stablehlo/mixtral_moe_layer.mlir:8-68; simple_moe.mlir:16-35)

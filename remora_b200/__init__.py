@@ -16,7 +16,9 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 import os
+import struct
 from typing import NamedTuple
 
 import torch
@@ -79,17 +81,11 @@ _SIGNATURES = {
     "remora_b200_gemm_bf16": ([P, P, P, I64, I64, I64, I64, I64, I64, I64, I64, I64, I64, I, P], I),
     "remora_b200_gemm_f32_exact": ([P, P, P, I64, I64, I64, I64, I64, I64, I, P], I),
     "remora_b200_attention_fwd_bf16": ([P, P, P, P, I64, I64, I64, I64, I, F, P], I),
-    "remora_b200_kv_block_table": ([P, P, I64, P, I64, I64, P, P, I64, I64, P, P, P, P, P, P, I64,
-                                    P, P], I),
-    "remora_b200_rope": ([P, P, I, I64, I64, I64, I64, I64, I64, I64, I64, I64, I64, P, I64, I, P,
-                          P, I64, I, I, P], I),
-    "remora_b200_rope_kv_append": ([P, P, P, P, I, I64, I64, I64, I64, I64, I64, I64, I64, I64,
-                                    I64, I64, I64, P, I64, I, P, P, I64, I, P, P, P, I, I64, I64,
-                                    I64, I64, I64, I64, I64, I64, F, F, P], I),
+    "remora_b200_kv_block_table": ([ctypes.c_char_p, P], I),
+    "remora_b200_rope": ([ctypes.c_char_p, P], I),
+    "remora_b200_rope_kv_append": ([ctypes.c_char_p, P], I),
     "remora_b200_paged_attention_workspace_bytes": ([I64, I64, I64, I64], ctypes.c_size_t),
-    "remora_b200_paged_attention": ([P, P, P, P, P, P, P, I, I, I64, I64, I64, I64, I64, I64, I64,
-                                     I64, I64, I64, I64, I64, I64, I64, I64, I64, I64, I64, F,
-                                     I64, F, F, P, ctypes.c_size_t, P], I),
+    "remora_b200_paged_attention": ([ctypes.c_char_p, P], I),
     "remora_b200_moe_router_topk_bf16": ([P, P, I64, I64, I, I, P, P, P], I),
     "remora_b200_moe_dispatch_workspace_bytes": ([I64, I, I], ctypes.c_size_t),
     "remora_b200_moe_dispatch": ([P, I64, I, I, P, P, P, P, P, ctypes.c_size_t, P], I),
@@ -166,6 +162,12 @@ def _check(rc: int) -> None:
 
 def _stream(t: torch.Tensor) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
+
+
+def _raw_stream(device_index: int) -> int:
+    """torch's current stream on a device as its cudaStream_t (without the Stream object that
+    torch.cuda.current_stream makes: 1 us against 4 on the latency-bound calls)."""
+    return torch._C._cuda_getCurrentRawStream(device_index)
 
 
 def _dev(*ts: torch.Tensor) -> None:
@@ -306,22 +308,34 @@ _DTYPES = {torch.bfloat16: BF16, torch.float16: F16, torch.float32: F32,
            torch.float8_e4m3fn: E4M3}
 
 
+# The argument structs of the C ABI (their fields in order), packed in one go: ctypes converts
+# arguments one at a time, which for these calls took longer than the launch.
+_BLOCK_TABLE_ARGS = struct.Struct("=12Q6q")
+_ROPE_ARGS = struct.Struct("=5Q12q4i")
+_APPEND_ARGS = struct.Struct("=10Q22q2f4i")
+_ATTENTION_ARGS = struct.Struct("=9Q19q3f2i4x")
+
+_HERE_ALREADY = contextlib.nullcontext()
+
+
 def _on(*ts: torch.Tensor):
-    """Checks that all tensors are on one CUDA device and makes it current for
-    the launch (a context manager; no cost where it is current already)."""
+    """Checks that all tensors are on one CUDA device.  Returns a context manager that makes it
+    current for the launch (nothing to do where it is current already) and its index."""
     dev = ts[0].device
+    if dev.type != "cuda":
+        raise ValueError("remora_b200 operates on CUDA tensors only (no CPU fallback)")
     for t in ts:
-        if not t.is_cuda:
-            raise ValueError("remora_b200 operates on CUDA tensors only (no CPU fallback)")
         if t.device != dev:
+            if not t.is_cuda:
+                raise ValueError("remora_b200 operates on CUDA tensors only (no CPU fallback)")
             raise ValueError(f"tensors are on different devices: {dev} and {t.device}")
-    if dev.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(dev)
+    if dev.index == torch._C._cuda_getDevice():
+        return _HERE_ALREADY, dev.index
+    return torch.cuda.device(dev), dev.index
 
 
 def _ints(name: str, t: torch.Tensor, shape: tuple) -> None:
-    if t.dtype != torch.int32 or not t.is_contiguous() or tuple(t.shape) != shape:
+    if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 tensor of shape {list(shape)}, got "
                          f"{t.dtype} {list(t.shape)}")
 
@@ -356,32 +370,34 @@ def kv_block_table(lens: torch.Tensor, new_tokens: torch.Tensor, block_table: to
         raise ValueError("kv_block_table takes lens [R], block_table [R, max_blocks] and "
                          "free_blocks [num_blocks]")
     R, N = lens.shape[0], max_tokens
-    if block_table.shape[0] != R or block_table.shape[1] < 1 or free_blocks.shape[0] < 1:
+    max_blocks, num_blocks = block_table.shape[1], free_blocks.shape[0]
+    if block_table.shape[0] != R or max_blocks < 1 or num_blocks < 1:
         raise ValueError("block_table must have a row of at least one block per request and "
                          "free_blocks at least one entry")
     _ints("lens", lens, (R,))
     _ints("new_tokens", new_tokens, (R,))
-    _ints("free_blocks", free_blocks, (free_blocks.shape[0],))
+    _ints("free_blocks", free_blocks, (num_blocks,))
     _ints("free_count", free_count, (1,))
-    if block_table.dtype != torch.int32 or block_table.stride(1) != 1:
+    if block_table.dtype != torch.int32 or \
+            (max_blocks != 1 and block_table.stride(1) != 1):
         raise ValueError("block_table must be int32 with adjacent entries of a row")
     if N < 0:
         raise ValueError("max_tokens must not be negative")
-    guard = _on(lens, new_tokens, block_table, free_blocks, free_count)
-    if out is None:
-        # one allocation, cut up: lens, cu_tokens, status, count and the tokens' rows
+    guard, index = _on(lens, new_tokens, block_table, free_blocks, free_count)
+    if out is None:  # one allocation, cut up
         sizes = (R, 1, R + 1, N, N, N, R)
-        out = KvStep(*torch.empty(sum(sizes), dtype=torch.int32, device=lens.device).split(sizes))
+        out = KvStep(*torch.empty(sum(sizes), dtype=torch.int32,
+                                  device=lens.device).split_with_sizes(sizes))
     else:
         for name, n in zip(KvStep._fields, (R, 1, R + 1, N, N, N, R)):
             _ints(name, getattr(out, name), (n,))
         _on(lens, *out)
     with guard:
-        _check(lib().remora_b200_kv_block_table(
-            lens.data_ptr(), new_tokens.data_ptr(), R, block_table.data_ptr(),
-            block_table.stride(0) if R > 1 else block_table.shape[1], block_table.shape[1],
-            free_blocks.data_ptr(), free_count.data_ptr(), free_blocks.shape[0], block_size,
-            *(t.data_ptr() for t in out[:6]), N, out.status.data_ptr(), _stream(lens)))
+        _check(lib().remora_b200_kv_block_table(_BLOCK_TABLE_ARGS.pack(
+            lens.data_ptr(), new_tokens.data_ptr(), block_table.data_ptr(),
+            free_blocks.data_ptr(), free_count.data_ptr(), *[t.data_ptr() for t in out], R,
+            block_table.stride(0) if R > 1 else max_blocks, max_blocks, num_blocks, block_size, N),
+            _raw_stream(index)))
     return out
 
 
@@ -391,9 +407,9 @@ def _rope_plan(freq, axis_of, positions, tokens: tuple):
         raise ValueError("freq must be a host float64 tensor [rot / 2]")
     if positions.dtype != torch.int32:
         raise TypeError("positions must be int32")
-    if tuple(positions.shape) == tokens:
+    if positions.shape == tokens:
         n_axes = 1
-    elif positions.dim() == len(tokens) + 1 and tuple(positions.shape[1:]) == tokens:
+    elif positions.dim() == len(tokens) + 1 and positions.shape[1:] == tokens:
         n_axes = positions.shape[0]
     else:
         raise ValueError(f"positions must be [axes, *{list(tokens)}] or {list(tokens)}, got "
@@ -423,9 +439,8 @@ def rope(x: torch.Tensor, positions: torch.Tensor, freq: torch.Tensor,
         raise ValueError("rope takes x as [B, S, H, D] or [T, H, D]")
     if x.dtype not in (torch.bfloat16, torch.float16, torch.float32):
         raise TypeError(f"rope takes bf16, f16 or f32, got {x.dtype}")
-    n_axes, freq, axis_of, positions, rot = _rope_plan(freq, axis_of, positions,
-                                                       tuple(x.shape[:-2]))
-    guard = _on(x, positions) if out is None else _on(x, positions, out)
+    n_axes, freq, axis_of, positions, rot = _rope_plan(freq, axis_of, positions, x.shape[:-2])
+    guard, index = _on(x, positions, x if out is None else out)
     if out is None:
         out = torch.empty_like(x)
     elif out.shape != x.shape or out.dtype != x.dtype:
@@ -433,27 +448,32 @@ def rope(x: torch.Tensor, positions: torch.Tensor, freq: torch.Tensor,
     if x.stride(-1) != 1 or out.stride(-1) != 1:
         raise ValueError("the elements of a head must be adjacent")
     B, S = (x.shape[0], x.shape[1]) if x.dim() == 4 else (1, x.shape[0])
-    xs, os_ = ((t.stride() if t.dim() == 4 else (0,) + t.stride()) for t in (x, out))
+    xs, os_ = x.stride(), out.stride()
+    if x.dim() == 3:
+        xs, os_ = (0,) + xs, (0,) + os_
     with guard:
-        _check(lib().remora_b200_rope(
-            x.data_ptr(), out.data_ptr(), _DTYPES[x.dtype], B, S, x.shape[-2], x.shape[-1], *xs[:3],
-            *os_[:3], positions.data_ptr(), B * S, n_axes, freq.data_ptr(),
-            None if axis_of is None else axis_of.data_ptr(), rot, int(interleaved), int(inverse),
-            _stream(x)))
+        _check(lib().remora_b200_rope(_ROPE_ARGS.pack(
+            x.data_ptr(), out.data_ptr(), positions.data_ptr(), freq.data_ptr(),
+            0 if axis_of is None else axis_of.data_ptr(), B, S, x.shape[-2], x.shape[-1], rot,
+            *xs[:3], *os_[:3], B * S, _DTYPES[x.dtype], n_axes, interleaved, inverse),
+            _raw_stream(index)))
     return out
 
 
-def _cache(q, k_cache, v_cache, Hkv: int, D: int) -> int:
-    """Checks a pair of caches against q and gives their element type."""
-    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.shape[2:] != (Hkv, D):
+def _cache(q, k_cache, v_cache, Hkv: int, D: int) -> tuple:
+    """Checks a pair of caches against q; their element type, and their blocks and strides as
+    the C ABI takes them."""
+    shape = k_cache.shape
+    if len(shape) != 4 or shape != v_cache.shape or shape[2:] != (Hkv, D):
         raise ValueError(f"the caches must be [num_blocks, block_size, {Hkv}, {D}] of one shape, "
                          f"got {list(k_cache.shape)} and {list(v_cache.shape)}")
     if k_cache.dtype != v_cache.dtype or k_cache.dtype not in (q.dtype, torch.float8_e4m3fn):
         raise TypeError(f"the caches must be {q.dtype} or float8_e4m3fn, got {k_cache.dtype} and "
                         f"{v_cache.dtype}")
-    if k_cache.stride(3) != 1 or v_cache.stride(3) != 1:
+    ks, vs = k_cache.stride(), v_cache.stride()
+    if ks[3] != 1 or vs[3] != 1:
         raise ValueError("the elements of a cache row must be adjacent")
-    return _DTYPES[k_cache.dtype]
+    return _DTYPES[k_cache.dtype], (shape[0], shape[1], *ks[:3], *vs[:3])
 
 
 def rope_kv_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
@@ -476,30 +496,35 @@ def rope_kv_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions:
         raise TypeError("rope_kv_append takes q, k and v in bf16 or all in f16")
     T, Hq, D = q.shape
     Hkv = k.shape[1]
-    cdt = _cache(q, k_cache, v_cache, Hkv, D)
+    cdt, cdims = _cache(q, k_cache, v_cache, Hkv, D)
     n_axes, freq, axis_of, positions, rot = _rope_plan(freq, axis_of, positions, (T,))
     _ints("slots", slots, (T,))
-    guard = _on(q, k, v, positions, slots, k_cache, v_cache)
+    guard, index = _on(q, k, v, positions, slots, k_cache, v_cache)
     if q_out is None:
-        q_out = torch.empty((T, Hq, D), dtype=q.dtype, device=q.device)
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif q_out.shape != q.shape or q_out.dtype != q.dtype or q_out.device != q.device:
         raise ValueError("q_out must have q's shape, type and device")
-    if any(t.stride(2) != 1 for t in (q, k, v, q_out)):
+    qs, ks, vs, os_ = q.stride(), k.stride(), v.stride(), q_out.stride()
+    if qs[2] != 1 or ks[2] != 1 or vs[2] != 1 or os_[2] != 1:
         raise ValueError("the elements of a head must be adjacent")
     with guard:
-        _check(lib().remora_b200_rope_kv_append(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), q_out.data_ptr(), _DTYPES[q.dtype], T, Hq,
-            Hkv, D, q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
-            q_out.stride(0), q_out.stride(1), positions.data_ptr(), T, n_axes, freq.data_ptr(),
-            None if axis_of is None else axis_of.data_ptr(), rot, int(interleaved),
-            slots.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), cdt, k_cache.shape[0],
-            k_cache.shape[1], *k_cache.stride()[:3], *v_cache.stride()[:3], k_scale, v_scale,
-            _stream(q)))
+        _check(lib().remora_b200_rope_kv_append(_APPEND_ARGS.pack(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), q_out.data_ptr(), k_cache.data_ptr(),
+            v_cache.data_ptr(), positions.data_ptr(), slots.data_ptr(), freq.data_ptr(),
+            0 if axis_of is None else axis_of.data_ptr(), T, Hq, Hkv, D, rot, *qs[:2], *ks[:2],
+            *vs[:2], *os_[:2], T, *cdims, k_scale, v_scale, _DTYPES[q.dtype], cdt, n_axes,
+            interleaved), _raw_stream(index)))
     return q_out
 
 
 def paged_attention_workspace_bytes(R: int, Hq: int, Hkv: int, D: int) -> int:
     return int(lib().remora_b200_paged_attention_workspace_bytes(R, Hq, Hkv, D))
+
+
+@functools.lru_cache(maxsize=256)
+def _attention_workspace(R, Hq, Hkv, D, index) -> int:
+    with torch.cuda.device(index):
+        return paged_attention_workspace_bytes(R, Hq, Hkv, D)
 
 
 def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -521,35 +546,36 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         raise TypeError(f"paged_attention takes q in bf16 or f16, got {q.dtype}")
     R, Hq, D = q.shape
     Hkv = k_cache.shape[2] if k_cache.dim() == 4 else 0
-    cdt = _cache(q, k_cache, v_cache, Hkv, D)
+    cdt, cdims = _cache(q, k_cache, v_cache, Hkv, D)
     _ints("lens", lens, (R,))
+    max_blocks = block_table.shape[1]
     if block_table.dtype != torch.int32 or block_table.shape[0] != R or \
-            block_table.stride(1) != 1:
+            (max_blocks != 1 and block_table.stride(1) != 1):
         raise ValueError("block_table must be int32 [R, max_blocks] with adjacent entries")
-    guard = _on(q, k_cache, v_cache, block_table, lens)
+    guard, index = _on(q, k_cache, v_cache, block_table, lens)
     if out is None:
-        out = torch.empty((R, Hq, D), dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
         raise ValueError("out must have q's shape, type and device")
-    if q.stride(2) != 1 or out.stride(2) != 1:
+    qs, os_ = q.stride(), out.stride()
+    if qs[2] != 1 or os_[2] != 1:
         raise ValueError("the elements of a head must be adjacent")
-    if lse is not None and (lse.dtype != torch.float32 or tuple(lse.shape) != (R, Hq) or
+    if lse is not None and (lse.dtype != torch.float32 or lse.shape != (R, Hq) or
                             not lse.is_contiguous() or lse.device != q.device):
         raise ValueError("lse must be a contiguous float32 tensor [R, Hq]")
     if workspace is None:
-        need = paged_attention_workspace_bytes(R, Hq, Hkv, D)
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+        workspace = torch.empty(_attention_workspace(R, Hq, Hkv, D, index), dtype=torch.uint8,
+                                device=q.device)
     elif workspace.device != q.device or not workspace.is_contiguous():
         raise ValueError("workspace must be a contiguous tensor on q's device")
     with guard:
-        _check(lib().remora_b200_paged_attention(
+        _check(lib().remora_b200_paged_attention(_ATTENTION_ARGS.pack(
             q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
-            lens.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(),
-            _DTYPES[q.dtype], cdt, R, Hq, Hkv, D, q.stride(0), q.stride(1), out.stride(0),
-            out.stride(1), k_cache.shape[0], k_cache.shape[1], *k_cache.stride()[:3],
-            *v_cache.stride()[:3], block_table.stride(0) if R > 1 else block_table.shape[1],
-            block_table.shape[1], D ** -0.5 if scale is None else scale, window, k_scale, v_scale,
-            workspace.data_ptr(), workspace.numel() * workspace.element_size(), _stream(q)))
+            lens.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
+            workspace.data_ptr(), workspace.nbytes, R, Hq, Hkv, D, *qs[:2], *os_[:2], *cdims,
+            block_table.stride(0) if R > 1 else max_blocks, max_blocks, window,
+            D ** -0.5 if scale is None else scale, k_scale, v_scale, _DTYPES[q.dtype], cdt),
+            _raw_stream(index)))
     return out
 
 

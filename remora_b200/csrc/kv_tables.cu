@@ -232,40 +232,38 @@ __global__ void __launch_bounds__(1024) k_block_table(const TableArgs a) {
 }  // namespace kv
 }  // namespace rb
 
-extern "C" int remora_b200_kv_block_table(
-    const int32_t* lens, const int32_t* new_tokens, int64_t R, int32_t* block_table,
-    int64_t ld_table, int64_t max_blocks, int32_t* free_blocks, const int32_t* free_count,
-    int64_t num_blocks, int64_t block_size, int32_t* lens_out, int32_t* free_count_out,
-    int32_t* cu_tokens, int32_t* slots, int32_t* positions, int32_t* requests,
-    int64_t max_tokens, int32_t* status, void* stream) {
+extern "C" int remora_b200_kv_block_table(const remora_b200_kv_block_table_args* args,
+                                          void* stream) {
   using namespace rb;
   using namespace rb::kv;
   clear_error();
-  RB_CHECK_ARG(R >= 0 && R <= kMaxRequests, "kv_block_table: R must be in [0, %d], got %lld",
-               kMaxRequests, (long long)R);
-  RB_CHECK_ARG(max_tokens >= 0 && max_tokens < 0x7fffffff,
+  RB_CHECK_ARG(args, "kv_block_table: args is null");
+  const remora_b200_kv_block_table_args& x = *args;
+  RB_CHECK_ARG(x.R >= 0 && x.R <= kMaxRequests, "kv_block_table: R must be in [0, %d], got %lld",
+               kMaxRequests, (long long)x.R);
+  RB_CHECK_ARG(x.max_tokens >= 0 && x.max_tokens < 0x7fffffff,
                "kv_block_table: max_tokens must be in [0, 2^31 - 1)");
-  RB_CHECK_ARG(block_size >= 1 && num_blocks >= 1 && num_blocks < 0x7fffffff &&
-                   block_size <= 0x7fffffff && num_blocks <= 0x7fffffff / block_size,
+  RB_CHECK_ARG(x.block_size >= 1 && x.num_blocks >= 1 && x.num_blocks < 0x7fffffff &&
+                   x.block_size <= 0x7fffffff && x.num_blocks <= 0x7fffffff / x.block_size,
                "kv_block_table: num_blocks * block_size must be in [1, 2^31)");
-  RB_CHECK_ARG(max_blocks >= 1 && max_blocks <= 0x7fffffff / block_size,
+  RB_CHECK_ARG(x.max_blocks >= 1 && x.max_blocks <= 0x7fffffff / x.block_size,
                "kv_block_table: max_blocks * block_size must be in [1, 2^31)");
-  RB_CHECK_ARG(ld_table >= max_blocks, "kv_block_table: ld_table must be at least max_blocks");
-  RB_CHECK_ARG(free_blocks && free_count && free_count_out && cu_tokens,
+  RB_CHECK_ARG(x.ld_table >= x.max_blocks, "kv_block_table: ld_table must be at least max_blocks");
+  RB_CHECK_ARG(x.free_blocks && x.free_count && x.free_count_out && x.cu_tokens,
                "kv_block_table: null pointer");
-  RB_CHECK_ARG(R == 0 || (lens && new_tokens && block_table && lens_out && status),
+  RB_CHECK_ARG(x.R == 0 || (x.lens && x.new_tokens && x.block_table && x.lens_out && x.status),
                "kv_block_table: null pointer");
-  RB_CHECK_ARG(max_tokens == 0 || (slots && positions && requests),
+  RB_CHECK_ARG(x.max_tokens == 0 || (x.slots && x.positions && x.requests),
                "kv_block_table: null pointer");
-  TableArgs a{lens, new_tokens, block_table, ld_table, free_blocks, lens_out, free_count_out,
-              cu_tokens, slots, positions, requests, status, free_count, (int32_t)R,
-              (int32_t)max_blocks, (int32_t)num_blocks, (int32_t)block_size,
-              (int32_t)max_tokens};
-  const size_t smem = (4 * (size_t)R + 3) * sizeof(int32_t);
+  TableArgs a{x.lens, x.new_tokens, x.block_table, x.ld_table, x.free_blocks, x.lens_out,
+              x.free_count_out, x.cu_tokens, x.slots, x.positions, x.requests, x.status,
+              x.free_count, (int32_t)x.R, (int32_t)x.max_blocks, (int32_t)x.num_blocks,
+              (int32_t)x.block_size, (int32_t)x.max_tokens};
+  const size_t smem = (4 * (size_t)x.R + 3) * sizeof(int32_t);
   if (smem > 48 * 1024)
     RB_CUDA(cudaFuncSetAttribute(k_block_table, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  (4 * kMaxRequests + 3) * (int)sizeof(int32_t)));
-  const int threads = 1024, ctas = max_tokens > 4096 ? 8 : 1;
+  const int threads = 1024, ctas = x.max_tokens > 4096 ? 8 : 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas);
   cfg.blockDim = dim3(threads);

@@ -844,59 +844,56 @@ extern "C" size_t remora_b200_paged_attention_workspace_bytes(int64_t R, int64_t
   return (size_t)(sms * (8 + 2) * part_floats(Hq, Hkv, D) * 4 + sms * (int64_t)sizeof(Cross));
 }
 
-extern "C" int remora_b200_paged_attention(
-    const void* q, const void* k_cache, const void* v_cache, const int32_t* block_table,
-    const int32_t* lens, void* out, float* lse, int dtype, int cache_dtype, int64_t R, int64_t Hq,
-    int64_t Hkv, int64_t D, int64_t q_t, int64_t q_h, int64_t out_t, int64_t out_h,
-    int64_t num_blocks, int64_t block_size, int64_t kc_block, int64_t kc_token, int64_t kc_head,
-    int64_t vc_block, int64_t vc_token, int64_t vc_head, int64_t ld_table, int64_t max_blocks,
-    float scale, int64_t window, float k_scale, float v_scale, void* workspace,
-    size_t workspace_bytes, void* stream) {
+extern "C" int remora_b200_paged_attention(const remora_b200_paged_attention_args* args,
+                                           void* stream) {
   using namespace rb;
   using namespace rb::paged;
   clear_error();
-  RB_CHECK_ARG(dtype == REMORA_B200_BF16 || dtype == REMORA_B200_F16,
+  RB_CHECK_ARG(args, "paged_attention: args is null");
+  const remora_b200_paged_attention_args& p = *args;
+  const int64_t R = p.R, Hq = p.Hq, Hkv = p.Hkv, D = p.D;
+  RB_CHECK_ARG(p.dtype == REMORA_B200_BF16 || p.dtype == REMORA_B200_F16,
                "paged_attention: dtype must be BF16 or F16");
-  RB_CHECK_ARG(cache_dtype == dtype || cache_dtype == REMORA_B200_E4M3,
+  RB_CHECK_ARG(p.cache_dtype == p.dtype || p.cache_dtype == REMORA_B200_E4M3,
                "paged_attention: cache_dtype must be dtype or E4M3");
   RB_CHECK_ARG(shape_ok(R, Hq, Hkv, D),
                "paged_attention: needs R in [0, %d], Hq a multiple of Hkv and head_dim 64, 128 or "
                "256 (got R %lld, Hq %lld, Hkv %lld, head_dim %lld)",
                kMaxRequests, (long long)R, (long long)Hq, (long long)Hkv, (long long)D);
-  RB_CHECK_ARG(block_size >= 1 && num_blocks >= 1 && block_size <= 0x7fffffff &&
-                   num_blocks <= 0x7fffffff / block_size,
+  RB_CHECK_ARG(p.block_size >= 1 && p.num_blocks >= 1 && p.block_size <= 0x7fffffff &&
+                   p.num_blocks <= 0x7fffffff / p.block_size,
                "paged_attention: num_blocks * block_size must be in [1, 2^31)");
-  RB_CHECK_ARG(max_blocks >= 1 && max_blocks <= 0x7fffffff / block_size && ld_table >= max_blocks,
+  RB_CHECK_ARG(p.max_blocks >= 1 && p.max_blocks <= 0x7fffffff / p.block_size && p.ld_table >= p.max_blocks,
                "paged_attention: max_blocks * block_size must be in [1, 2^31) and ld_table at "
                "least max_blocks");
-  RB_CHECK_ARG(std::isfinite(scale), "paged_attention: scale is not finite");
-  RB_CHECK_ARG(window >= 0, "paged_attention: window must not be negative");
-  RB_CHECK_ARG(std::isfinite(k_scale) && k_scale > 0 && std::isfinite(v_scale) && v_scale > 0,
+  RB_CHECK_ARG(std::isfinite(p.scale), "paged_attention: scale is not finite");
+  RB_CHECK_ARG(p.window >= 0, "paged_attention: window must not be negative");
+  RB_CHECK_ARG(std::isfinite(p.k_scale) && p.k_scale > 0 && std::isfinite(p.v_scale) && p.v_scale > 0,
                "paged_attention: the cache scales must be positive and finite");
-  RB_CHECK_ARG(cache_dtype == REMORA_B200_E4M3 || (k_scale == 1.0f && v_scale == 1.0f),
+  RB_CHECK_ARG(p.cache_dtype == REMORA_B200_E4M3 || (p.k_scale == 1.0f && p.v_scale == 1.0f),
                "paged_attention: the scales must be 1 unless the cache is E4M3");
   if (R == 0) return REMORA_B200_OK;
-  RB_CHECK_ARG(q && k_cache && v_cache && block_table && lens && out,
+  RB_CHECK_ARG(p.q && p.k_cache && p.v_cache && p.block_table && p.lens && p.out,
                "paged_attention: null pointer");
-  RB_CHECK_ARG(aligned16(q) && aligned16(k_cache) && aligned16(v_cache) && aligned16(out),
+  RB_CHECK_ARG(aligned16(p.q) && aligned16(p.k_cache) && aligned16(p.v_cache) && aligned16(p.out),
                "paged_attention: q, the caches and out must be 16-byte aligned");
-  const int64_t ce = cache_dtype == REMORA_B200_E4M3 ? 16 : 8;
-  RB_CHECK_ARG(q_t % 8 == 0 && q_h % 8 == 0 && out_t % 8 == 0 && out_h % 8 == 0 &&
-                   kc_block % ce == 0 && kc_token % ce == 0 && kc_head % ce == 0 &&
-                   vc_block % ce == 0 && vc_token % ce == 0 && vc_head % ce == 0,
+  const int64_t ce = p.cache_dtype == REMORA_B200_E4M3 ? 16 : 8;
+  RB_CHECK_ARG(p.q_t % 8 == 0 && p.q_h % 8 == 0 && p.out_t % 8 == 0 && p.out_h % 8 == 0 &&
+                   p.kc_block % ce == 0 && p.kc_token % ce == 0 && p.kc_head % ce == 0 &&
+                   p.vc_block % ce == 0 && p.vc_token % ce == 0 && p.vc_head % ce == 0,
                "paged_attention: strides must be multiples of 16 bytes");
   const size_t need = remora_b200_paged_attention_workspace_bytes(R, Hq, Hkv, D);
-  RB_CHECK_ARG(workspace && workspace_bytes >= need && aligned16(workspace),
+  RB_CHECK_ARG(p.workspace && p.workspace_bytes >= need && aligned16(p.workspace),
                "paged_attention: workspace of %zu bytes, 16-byte aligned, is needed", need);
-  Args a{q, k_cache, v_cache, block_table, lens, out, lse, q_t, q_h, out_t, out_h, kc_block,
-         kc_token, kc_head, vc_block, vc_token, vc_head, ld_table, window, (int32_t)R, (int32_t)Hq,
-         (int32_t)Hkv, (int32_t)D, (int32_t)num_blocks, (int32_t)block_size, (int32_t)max_blocks,
-         scale * 1.4426950408889634f * k_scale, v_scale};
+  Args a{p.q, p.k_cache, p.v_cache, p.block_table, p.lens, p.out, p.lse, p.q_t, p.q_h, p.out_t, p.out_h, p.kc_block,
+         p.kc_token, p.kc_head, p.vc_block, p.vc_token, p.vc_head, p.ld_table, p.window, (int32_t)R, (int32_t)Hq,
+         (int32_t)Hkv, (int32_t)D, (int32_t)p.num_blocks, (int32_t)p.block_size, (int32_t)p.max_blocks,
+         p.scale * 1.4426950408889634f * p.k_scale, p.v_scale};
   cudaStream_t st = as_stream(stream);
-  const bool f8 = cache_dtype == REMORA_B200_E4M3;
-  if (dtype == REMORA_B200_BF16)
-    return f8 ? launch_shape<__nv_bfloat16, __nv_fp8_e4m3>(a, workspace, st)
-              : launch_shape<__nv_bfloat16, __nv_bfloat16>(a, workspace, st);
-  return f8 ? launch_shape<__half, __nv_fp8_e4m3>(a, workspace, st)
-            : launch_shape<__half, __half>(a, workspace, st);
+  const bool f8 = p.cache_dtype == REMORA_B200_E4M3;
+  if (p.dtype == REMORA_B200_BF16)
+    return f8 ? launch_shape<__nv_bfloat16, __nv_fp8_e4m3>(a, p.workspace, st)
+              : launch_shape<__nv_bfloat16, __nv_bfloat16>(a, p.workspace, st);
+  return f8 ? launch_shape<__half, __nv_fp8_e4m3>(a, p.workspace, st)
+            : launch_shape<__half, __half>(a, p.workspace, st);
 }

@@ -361,106 +361,101 @@ inline int angles(const char* who, Args& a, const int32_t* positions, int64_t ld
 }  // namespace rope
 }  // namespace rb
 
-extern "C" int remora_b200_rope(const void* x, void* out, int dtype, int64_t B, int64_t S,
-                                int64_t H, int64_t D, int64_t x_b, int64_t x_s, int64_t x_h,
-                                int64_t out_b, int64_t out_s, int64_t out_h,
-                                const int32_t* positions, int64_t ld_pos, int n_axes,
-                                const double* freq, const int32_t* axis_of, int64_t rot,
-                                int interleaved, int inverse, void* stream) {
+extern "C" int remora_b200_rope(const remora_b200_rope_args* args, void* stream) {
   using namespace rb;
   using namespace rb::rope;
   clear_error();
-  RB_CHECK_ARG(dtype == REMORA_B200_BF16 || dtype == REMORA_B200_F16 || dtype == REMORA_B200_F32,
+  RB_CHECK_ARG(args, "rope: args is null");
+  const remora_b200_rope_args& p = *args;
+  const int64_t B = p.B, S = p.S, H = p.H, D = p.D;
+  RB_CHECK_ARG(p.dtype == REMORA_B200_BF16 || p.dtype == REMORA_B200_F16 || p.dtype == REMORA_B200_F32,
                "rope: dtype must be BF16, F16 or F32");
   RB_CHECK_ARG(B >= 0 && S >= 0 && H >= 0 && H <= 65536, "rope: bad shape");
   RB_CHECK_ARG(B <= (1ll << 31) && S <= (1ll << 31), "rope: bad shape");
   Args a = {};
-  int rc = angles("rope", a, positions, ld_pos, n_axes, freq, axis_of, rot, D, B * S);
+  int rc = angles("rope", a, p.positions, p.ld_pos, p.n_axes, p.freq, p.axis_of, p.rot, D, B * S);
   if (rc) return rc;
   if (B * S * H == 0) return REMORA_B200_OK;
-  RB_CHECK_ARG(x && out, "rope: null pointer");
+  RB_CHECK_ARG(p.x && p.out, "rope: null pointer");
   a.S = S;
-  a.q = Heads{x, out, x_b, x_s, x_h, out_b, out_s, out_h, (int32_t)H};
-  a.sign = inverse ? -1.0f : 1.0f;
-  const int e = dtype_bytes(dtype);
+  a.q = Heads{p.x, p.out, p.x_b, p.x_s, p.x_h, p.out_b, p.out_s, p.out_h, (int32_t)H};
+  a.sign = p.inverse ? -1.0f : 1.0f;
+  const int e = dtype_bytes(p.dtype);
   Fit f;
   f.elems(a.half);
   f.elems(D);
-  f.rows(x, e, B > 1 ? x_b : 0, x_s, x_h);
-  f.rows(out, e, B > 1 ? out_b : 0, out_s, out_h);
+  f.rows(p.x, e, B > 1 ? p.x_b : 0, p.x_s, p.x_h);
+  f.rows(p.out, e, B > 1 ? p.out_b : 0, p.out_s, p.out_h);
   RB_CHECK_ARG(f.whole, "rope: a pointer is not aligned to its elements");
   cudaStream_t st = as_stream(stream);
-  if (dtype == REMORA_B200_BF16)
-    return launch<__nv_bfloat16, __nv_bfloat16, false>(a, f.v, interleaved, st);
-  if (dtype == REMORA_B200_F16) return launch<__half, __half, false>(a, f.v, interleaved, st);
-  return launch<float, float, false>(a, f.v, interleaved, st);
+  if (p.dtype == REMORA_B200_BF16)
+    return launch<__nv_bfloat16, __nv_bfloat16, false>(a, f.v, p.interleaved, st);
+  if (p.dtype == REMORA_B200_F16) return launch<__half, __half, false>(a, f.v, p.interleaved, st);
+  return launch<float, float, false>(a, f.v, p.interleaved, st);
 }
 
-extern "C" int remora_b200_rope_kv_append(
-    const void* q, const void* k, const void* v, void* q_out, int dtype, int64_t T, int64_t Hq,
-    int64_t Hkv, int64_t D, int64_t q_t, int64_t q_h, int64_t k_t, int64_t k_h, int64_t v_t,
-    int64_t v_h, int64_t qo_t, int64_t qo_h, const int32_t* positions, int64_t ld_pos, int n_axes,
-    const double* freq, const int32_t* axis_of, int64_t rot, int interleaved,
-    const int32_t* slots, void* k_cache, void* v_cache, int cache_dtype, int64_t num_blocks,
-    int64_t block_size, int64_t kc_block, int64_t kc_token, int64_t kc_head, int64_t vc_block,
-    int64_t vc_token, int64_t vc_head, float k_scale, float v_scale, void* stream) {
+extern "C" int remora_b200_rope_kv_append(const remora_b200_rope_kv_append_args* args,
+                                          void* stream) {
   using namespace rb;
   using namespace rb::rope;
   clear_error();
-  RB_CHECK_ARG(dtype == REMORA_B200_BF16 || dtype == REMORA_B200_F16,
+  RB_CHECK_ARG(args, "rope_kv_append: args is null");
+  const remora_b200_rope_kv_append_args& p = *args;
+  const int64_t T = p.T, Hq = p.Hq, Hkv = p.Hkv, D = p.D;
+  RB_CHECK_ARG(p.dtype == REMORA_B200_BF16 || p.dtype == REMORA_B200_F16,
                "rope_kv_append: dtype must be BF16 or F16");
-  RB_CHECK_ARG(cache_dtype == dtype || cache_dtype == REMORA_B200_E4M3,
+  RB_CHECK_ARG(p.cache_dtype == p.dtype || p.cache_dtype == REMORA_B200_E4M3,
                "rope_kv_append: cache_dtype must be dtype or E4M3");
   RB_CHECK_ARG(T >= 0 && Hq >= 0 && Hkv >= 1 && Hq <= 65536 && Hkv <= 65536,
                "rope_kv_append: bad shape");
-  RB_CHECK_ARG(block_size >= 1 && num_blocks >= 1 && block_size <= 0x7fffffff &&
-                   num_blocks <= 0x7fffffff / block_size,
+  RB_CHECK_ARG(p.block_size >= 1 && p.num_blocks >= 1 && p.block_size <= 0x7fffffff &&
+                   p.num_blocks <= 0x7fffffff / p.block_size,
                "rope_kv_append: num_blocks * block_size must be in [1, 2^31)");
-  RB_CHECK_ARG(std::isfinite(k_scale) && k_scale > 0 && std::isfinite(v_scale) && v_scale > 0,
+  RB_CHECK_ARG(std::isfinite(p.k_scale) && p.k_scale > 0 && std::isfinite(p.v_scale) && p.v_scale > 0,
                "rope_kv_append: the scales must be positive and finite");
-  RB_CHECK_ARG(cache_dtype == REMORA_B200_E4M3 || (k_scale == 1.0f && v_scale == 1.0f),
+  RB_CHECK_ARG(p.cache_dtype == REMORA_B200_E4M3 || (p.k_scale == 1.0f && p.v_scale == 1.0f),
                "rope_kv_append: the scales must be 1 unless the cache is E4M3");
   Args a = {};
-  int rc = angles("rope_kv_append", a, positions, ld_pos, n_axes, freq, axis_of, rot, D, T);
+  int rc = angles("rope_kv_append", a, p.positions, p.ld_pos, p.n_axes, p.freq, p.axis_of, p.rot, D, T);
   if (rc) return rc;
   if (T == 0) return REMORA_B200_OK;
-  RB_CHECK_ARG((Hq == 0 || (q && q_out)) && k && v && slots && k_cache && v_cache,
+  RB_CHECK_ARG((Hq == 0 || (p.q && p.q_out)) && p.k && p.v && p.slots && p.k_cache && p.v_cache,
                "rope_kv_append: null pointer");
   a.S = T;
-  a.q = Heads{q, q_out, 0, q_t, q_h, 0, qo_t, qo_h, (int32_t)Hq};
-  a.k = Heads{k, k_cache, 0, k_t, k_h, 0, 0, 0, (int32_t)Hkv};
-  a.v = Heads{v, v_cache, 0, v_t, v_h, 0, 0, 0, (int32_t)Hkv};
-  a.slots = slots;
-  a.num_blocks = (int32_t)num_blocks;
-  a.bs = (int32_t)block_size;
-  a.c_blk_k = kc_block;
-  a.c_tok_k = kc_token;
-  a.c_head_k = kc_head;
-  a.c_blk_v = vc_block;
-  a.c_tok_v = vc_token;
-  a.c_head_v = vc_head;
-  a.k_scale = k_scale;
-  a.v_scale = v_scale;
+  a.q = Heads{p.q, p.q_out, 0, p.q_t, p.q_h, 0, p.q_out_t, p.q_out_h, (int32_t)Hq};
+  a.k = Heads{p.k, p.k_cache, 0, p.k_t, p.k_h, 0, 0, 0, (int32_t)Hkv};
+  a.v = Heads{p.v, p.v_cache, 0, p.v_t, p.v_h, 0, 0, 0, (int32_t)Hkv};
+  a.slots = p.slots;
+  a.num_blocks = (int32_t)p.num_blocks;
+  a.bs = (int32_t)p.block_size;
+  a.c_blk_k = p.kc_block;
+  a.c_tok_k = p.kc_token;
+  a.c_head_k = p.kc_head;
+  a.c_blk_v = p.vc_block;
+  a.c_tok_v = p.vc_token;
+  a.c_head_v = p.vc_head;
+  a.k_scale = p.k_scale;
+  a.v_scale = p.v_scale;
   a.sign = 1.0f;
-  const int c = dtype_bytes(cache_dtype);
+  const int c = dtype_bytes(p.cache_dtype);
   Fit f;
   f.elems(a.half);
   f.elems(D);
   if (Hq) {
-    f.rows(q, 2, q_t, q_h, 0);
-    f.rows(q_out, 2, qo_t, qo_h, 0);
+    f.rows(p.q, 2, p.q_t, p.q_h, 0);
+    f.rows(p.q_out, 2, p.q_out_t, p.q_out_h, 0);
   }
-  f.rows(k, 2, k_t, k_h, 0);
-  f.rows(v, 2, v_t, v_h, 0);
-  f.rows(k_cache, c, kc_block, kc_token, kc_head);
-  f.rows(v_cache, c, vc_block, vc_token, vc_head);
+  f.rows(p.k, 2, p.k_t, p.k_h, 0);
+  f.rows(p.v, 2, p.v_t, p.v_h, 0);
+  f.rows(p.k_cache, c, p.kc_block, p.kc_token, p.kc_head);
+  f.rows(p.v_cache, c, p.vc_block, p.vc_token, p.vc_head);
   RB_CHECK_ARG(f.whole, "rope_kv_append: a pointer is not aligned to its elements");
   cudaStream_t st = as_stream(stream);
-  if (dtype == REMORA_B200_BF16)
-    return cache_dtype == REMORA_B200_E4M3
-               ? launch<__nv_bfloat16, __nv_fp8_e4m3, true>(a, f.v, interleaved, st)
-               : launch<__nv_bfloat16, __nv_bfloat16, true>(a, f.v, interleaved, st);
-  return cache_dtype == REMORA_B200_E4M3
-             ? launch<__half, __nv_fp8_e4m3, true>(a, f.v, interleaved, st)
-             : launch<__half, __half, true>(a, f.v, interleaved, st);
+  if (p.dtype == REMORA_B200_BF16)
+    return p.cache_dtype == REMORA_B200_E4M3
+               ? launch<__nv_bfloat16, __nv_fp8_e4m3, true>(a, f.v, p.interleaved, st)
+               : launch<__nv_bfloat16, __nv_bfloat16, true>(a, f.v, p.interleaved, st);
+  return p.cache_dtype == REMORA_B200_E4M3
+             ? launch<__half, __nv_fp8_e4m3, true>(a, f.v, p.interleaved, st)
+             : launch<__half, __half, true>(a, f.v, p.interleaved, st);
 }

@@ -9,8 +9,13 @@ import torch
 import remora_b200 as rb
 from tests import _paged as ref
 
-A = ctypes.c_void_p(1 << 20)
-ODD = ctypes.c_void_p((1 << 20) + 8)
+A = 1 << 20  # never read: every refusal comes before the first access
+ODD = A + 8
+
+
+def call(fn, packer, fields):
+    """The entry point on a packed argument struct (None = a null pointer)."""
+    return fn(packer.pack(*(0 if v is None else v for v in fields.values())), None)
 
 
 @pytest.fixture(scope="module")
@@ -22,10 +27,10 @@ def L():
 
 
 def tables(L, **c):
-    d = dict(lens=A, new=A, R=4, table=A, ld=8, mb=8, free=A, count=A, nb=32, bs=16, lo=A, co=A,
-             cu=A, slots=A, pos=A, req=A, mt=4, status=A)
+    d = dict(lens=A, new=A, table=A, free=A, count=A, lo=A, co=A, cu=A, slots=A, pos=A, req=A,
+             status=A, R=4, ld=8, mb=8, nb=32, bs=16, mt=4)
     d.update(c)
-    return L.remora_b200_kv_block_table(*d.values(), None)
+    return call(L.remora_b200_kv_block_table, rb._BLOCK_TABLE_ARGS, d)
 
 
 @pytest.mark.parametrize("bad", [
@@ -38,23 +43,25 @@ def test_block_table_refuses(L, bad):
     assert tables(L, **bad) == rb.ERR_INVALID and "kv_block_table" in rb.last_error()
 
 
-FREQ = (ctypes.c_double * 64)(*[0.5] * 64)
-AXES = (ctypes.c_int32 * 64)(*[0] * 63, 1)
+_FREQ = (ctypes.c_double * 64)(*[0.5] * 64)
+_NAN = (ctypes.c_double * 64)(*[0.5] * 63, float("nan"))
+_INF = (ctypes.c_double * 64)(*[float("inf")] * 64)
+_AXES = (ctypes.c_int32 * 64)(*[0] * 63, 1)
+FREQ, NAN, INF, AXES = (ctypes.addressof(x) for x in (_FREQ, _NAN, _INF, _AXES))
 
 
 def rope(L, **c):
-    d = dict(x=A, out=A, dt=rb.BF16, B=1, S=4, H=2, D=128, xb=0, xs=256, xh=128, ob=0, os=256,
-             oh=128, pos=A, ld=4, axes=1, freq=FREQ, ax=None, rot=128, inter=0, inv=0)
+    d = dict(x=A, out=A, pos=A, freq=FREQ, ax=None, B=1, S=4, H=2, D=128, rot=128, xb=0, xs=256,
+             xh=128, ob=0, os=256, oh=128, ld=4, dt=rb.BF16, axes=1, inter=0, inv=0)
     d.update(c)
-    return L.remora_b200_rope(*d.values(), None)
+    return call(L.remora_b200_rope, rb._ROPE_ARGS, d)
 
 
 @pytest.mark.parametrize("bad", [
     dict(x=None), dict(out=None), dict(dt=rb.E4M3), dict(dt=9), dict(B=-1), dict(S=-1), dict(H=-1),
     dict(D=0), dict(D=2048), dict(pos=None), dict(ld=3, axes=2), dict(axes=0), dict(axes=9),
     dict(freq=None), dict(ax=AXES), dict(rot=3), dict(rot=130), dict(rot=258, D=512),
-    dict(x=ctypes.c_void_p((1 << 20) + 1)), dict(freq=(ctypes.c_double * 64)(*[float("nan")] * 64)),
-    dict(freq=(ctypes.c_double * 64)(*[float("inf")] * 64))])
+    dict(x=A + 1), dict(freq=NAN), dict(freq=INF)])
 def test_rope_refuses(L, bad):
     assert rope(L, **bad) == rb.ERR_INVALID and "rope" in rb.last_error()
 
@@ -65,12 +72,12 @@ def test_rope_without_rows_is_done(L):
 
 
 def append(L, **c):
-    d = dict(q=A, k=A, v=A, qo=A, dt=rb.BF16, T=4, Hq=4, Hkv=2, D=128, qt=512, qh=128, kt=256,
-             kh=128, vt=256, vh=128, ot=512, oh=128, pos=A, ld=4, axes=1, freq=FREQ, ax=None,
-             rot=128, inter=0, slots=A, kc=A, vc=A, cdt=rb.BF16, nb=4, bs=16, kb=4096, ktok=256,
-             khd=128, vb=4096, vtok=256, vhd=128, ks=1.0, vs=1.0)
+    d = dict(q=A, k=A, v=A, qo=A, kc=A, vc=A, pos=A, slots=A, freq=FREQ, ax=None, T=4, Hq=4, Hkv=2,
+             D=128, rot=128, qt=512, qh=128, kt=256, kh=128, vt=256, vh=128, ot=512, oh=128, ld=4,
+             nb=4, bs=16, kb=4096, ktok=256, khd=128, vb=4096, vtok=256, vhd=128, ks=1.0, vs=1.0,
+             dt=rb.BF16, cdt=rb.BF16, axes=1, inter=0)
     d.update(c)
-    return L.remora_b200_rope_kv_append(*d.values(), None)
+    return call(L.remora_b200_rope_kv_append, rb._APPEND_ARGS, d)
 
 
 @pytest.mark.parametrize("bad", [
@@ -78,18 +85,18 @@ def append(L, **c):
     dict(vc=None), dict(pos=None), dict(dt=rb.F32), dict(cdt=rb.F16), dict(T=-1), dict(Hkv=0),
     dict(nb=0), dict(bs=0), dict(nb=2 ** 28), dict(ks=0.0), dict(vs=-1.0), dict(ks=2.0),
     dict(cdt=rb.E4M3, ks=float("nan")), dict(cdt=rb.E4M3, vs=float("inf")), dict(rot=200),
-    dict(kc=ctypes.c_void_p((1 << 20) + 1))])
+    dict(kc=A + 1)])
 def test_append_refuses(L, bad):
     assert append(L, **bad) == rb.ERR_INVALID and "rope_kv_append" in rb.last_error()
 
 
 def attention(L, **c):
-    d = dict(q=A, kc=A, vc=A, table=A, lens=A, out=A, lse=None, dt=rb.BF16, cdt=rb.BF16, R=2, Hq=8,
-             Hkv=2, D=128, qt=1024, qh=128, ot=1024, oh=128, nb=8, bs=16, kb=4096, kt=256, kh=128,
-             vb=4096, vt=256, vh=128, ld=8, mb=8, scale=1.0, window=0, ks=1.0, vs=1.0, ws=A,
-             wsb=1 << 40)
+    d = dict(q=A, kc=A, vc=A, table=A, lens=A, out=A, lse=None, ws=A, wsb=1 << 40, R=2, Hq=8, Hkv=2,
+             D=128, qt=1024, qh=128, ot=1024, oh=128, nb=8, bs=16, kb=4096, kt=256, kh=128, vb=4096,
+             vt=256, vh=128, ld=8, mb=8, window=0, scale=1.0, ks=1.0, vs=1.0, dt=rb.BF16,
+             cdt=rb.BF16)
     d.update(c)
-    return L.remora_b200_paged_attention(*d.values(), None)
+    return call(L.remora_b200_paged_attention, rb._ATTENTION_ARGS, d)
 
 
 @pytest.mark.parametrize("bad", [
@@ -102,6 +109,38 @@ def attention(L, **c):
     dict(cdt=rb.E4M3, kt=264), dict(qt=1020), dict(oh=4), dict(kt=12), dict(vb=4)])
 def test_attention_refuses(L, bad):
     assert attention(L, **bad) == rb.ERR_INVALID and "paged_attention" in rb.last_error()
+
+
+def test_null_argument_structs_are_refused(L):
+    for fn in (L.remora_b200_kv_block_table, L.remora_b200_rope, L.remora_b200_rope_kv_append,
+               L.remora_b200_paged_attention):
+        assert fn(None, None) == rb.ERR_INVALID and "null" in rb.last_error()
+
+
+def test_packed_structs_have_the_headers_layout(tmp_path):
+    """The packers' sizes, and their last fields' places, as a C compiler lays the structs out."""
+    import os
+    import subprocess
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    names = {"kv_block_table": ("max_tokens", rb._BLOCK_TABLE_ARGS),
+             "rope": ("inverse", rb._ROPE_ARGS),
+             "rope_kv_append": ("interleaved", rb._APPEND_ARGS),
+             "paged_attention": ("cache_dtype", rb._ATTENTION_ARGS)}
+    src = '#include <stdio.h>\n#include <stddef.h>\n#include "remora_b200.h"\nint main(void) {\n'
+    for n, (last, _) in names.items():
+        src += f'printf("%zu %zu\\n", sizeof(remora_b200_{n}_args), ' \
+               f'offsetof(remora_b200_{n}_args, {last}));\n'
+    (tmp_path / "s.c").write_text(src + "return 0; }\n")
+    exe = str(tmp_path / "s")
+    subprocess.run(["gcc", "-I", os.path.join(root, "include"), str(tmp_path / "s.c"), "-o", exe],
+                   check=True)
+    lines = subprocess.run([exe], capture_output=True, text=True, check=True).stdout.split("\n")
+    for line, (n, (last, packer)) in zip(lines, names.items()):
+        size, at = map(int, line.split())
+        pad = 4 if n == "paged_attention" else 0
+        width = 8 if n == "kv_block_table" else 4
+        assert size == packer.size and at == packer.size - pad - width, n
 
 
 def test_attention_without_requests_is_done_and_workspace_sizes(L):
