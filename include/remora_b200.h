@@ -239,7 +239,7 @@ int remora_b200_kv_block_table(const remora_b200_kv_block_table_args* args, void
  * x_h (elements; out may be x).  positions: n_axes rows of B * S int32 on the
  * device.  freq (rot / 2 doubles) and axis_of (rot / 2 ints, NULL = all 0)
  * are HOST arrays, read before the call returns.  rot even, <= min(D, 256);
- * D <= 1024; n_axes <= 8.  Angles are exact to 2^-25 of a quarter turn at
+ * D <= 512; n_axes <= 8.  Angles are exact to 2^-25 of a quarter turn at
  * every 32-bit position.  Any strides; sizes, strides and bases that are
  * multiples of 8 elements (and 16 bytes) move 8 pairs at a time. */
 typedef struct remora_b200_rope_args {

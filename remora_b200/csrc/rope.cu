@@ -26,6 +26,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "runtime.cuh"
 
@@ -35,7 +36,10 @@ namespace rope {
 constexpr int kThreads = 256;
 constexpr int kMaxHalf = 128;     // pairs of a head: rot <= 256
 constexpr int kMaxAxes = 8;
-constexpr int kTileAngles = 2048;  // shared-memory pairs of one tile of tokens
+constexpr int kTileAngles = 1024;  // pairs of one tile of tokens in shared memory
+constexpr int kTileTokens = 128;
+constexpr int64_t kNone = INT64_MIN;
+constexpr int kUnits = 2;          // units a thread holds in registers
 
 struct Turns {
   uint64_t f[kMaxHalf];  // freq / (2 pi), fraction of a turn in 2^-64
@@ -51,6 +55,20 @@ struct Heads {
   int32_t H;
 };
 
+// Division of n < 2^31 by d, as a multiplication: m = floor(2^(31 + s) / d) + 1 with 2^s >= d
+// is off by at most 2^s / d < 1 per n / 2^31, which never carries into the quotient.
+struct Divisor {
+  uint32_t d, m, s;
+  Divisor() = default;
+  explicit Divisor(uint32_t d_) : d(d_), s(0) {
+    while ((1ull << s) < d) ++s;
+    m = (uint32_t)((1ull << (31 + s)) / d + 1);
+  }
+  __device__ __forceinline__ int div(int n) const {
+    return (int)((uint64_t)(uint32_t)n * m >> (31 + s));
+  }
+};
+
 struct Args {
   Heads q, k, v;  // k and v: out is the cache, addressed by slot
   const int32_t* pos;
@@ -60,9 +78,11 @@ struct Args {
   int64_t c_blk_k, c_tok_k, c_head_k, c_blk_v, c_tok_v, c_head_v;
   int32_t num_blocks, bs;
   int32_t D, half, n_axes;
-  int32_t tile;         // tokens of a block's iteration
-  int32_t rot_units;    // units of V pairs in a head
-  int32_t units;        // those and the units of V plain elements behind them
+  int32_t tile;       // tokens of a block's iteration
+  int32_t rot_units;  // units of V pairs in a head
+  int32_t units;      // those and the units of 2V plain elements behind them
+  int32_t pass;       // heads side by side: kThreads / units
+  Divisor heads;      // of a token
   float k_scale, v_scale;
   float sign;
   Turns turns;
@@ -87,50 +107,38 @@ template <> __device__ __forceinline__ __nv_fp8_e4m3 from_f(float v) {
 // V elements in accesses of up to 16 bytes (V * sizeof(T) is a power of two;
 // the host checked that every address is a multiple of it, up to 16).
 template <typename T, int V>
-struct Vec {
+struct alignas(V * sizeof(T) < 16 ? V * sizeof(T) : 16) Raw {
   static constexpr int kBytes = V * (int)sizeof(T);
-  union U {
-    T e[V];
-    uint4 w16[kBytes >= 16 ? kBytes / 16 : 1];
-    uint2 w8;
-    uint32_t w4;
-    uint16_t w2;
-    uint8_t w1;
-    __device__ U() {}
-  };
-  static __device__ __forceinline__ void load(const T* p, float (&x)[V]) {
-    U u;
-    if constexpr (kBytes >= 16) {
+  using Piece = typename std::conditional<
+      kBytes >= 16, uint4,
+      typename std::conditional<
+          kBytes == 8, uint2,
+          typename std::conditional<kBytes == 4, uint32_t,
+                                    typename std::conditional<kBytes == 2, uint16_t,
+                                                              uint8_t>::type>::type>::type>::type;
+  static constexpr int kPieces = kBytes / (int)sizeof(Piece);
+  T e[V];
+  __device__ __forceinline__ Piece* pieces() { return reinterpret_cast<Piece*>(e); }
+  __device__ __forceinline__ void load(const T* p) {  // read once: not kept in the caches
 #pragma unroll
-      for (int i = 0; i < kBytes / 16; ++i) u.w16[i] = __ldcs(reinterpret_cast<const uint4*>(p) + i);
-    } else if constexpr (kBytes == 8) {
-      u.w8 = __ldcs(reinterpret_cast<const uint2*>(p));
-    } else if constexpr (kBytes == 4) {
-      u.w4 = __ldcs(reinterpret_cast<const uint32_t*>(p));
-    } else {
-      u.w2 = __ldcs(reinterpret_cast<const uint16_t*>(p));
-    }
-#pragma unroll
-    for (int i = 0; i < V; ++i) x[i] = to_f<T>(u.e[i]);
+    for (int i = 0; i < kPieces; ++i) pieces()[i] = __ldcs(reinterpret_cast<const Piece*>(p) + i);
   }
-  static __device__ __forceinline__ void store(T* p, const float (&x)[V]) {
-    U u;
+  __device__ __forceinline__ void store(T* p) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) u.e[i] = from_f<T>(x[i]);
-    if constexpr (kBytes >= 16) {
+    for (int i = 0; i < kPieces; ++i) reinterpret_cast<Piece*>(p)[i] = pieces()[i];
+  }
+  __device__ __forceinline__ void widen(float (&x)[V]) const {
 #pragma unroll
-      for (int i = 0; i < kBytes / 16; ++i) reinterpret_cast<uint4*>(p)[i] = u.w16[i];
-    } else if constexpr (kBytes == 8) {
-      *reinterpret_cast<uint2*>(p) = u.w8;
-    } else if constexpr (kBytes == 4) {
-      *reinterpret_cast<uint32_t*>(p) = u.w4;
-    } else if constexpr (kBytes == 2) {
-      *reinterpret_cast<uint16_t*>(p) = u.w2;
-    } else {
-      *reinterpret_cast<uint8_t*>(p) = u.w1;
-    }
+    for (int i = 0; i < V; ++i) x[i] = to_f<T>(e[i]);
   }
 };
+template <typename T, int V>
+__device__ __forceinline__ void store_raw(T* p, const float (&x)[V]) {
+  Raw<T, V> r;
+#pragma unroll
+  for (int i = 0; i < V; ++i) r.e[i] = from_f<T>(x[i]);
+  r.store(p);
+}
 
 // cos and sin of pos turns of F, with the sine's sign.
 __device__ __forceinline__ float2 phase(int32_t pos, uint64_t F, float sign) {
@@ -145,129 +153,144 @@ __device__ __forceinline__ float2 phase(int32_t pos, uint64_t F, float sign) {
   return make_float2(cs, sn * sign);
 }
 
-// The same division for every element: IEEE, so that a value next to a border
-// of the 8-bit type falls as x / scale says.
-template <typename C>
-__device__ __forceinline__ float stored(float x, float scale) {
-  if constexpr (sizeof(C) == 1) return __fdiv_rn(x, scale);
-  return x;
-}
+// What a thread holds of one head: two vectors of V elements, at lo and hi: V pairs to turn,
+// or up to 2V elements to copy.
+template <typename T, int V>
+struct Unit {
+  Raw<T, V> x, y;
+  T* out;     // q: where its head goes
+  int32_t t;  // token of the tile, -1: none
+  int32_t h;  // head: q's, then k's, then v's
+};
 
-template <typename T, typename C, int V, bool kInter>
-__device__ __forceinline__ void turn_unit(const T* in, C* out, int half, int unit,
-                                          const float2* cs, float scale) {
-  float a[V], b[V], x[V], y[V];
-  const int lo = kInter ? 2 * V * unit : V * unit;
-  const int hi = kInter ? lo + V : half + lo;
-  Vec<T, V>::load(in + lo, x);
-  Vec<T, V>::load(in + hi, y);
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    // interleaved: pairs are neighbours of the 2V elements x | y
-    a[i] = kInter ? (2 * i < V ? x[2 * i < V ? 2 * i : 0] : y[2 * i < V ? 0 : 2 * i - V]) : x[i];
-    b[i] = kInter ? (2 * i + 1 < V ? x[2 * i + 1 < V ? 2 * i + 1 : 0]
-                                   : y[2 * i + 1 < V ? 0 : 2 * i + 1 - V])
-                  : y[i];
-  }
-  float p[V], r[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const float2 w = cs[V * unit + i];
-    p[i] = stored<C>(a[i] * w.x - b[i] * w.y, scale);
-    r[i] = stored<C>(a[i] * w.y + b[i] * w.x, scale);
-  }
-#pragma unroll
-  for (int i = 0; i < V; ++i) {
-    if (kInter) {
-      if (2 * i < V) x[2 * i < V ? 2 * i : 0] = p[i];
-      else y[2 * i < V ? 0 : 2 * i - V] = p[i];
-      if (2 * i + 1 < V) x[2 * i + 1 < V ? 2 * i + 1 : 0] = r[i];
-      else y[2 * i + 1 < V ? 0 : 2 * i + 1 - V] = r[i];
-    } else {
-      x[i] = p[i];
-      y[i] = r[i];
-    }
-  }
-  Vec<C, V>::store(out + lo, x);
-  Vec<C, V>::store(out + hi, y);
-}
-
-template <typename T, typename C, int V>
-__device__ __forceinline__ void copy_unit(const T* in, C* out, int at, float scale) {
-  float x[V];
-  Vec<T, V>::load(in + at, x);
-  if constexpr (sizeof(C) == 1) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) x[i] = stored<C>(x[i], scale);
-  }
-  Vec<C, V>::store(out + at, x);
-}
-
+// Every head, of q, k or v, is cut into the same units, so a thread keeps its unit (lo, hi and
+// the pairs in between) and walks over heads; 256 / units heads go side by side.
 template <typename T, typename C, int V, bool kInter, bool kAppend>
-__global__ void __launch_bounds__(kThreads) k_rope(const __grid_constant__ Args a) {
-  __shared__ float2 cs[kTileAngles];
-  // a token's offsets: rope: its row in x and in out; append: its slot's rows in
-  // the two caches, and whether it has a slot
-  __shared__ int64_t first[kThreads], second[kThreads];
-  __shared__ bool slot[kThreads];
+__global__ void __launch_bounds__(kThreads, 4) k_rope(const __grid_constant__ Args a) {
+  __shared__ __align__(16) float2 cs[2][kTileAngles];
+  // append: a token's rows in the two caches, or kNone
+  __shared__ int64_t krow[2][kAppend ? kTileTokens : 1], vrow[2][kAppend ? kTileTokens : 1];
   const int tid = threadIdx.x;
-  const int plain = a.D / V;  // units of a head of v
-  const int per_q = a.q.H * a.units;
-  const int per_k = kAppend ? a.k.H * a.units : 0;
-  const int per_tok = per_q + per_k + (kAppend ? a.v.H * plain : 0);
+  const int mine = tid / a.units, unit = tid - mine * a.units;  // head of the pass, unit
+  const int lo = unit < a.rot_units ? (kInter ? 2 * V * unit : V * unit)
+                                    : 2 * a.half + 2 * V * (unit - a.rot_units);
+  const int hi = unit < a.rot_units && !kInter ? a.half + lo : lo + V;
+  const bool turns_ = unit < a.rot_units, two = hi < a.D, any = mine < a.pass;
+  // through a pointer that the compiler cannot see into: the lanes read different frequencies,
+  // which the constant cache would serve one at a time
+  const Turns* turns = &a.turns;
+  asm volatile("" : "+l"(turns));
+  Unit<T, V> u[kUnits];
+
+  auto load = [&](Unit<T, V>& w, int64_t t0, int all, int r0) {
+    const int row = r0 + mine;
+    w.t = -1;
+    if (!any || row >= all) return;
+    w.t = a.heads.div(row);
+    w.h = row - w.t * (int)a.heads.d;
+    const int64_t tok = t0 + w.t;
+    const T* in;
+    if (!kAppend || w.h < a.q.H) {
+      int64_t b = 0, s = tok;
+      if (!kAppend && a.S != a.tokens) {
+        b = a.tokens <= 0x7fffffff ? (int64_t)((uint32_t)tok / (uint32_t)a.S) : tok / a.S;
+        s -= b * a.S;
+      }
+      in = (const T*)a.q.in + b * a.q.in_b + s * a.q.in_s + w.h * a.q.in_h;
+      w.out = (T*)a.q.out + b * a.q.out_b + s * a.q.out_s + w.h * a.q.out_h;
+    } else {
+      const int h = w.h - a.q.H;
+      in = h < a.k.H ? (const T*)a.k.in + tok * a.k.in_s + h * a.k.in_h
+                     : (const T*)a.v.in + tok * a.v.in_s + (h - a.k.H) * a.v.in_h;
+    }
+    w.x.load(in + lo);
+    if (two) w.y.load(in + hi);
+  };
+  auto finish = [&](const Unit<T, V>& w, int buf) {
+    if (w.t < 0) return;
+    float x[V], y[V];
+    w.x.widen(x);
+    w.y.widen(y);
+    if (turns_ && (!kAppend || w.h < a.q.H + a.k.H)) {
+      float2 turn[V];
+      if constexpr (V == 1) {
+        turn[0] = cs[buf][w.t * a.half + unit];
+      } else {
+        // pairs 2j and 2j+1 of a unit lie together, those of all units after one another: the
+        // lanes of a warp read neighbouring 16 bytes
+        const float4* p =
+            reinterpret_cast<const float4*>(cs[buf]) + w.t * (V / 2) * a.rot_units + unit;
+#pragma unroll
+        for (int j = 0; j < V / 2; ++j) {
+          const float4 r = p[j * a.rot_units];
+          turn[2 * j] = make_float2(r.x, r.y);
+          turn[(2 * j + 1) % V] = make_float2(r.z, r.w);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const float2 r = turn[i];
+        // interleaved: the pairs are neighbours of the 2V elements x | y
+        float& p = kInter ? (2 * i < V ? x[2 * i % V] : y[2 * i % V]) : x[i];
+        float& q = kInter ? (2 * i + 1 < V ? x[(2 * i + 1) % V] : y[(2 * i + 1) % V]) : y[i];
+        const float b = p;
+        p = b * r.x - q * r.y;
+        q = b * r.y + q * r.x;
+      }
+    }
+    if (!kAppend || w.h < a.q.H) {
+      store_raw<T, V>(w.out + lo, x);
+      if (two) store_raw<T, V>(w.out + hi, y);
+      return;
+    }
+    const bool is_v = w.h >= a.q.H + a.k.H;
+    const int64_t row = is_v ? vrow[buf][w.t] : krow[buf][w.t];
+    if (row == kNone) return;
+    if constexpr (sizeof(C) == 1) {
+      // IEEE division, so that a value next to a border of the 8-bit type falls as x / scale says
+      const float scale = is_v ? a.v_scale : a.k_scale;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        x[i] = __fdiv_rn(x[i], scale);
+        y[i] = __fdiv_rn(y[i], scale);
+      }
+    }
+    C* out = is_v ? (C*)a.v.out + row + (w.h - a.q.H - a.k.H) * a.c_head_v
+                  : (C*)a.k.out + row + (w.h - a.q.H) * a.c_head_k;
+    store_raw<C, V>(out + lo, x);
+    if (two) store_raw<C, V>(out + hi, y);
+  };
+
+  int buf = 0;
   for (int64_t t0 = (int64_t)blockIdx.x * a.tile; t0 < a.tokens;
-       t0 += (int64_t)gridDim.x * a.tile) {
-    const int n = (int)min((int64_t)a.tile, a.tokens - t0);
-    __syncthreads();  // the tile before is read
+       t0 += (int64_t)gridDim.x * a.tile, buf ^= 1) {
+    const int n = (int)min((int64_t)a.tile, a.tokens - t0), all = n * (int)a.heads.d;
+#pragma unroll
+    for (int e = 0; e < kUnits; ++e) load(u[e], t0, all, e * a.pass);
+    // the angles, while the loads are under way
     for (int i = tid; i < n * a.half; i += kThreads) {
       const int t = i / a.half, f = i - t * a.half;
-      const int32_t pos = a.pos[a.turns.axis[f] * a.ld_pos + t0 + t];
-      cs[i] = phase(pos, a.turns.f[f], a.sign);
+      const float2 r = phase(a.pos[turns->axis[f] * a.ld_pos + t0 + t], turns->f[f], a.sign);
+      const int k = f / V, in = f % V;
+      cs[buf][V == 1 ? i : 2 * ((t * (V / 2) + in / 2) * a.rot_units + k) + in % 2] = r;
     }
     if (kAppend && tid < n) {
       const int32_t s = a.slots[t0 + tid];
       const int32_t page = s / a.bs, off = s - page * a.bs;
-      const bool there = s >= 0 && page < a.num_blocks;
-      if (!there && s != -1) atomicExch(&g_device_error, 3);
-      slot[tid] = there;
-      first[tid] = page * a.c_blk_k + off * a.c_tok_k;
-      second[tid] = page * a.c_blk_v + off * a.c_tok_v;
-    } else if (!kAppend && tid < n) {
-      const int64_t b = (t0 + tid) / a.S, s = t0 + tid - b * a.S;
-      first[tid] = b * a.q.in_b + s * a.q.in_s;
-      second[tid] = b * a.q.out_b + s * a.q.out_s;
+      const bool in = s >= 0 && page < a.num_blocks;
+      if (!in && s != -1) atomicExch(&g_device_error, 3);
+      krow[buf][tid] = in ? page * a.c_blk_k + off * a.c_tok_k : kNone;
+      vrow[buf][tid] = in ? page * a.c_blk_v + off * a.c_tok_v : kNone;
     }
+    // one barrier a tile: its buffers are written again two tiles on, behind the next barrier
     __syncthreads();
-    for (int i = tid; i < n * per_tok; i += kThreads) {
-      const int t = i / per_tok;
-      int u = i - t * per_tok;
-      const int64_t tok = t0 + t;
-      const float2* w = cs + t * a.half;
-      if (u < per_q) {
-        const int h = u / a.units;
-        u -= h * a.units;
-        const T* in = (const T*)a.q.in + (kAppend ? tok * a.q.in_s : first[t]) + h * a.q.in_h;
-        T* out = (T*)a.q.out + (kAppend ? tok * a.q.out_s : second[t]) + h * a.q.out_h;
-        if (u < a.rot_units) turn_unit<T, T, V, kInter>(in, out, a.half, u, w, 1.0f);
-        else copy_unit<T, T, V>(in, out, 2 * a.half + (u - a.rot_units) * V, 1.0f);
-      } else if (kAppend && slot[t]) {
-        u -= per_q;
-        if (u < per_k) {
-          const int h = u / a.units;
-          u -= h * a.units;
-          const T* in = (const T*)a.k.in + tok * a.k.in_s + h * a.k.in_h;
-          C* out = (C*)a.k.out + first[t] + h * a.c_head_k;
-          if (u < a.rot_units) turn_unit<T, C, V, kInter>(in, out, a.half, u, w, a.k_scale);
-          else copy_unit<T, C, V>(in, out, 2 * a.half + (u - a.rot_units) * V, a.k_scale);
-        } else {
-          u -= per_k;
-          const int h = u / plain;
-          u -= h * plain;
-          const T* in = (const T*)a.v.in + tok * a.v.in_s + h * a.v.in_h;
-          C* out = (C*)a.v.out + second[t] + h * a.c_head_v;
-          copy_unit<T, C, V>(in, out, u * V, a.v_scale);
-        }
-      }
+    for (int r0 = 0;;) {
+#pragma unroll
+      for (int e = 0; e < kUnits; ++e) finish(u[e], buf);
+      r0 += kUnits * a.pass;
+      if (r0 >= all) break;
+#pragma unroll
+      for (int e = 0; e < kUnits; ++e) load(u[e], t0, all, r0 + e * a.pass);
     }
   }
 }
@@ -276,10 +299,11 @@ inline int dtype_bytes(int dt) {
   return dt == REMORA_B200_F32 ? 4 : dt == REMORA_B200_E4M3 ? 1 : 2;
 }
 
-// The widest V in {8, 4, 1} that keeps every vector access aligned: the pairs'
-// halves, the plain tail, the strides and the bases.
+// The widest V in {8 (16-bit types only), 4, 1} that keeps every vector access
+// aligned: the pairs' halves, the plain tail, the strides and the bases.
 struct Fit {
-  int v = 8;
+  int v;
+  explicit Fit(int bytes) : v(bytes == 2 ? 8 : 4) {}
   void elems(int64_t n) { while (v > 1 && n % v) v = v == 8 ? 4 : 1; }
   void base(const void* p, int bytes) {
     while (v > 1 && reinterpret_cast<uintptr_t>(p) % (v * bytes < 16 ? v * bytes : 16))
@@ -297,27 +321,39 @@ struct Fit {
 
 template <typename T, typename C, bool kAppend>
 int launch(Args& a, int v, int interleaved, cudaStream_t st) {
-  const int plain = a.D / v;
   a.rot_units = a.half / v;
-  a.units = a.rot_units + (a.D - 2 * a.half) / v;
-  const int64_t per_tok = (int64_t)a.q.H * a.units +
-                          (kAppend ? (int64_t)a.k.H * a.units + (int64_t)a.v.H * plain : 0);
-  // enough tokens for two units a thread, but no more than the angles' room
-  int64_t tile = (2 * kThreads + per_tok - 1) / per_tok;
-  tile = std::min<int64_t>({tile, kTileAngles / std::max(a.half, 8), kThreads});
-  a.tile = (int)std::max<int64_t>(tile, 1);
+  a.units = (a.D / v + 1) / 2;  // = rot_units + ceil of half the rest
+  a.pass = kThreads / a.units;  // D <= 512: at least one
+  const int heads = a.q.H + (kAppend ? a.k.H + a.v.H : 0);
+  a.heads = Divisor((uint32_t)heads);
+  // as many tokens as fill passes of kUnits heads a thread best (the fewest of those), within
+  // the angles' room, and no more than leave every SM a tile
+  const int64_t chunk = kUnits * a.pass;
+  const int64_t room = std::min<int64_t>(kTileAngles / std::max(a.half, 1), kTileTokens);
+  const int64_t most = std::max<int64_t>(std::min(room, a.tokens / num_sms()), 1);
+  a.tile = 1;
+  double best = 0;
+  for (int64_t t = 1; t <= most; ++t) {
+    const double fill = (double)(t * heads) / ((t * heads + chunk - 1) / chunk * chunk);
+    if (fill > best + 0.01) {
+      best = fill;
+      a.tile = (int)t;
+    }
+  }
   const int64_t tiles = (a.tokens + a.tile - 1) / a.tile;
   const int grid = (int)std::min<int64_t>(tiles, (int64_t)num_sms() * 8);
 #define RB_ROPE(VV, I) k_rope<T, C, VV, I, kAppend><<<grid, kThreads, 0, st>>>(a)
-  if (interleaved) {
-    if (v == 8) RB_ROPE(8, true);
-    else if (v == 4) RB_ROPE(4, true);
-    else RB_ROPE(1, true);
-  } else {
-    if (v == 8) RB_ROPE(8, false);
-    else if (v == 4) RB_ROPE(4, false);
-    else RB_ROPE(1, false);
-  }
+#define RB_ROPE_V(I)                          \
+  do {                                        \
+    if constexpr (sizeof(T) == 2) {           \
+      if (v == 8) RB_ROPE(8, I);              \
+    }                                         \
+    if (v == 4) RB_ROPE(4, I);                \
+    else if (v == 1) RB_ROPE(1, I);           \
+  } while (0)
+  if (interleaved) RB_ROPE_V(true);
+  else RB_ROPE_V(false);
+#undef RB_ROPE_V
 #undef RB_ROPE
   RB_LAUNCH_CHECK();
   return REMORA_B200_OK;
@@ -327,7 +363,7 @@ int launch(Args& a, int v, int interleaved, cudaStream_t st) {
 inline int angles(const char* who, Args& a, const int32_t* positions, int64_t ld_pos, int n_axes,
                   const double* freq, const int32_t* axis_of, int64_t rot, int64_t D,
                   int64_t tokens) {
-  RB_CHECK_ARG(D >= 1 && D <= 1024, "%s: head_dim must be in [1, 1024], got %lld", who,
+  RB_CHECK_ARG(D >= 1 && D <= 512, "%s: head_dim must be in [1, 512], got %lld", who,
                (long long)D);
   RB_CHECK_ARG(rot >= 0 && rot % 2 == 0 && rot <= 2 * kMaxHalf && rot <= D,
                "%s: rot must be even, at most head_dim and at most %d, got %lld", who,
@@ -381,7 +417,7 @@ extern "C" int remora_b200_rope(const remora_b200_rope_args* args, void* stream)
   a.q = Heads{p.x, p.out, p.x_b, p.x_s, p.x_h, p.out_b, p.out_s, p.out_h, (int32_t)H};
   a.sign = p.inverse ? -1.0f : 1.0f;
   const int e = dtype_bytes(p.dtype);
-  Fit f;
+  Fit f(e);
   f.elems(a.half);
   f.elems(D);
   f.rows(p.x, e, B > 1 ? p.x_b : 0, p.x_s, p.x_h);
@@ -438,7 +474,7 @@ extern "C" int remora_b200_rope_kv_append(const remora_b200_rope_kv_append_args*
   a.v_scale = p.v_scale;
   a.sign = 1.0f;
   const int c = dtype_bytes(p.cache_dtype);
-  Fit f;
+  Fit f(2);
   f.elems(a.half);
   f.elems(D);
   if (Hq) {
