@@ -187,7 +187,8 @@ int remora_b200_attention_fwd_bf16(const void* q, const void* k, const void* v, 
  * addressed by element strides of block, token and head (the head_dim
  * elements of a row are adjacent), so [block][token][head][dim] and
  * [block][head][token][dim] are both taken as they lie.  An E4M3 cache
- * stores x / scale, rounded to nearest even and saturated at +-448.
+ * stores x / scale, rounded to nearest even and saturated at +-448 (scales
+ * in [1e-30, 1e30]).
  * Values that only the device sees (block ids, slots, lengths) are checked
  * there: a bad one is skipped and reported by remora_b200_device_status()
  * as REMORA_B200_ERR_INVALID.
@@ -240,8 +241,9 @@ int remora_b200_kv_block_table(const remora_b200_kv_block_table_args* args, void
  * device.  freq (rot / 2 doubles) and axis_of (rot / 2 ints, NULL = all 0)
  * are HOST arrays, read before the call returns.  rot even, <= min(D, 256);
  * D <= 512; n_axes <= 8.  Angles are exact to 2^-25 of a quarter turn at
- * every 32-bit position.  Any strides; sizes, strides and bases that are
- * multiples of 8 elements (and 16 bytes) move 8 pairs at a time. */
+ * every 32-bit position.  Any strides (of tokens and heads below 2^31
+ * elements), at most 2^30 tokens; sizes, strides and bases that are multiples
+ * of 8 elements (and 16 bytes) move 8 pairs at a time. */
 typedef struct remora_b200_rope_args {
   const void* x;
   void* out;

@@ -868,8 +868,8 @@ extern "C" int remora_b200_paged_attention(const remora_b200_paged_attention_arg
                "least max_blocks");
   RB_CHECK_ARG(std::isfinite(p.scale), "paged_attention: scale is not finite");
   RB_CHECK_ARG(p.window >= 0, "paged_attention: window must not be negative");
-  RB_CHECK_ARG(std::isfinite(p.k_scale) && p.k_scale > 0 && std::isfinite(p.v_scale) && p.v_scale > 0,
-               "paged_attention: the cache scales must be positive and finite");
+  RB_CHECK_ARG(rope::scale_ok(p.k_scale) && rope::scale_ok(p.v_scale),
+               "paged_attention: the cache scales must lie in [1e-30, 1e30]");
   RB_CHECK_ARG(p.cache_dtype == REMORA_B200_E4M3 || (p.k_scale == 1.0f && p.v_scale == 1.0f),
                "paged_attention: the scales must be 1 unless the cache is E4M3");
   if (R == 0) return REMORA_B200_OK;

@@ -33,7 +33,7 @@
 namespace rb {
 namespace rope {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 constexpr int kMaxHalf = 128;     // pairs of a head: rot <= 256
 constexpr int kMaxAxes = 8;
 constexpr int kTileAngles = 1024;  // pairs of one tile of tokens in shared memory
@@ -46,12 +46,14 @@ struct Turns {
   uint8_t axis[kMaxHalf];
 };
 
-// One tensor of heads: rows [token][head][D], strides in elements.  A token is
-// b * S + s; a plain [token] stride has S = all tokens.
+// One tensor of heads: rows [token][head][D], strides in elements (of tokens and
+// heads in 32 bits, so that an address is one multiply-add each).  A token is
+// b * S + s.
 struct Heads {
   const void* in;
   void* out;
-  int64_t in_b, in_s, in_h, out_b, out_s, out_h;
+  int64_t in_b, out_b;
+  int32_t in_s, in_h, out_s, out_h;
   int32_t H;
 };
 
@@ -74,8 +76,9 @@ struct Args {
   const int32_t* pos;
   int64_t ld_pos;
   const int32_t* slots;
-  int64_t tokens, S;
   int64_t c_blk_k, c_tok_k, c_head_k, c_blk_v, c_tok_v, c_head_v;
+  int32_t tokens, S;
+  Divisor batch;      // S
   int32_t num_blocks, bs;
   int32_t D, half, n_axes;
   int32_t tile;       // tokens of a block's iteration
@@ -83,60 +86,107 @@ struct Args {
   int32_t units;      // those and the units of 2V plain elements behind them
   int32_t pass;       // heads side by side: kThreads / units
   Divisor heads;      // of a token
-  float k_scale, v_scale;
+  float k_scale, v_scale, k_inverse, v_inverse;
   float sign;
   Turns turns;
 };
 
-template <typename T> __device__ __forceinline__ float to_f(T v);
-template <> __device__ __forceinline__ float to_f(float v) { return v; }
-template <> __device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float(v); }
-template <> __device__ __forceinline__ float to_f(__half v) { return __half2float(v); }
-template <typename T> __device__ __forceinline__ T from_f(float v);
-template <> __device__ __forceinline__ float from_f(float v) { return v; }
-template <> __device__ __forceinline__ __nv_bfloat16 from_f(float v) {
-  return __float2bfloat16_rn(v);
+// Two neighbouring elements at a time (one for V = 1): the conversions of a pair are one
+// instruction each way.
+__device__ __forceinline__ float2 widen2(uint32_t w, __nv_bfloat16) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
-template <> __device__ __forceinline__ __half from_f(float v) { return __float2half_rn(v); }
-template <> __device__ __forceinline__ __nv_fp8_e4m3 from_f(float v) {
-  __nv_fp8_e4m3 r;
-  r.__x = __nv_cvt_float_to_fp8(v, __NV_SATFINITE, __NV_E4M3);
-  return r;
+__device__ __forceinline__ float2 widen2(uint32_t w, __half) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+__device__ __forceinline__ uint32_t narrow2(float x, float y, __nv_bfloat16) {
+  return pack_bf16x2(x, y);
+}
+__device__ __forceinline__ uint32_t narrow2(float x, float y, __half) {
+  const __half2 h = __floats2half2_rn(x, y);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint16_t narrow2(float x, float y, __nv_fp8_e4m3) {
+  return __nv_cvt_float2_to_fp8x2(make_float2(x, y), __NV_SATFINITE, __NV_E4M3);
 }
 
 // V elements in accesses of up to 16 bytes (V * sizeof(T) is a power of two;
 // the host checked that every address is a multiple of it, up to 16).
 template <typename T, int V>
-struct alignas(V * sizeof(T) < 16 ? V * sizeof(T) : 16) Raw {
+struct Raw {
   static constexpr int kBytes = V * (int)sizeof(T);
-  using Piece = typename std::conditional<
-      kBytes >= 16, uint4,
-      typename std::conditional<
-          kBytes == 8, uint2,
-          typename std::conditional<kBytes == 4, uint32_t,
-                                    typename std::conditional<kBytes == 2, uint16_t,
-                                                              uint8_t>::type>::type>::type>::type;
-  static constexpr int kPieces = kBytes / (int)sizeof(Piece);
-  T e[V];
-  __device__ __forceinline__ Piece* pieces() { return reinterpret_cast<Piece*>(e); }
+  static constexpr int kWords = kBytes >= 4 ? kBytes / 4 : 1;
+  uint32_t w[kWords];
   __device__ __forceinline__ void load(const T* p) {  // read once: not kept in the caches
+    if constexpr (kBytes >= 16) {
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) pieces()[i] = __ldcs(reinterpret_cast<const Piece*>(p) + i);
+      for (int i = 0; i < kBytes / 16; ++i) {
+        const uint4 v = __ldcs(reinterpret_cast<const uint4*>(p) + i);
+        w[4 * i] = v.x;
+        w[4 * i + 1] = v.y;
+        w[4 * i + 2] = v.z;
+        w[4 * i + 3] = v.w;
+      }
+    } else if constexpr (kBytes == 8) {
+      const uint2 v = __ldcs(reinterpret_cast<const uint2*>(p));
+      w[0] = v.x;
+      w[1] = v.y;
+    } else if constexpr (kBytes == 4) {
+      w[0] = __ldcs(reinterpret_cast<const uint32_t*>(p));
+    } else {
+      w[0] = __ldcs(reinterpret_cast<const uint16_t*>(p));
+    }
   }
-  __device__ __forceinline__ void store(T* p) {
+  __device__ __forceinline__ void store(T* p) const {
+    if constexpr (kBytes >= 16) {
 #pragma unroll
-    for (int i = 0; i < kPieces; ++i) reinterpret_cast<Piece*>(p)[i] = pieces()[i];
+      for (int i = 0; i < kBytes / 16; ++i)
+        reinterpret_cast<uint4*>(p)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2],
+                                                    w[4 * i + 3]);
+    } else if constexpr (kBytes == 8) {
+      *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+    } else if constexpr (kBytes == 4) {
+      *reinterpret_cast<uint32_t*>(p) = w[0];
+    } else if constexpr (kBytes == 2) {
+      *reinterpret_cast<uint16_t*>(p) = (uint16_t)w[0];
+    } else {
+      *reinterpret_cast<uint8_t*>(p) = (uint8_t)w[0];
+    }
   }
   __device__ __forceinline__ void widen(float (&x)[V]) const {
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) x[i] = to_f<T>(e[i]);
+      for (int i = 0; i < V; ++i) x[i] = __uint_as_float(w[i]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < (V + 1) / 2; ++i) {
+        const float2 f = widen2(w[i], T());
+        x[2 * i] = f.x;
+        if constexpr (V > 1) x[2 * i + 1] = f.y;
+      }
+    }
+  }
+  __device__ __forceinline__ void narrow(const float (&x)[V]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) w[i] = __float_as_uint(x[i]);
+    } else if constexpr (V == 1) {
+      w[0] = narrow2(x[0], 0.0f, T());
+    } else if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i) w[i] = narrow2(x[2 * i], x[2 * i + 1], T());
+    } else {
+#pragma unroll
+      for (int i = 0; i < V / 4; ++i)
+        w[i] = narrow2(x[4 * i], x[4 * i + 1], T()) |
+               (uint32_t)narrow2(x[4 * i + 2], x[4 * i + 3], T()) << 16;
+    }
   }
 };
 template <typename T, int V>
 __device__ __forceinline__ void store_raw(T* p, const float (&x)[V]) {
   Raw<T, V> r;
-#pragma unroll
-  for (int i = 0; i < V; ++i) r.e[i] = from_f<T>(x[i]);
+  r.narrow(x);
   r.store(p);
 }
 
@@ -153,6 +203,17 @@ __device__ __forceinline__ float2 phase(int32_t pos, uint64_t F, float sign) {
   return make_float2(cs, sn * sign);
 }
 
+// x / scale, rounded to nearest, from the rounded inverse of scale: a residual in one fused
+// step corrects the product (Markstein, "Computation of elementary functions on the IBM RISC
+// System/6000 processor", 1990).  So a value next to a border of the 8-bit type falls as the
+// division says.  Beyond 512 the 8-bit type is saturated and the plain product does (the
+// residual of an infinite one would be NaN).
+__device__ __forceinline__ float divided(float x, float scale, float inverse) {
+  const float q = x * inverse;
+  const float r = fmaf(fmaf(-q, scale, x), inverse, q);
+  return fabsf(q) < 512.0f ? r : q;
+}
+
 // What a thread holds of one head: two vectors of V elements, at lo and hi: V pairs to turn,
 // or up to 2V elements to copy.
 template <typename T, int V>
@@ -164,9 +225,9 @@ struct Unit {
 };
 
 // Every head, of q, k or v, is cut into the same units, so a thread keeps its unit (lo, hi and
-// the pairs in between) and walks over heads; 256 / units heads go side by side.
+// the pairs in between) and walks over heads; 128 / units heads go side by side.
 template <typename T, typename C, int V, bool kInter, bool kAppend>
-__global__ void __launch_bounds__(kThreads, 4) k_rope(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(kThreads, 8) k_rope(const __grid_constant__ Args a) {
   __shared__ __align__(16) float2 cs[2][kTileAngles];
   // append: a token's rows in the two caches, or kNone
   __shared__ int64_t krow[2][kAppend ? kTileTokens : 1], vrow[2][kAppend ? kTileTokens : 1];
@@ -182,26 +243,30 @@ __global__ void __launch_bounds__(kThreads, 4) k_rope(const __grid_constant__ Ar
   asm volatile("" : "+l"(turns));
   Unit<T, V> u[kUnits];
 
-  auto load = [&](Unit<T, V>& w, int64_t t0, int all, int r0) {
+  auto load = [&](Unit<T, V>& w, int t0, int all, int r0) {
     const int row = r0 + mine;
     w.t = -1;
     if (!any || row >= all) return;
     w.t = a.heads.div(row);
     w.h = row - w.t * (int)a.heads.d;
-    const int64_t tok = t0 + w.t;
+    const int tok = t0 + w.t;
     const T* in;
     if (!kAppend || w.h < a.q.H) {
-      int64_t b = 0, s = tok;
-      if (!kAppend && a.S != a.tokens) {
-        b = a.tokens <= 0x7fffffff ? (int64_t)((uint32_t)tok / (uint32_t)a.S) : tok / a.S;
-        s -= b * a.S;
+      in = (const T*)a.q.in + (int64_t)w.h * a.q.in_h;
+      w.out = (T*)a.q.out + (int64_t)w.h * a.q.out_h;
+      if (kAppend || a.S == a.tokens) {
+        in += (int64_t)tok * a.q.in_s;
+        w.out += (int64_t)tok * a.q.out_s;
+      } else {
+        const int b = a.batch.div(tok), s = tok - b * a.S;
+        in += b * a.q.in_b + (int64_t)s * a.q.in_s;
+        w.out += b * a.q.out_b + (int64_t)s * a.q.out_s;
       }
-      in = (const T*)a.q.in + b * a.q.in_b + s * a.q.in_s + w.h * a.q.in_h;
-      w.out = (T*)a.q.out + b * a.q.out_b + s * a.q.out_s + w.h * a.q.out_h;
     } else {
       const int h = w.h - a.q.H;
-      in = h < a.k.H ? (const T*)a.k.in + tok * a.k.in_s + h * a.k.in_h
-                     : (const T*)a.v.in + tok * a.v.in_s + (h - a.k.H) * a.v.in_h;
+      in = h < a.k.H
+               ? (const T*)a.k.in + (int64_t)tok * a.k.in_s + (int64_t)h * a.k.in_h
+               : (const T*)a.v.in + (int64_t)tok * a.v.in_s + (int64_t)(h - a.k.H) * a.v.in_h;
     }
     w.x.load(in + lo);
     if (two) w.y.load(in + hi);
@@ -247,12 +312,12 @@ __global__ void __launch_bounds__(kThreads, 4) k_rope(const __grid_constant__ Ar
     const int64_t row = is_v ? vrow[buf][w.t] : krow[buf][w.t];
     if (row == kNone) return;
     if constexpr (sizeof(C) == 1) {
-      // IEEE division, so that a value next to a border of the 8-bit type falls as x / scale says
       const float scale = is_v ? a.v_scale : a.k_scale;
+      const float inverse = is_v ? a.v_inverse : a.k_inverse;
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        x[i] = __fdiv_rn(x[i], scale);
-        y[i] = __fdiv_rn(y[i], scale);
+        x[i] = divided(x[i], scale, inverse);
+        y[i] = divided(y[i], scale, inverse);
       }
     }
     C* out = is_v ? (C*)a.v.out + row + (w.h - a.q.H - a.k.H) * a.c_head_v
@@ -262,9 +327,9 @@ __global__ void __launch_bounds__(kThreads, 4) k_rope(const __grid_constant__ Ar
   };
 
   int buf = 0;
-  for (int64_t t0 = (int64_t)blockIdx.x * a.tile; t0 < a.tokens;
-       t0 += (int64_t)gridDim.x * a.tile, buf ^= 1) {
-    const int n = (int)min((int64_t)a.tile, a.tokens - t0), all = n * (int)a.heads.d;
+  const int step = gridDim.x * a.tile;
+  for (int t0 = blockIdx.x * a.tile; t0 < a.tokens; t0 += step, buf ^= 1) {
+    const int n = min(a.tile, a.tokens - t0), all = n * (int)a.heads.d;
 #pragma unroll
     for (int e = 0; e < kUnits; ++e) load(u[e], t0, all, e * a.pass);
     // the angles, while the loads are under way
@@ -294,6 +359,9 @@ __global__ void __launch_bounds__(kThreads, 4) k_rope(const __grid_constant__ Ar
     }
   }
 }
+
+inline bool fits32(int64_t stride) { return stride < (1ll << 31) && stride > -(1ll << 31); }
+inline bool scale_ok(float s) { return s >= 1e-30f && s <= 1e30f; }
 
 inline int dtype_bytes(int dt) {
   return dt == REMORA_B200_F32 ? 4 : dt == REMORA_B200_E4M3 ? 1 : 2;
@@ -330,7 +398,7 @@ int launch(Args& a, int v, int interleaved, cudaStream_t st) {
   // the angles' room, and no more than leave every SM a tile
   const int64_t chunk = kUnits * a.pass;
   const int64_t room = std::min<int64_t>(kTileAngles / std::max(a.half, 1), kTileTokens);
-  const int64_t most = std::max<int64_t>(std::min(room, a.tokens / num_sms()), 1);
+  const int64_t most = std::max<int64_t>(std::min<int64_t>(room, a.tokens / num_sms()), 1);
   a.tile = 1;
   double best = 0;
   for (int64_t t = 1; t <= most; ++t) {
@@ -340,8 +408,8 @@ int launch(Args& a, int v, int interleaved, cudaStream_t st) {
       a.tile = (int)t;
     }
   }
-  const int64_t tiles = (a.tokens + a.tile - 1) / a.tile;
-  const int grid = (int)std::min<int64_t>(tiles, (int64_t)num_sms() * 8);
+  const int64_t tiles = ((int64_t)a.tokens + a.tile - 1) / a.tile;
+  const int grid = (int)std::min<int64_t>(tiles, (int64_t)num_sms() * 16);
 #define RB_ROPE(VV, I) k_rope<T, C, VV, I, kAppend><<<grid, kThreads, 0, st>>>(a)
 #define RB_ROPE_V(I)                          \
   do {                                        \
@@ -370,7 +438,8 @@ inline int angles(const char* who, Args& a, const int32_t* positions, int64_t ld
                2 * kMaxHalf, (long long)rot);
   RB_CHECK_ARG(n_axes >= 1 && n_axes <= kMaxAxes, "%s: n_axes must be in [1, %d], got %d", who,
                kMaxAxes, n_axes);
-  RB_CHECK_ARG(tokens >= 0 && tokens <= (1ll << 40), "%s: bad number of tokens", who);
+  RB_CHECK_ARG(tokens >= 0 && tokens <= (1ll << 30), "%s: at most 2^30 tokens, got %lld", who,
+               (long long)tokens);
   RB_CHECK_ARG(rot == 0 || freq, "%s: freq is null", who);
   RB_CHECK_ARG(rot == 0 || tokens == 0 || positions, "%s: positions is null", who);
   RB_CHECK_ARG(n_axes == 1 || ld_pos >= tokens, "%s: ld_pos must be at least the tokens", who);
@@ -379,7 +448,7 @@ inline int angles(const char* who, Args& a, const int32_t* positions, int64_t ld
   a.n_axes = n_axes;
   a.pos = positions;
   a.ld_pos = ld_pos;
-  a.tokens = tokens;
+  a.tokens = (int32_t)tokens;
   for (int i = 0; i < a.half; ++i) {
     RB_CHECK_ARG(std::isfinite(freq[i]), "%s: freq[%d] is not finite", who, i);
     const int ax = axis_of ? axis_of[i] : 0;
@@ -407,14 +476,18 @@ extern "C" int remora_b200_rope(const remora_b200_rope_args* args, void* stream)
   RB_CHECK_ARG(p.dtype == REMORA_B200_BF16 || p.dtype == REMORA_B200_F16 || p.dtype == REMORA_B200_F32,
                "rope: dtype must be BF16, F16 or F32");
   RB_CHECK_ARG(B >= 0 && S >= 0 && H >= 0 && H <= 65536, "rope: bad shape");
-  RB_CHECK_ARG(B <= (1ll << 31) && S <= (1ll << 31), "rope: bad shape");
+  RB_CHECK_ARG(B <= (1ll << 30) && S <= (1ll << 30), "rope: bad shape");
   Args a = {};
   int rc = angles("rope", a, p.positions, p.ld_pos, p.n_axes, p.freq, p.axis_of, p.rot, D, B * S);
   if (rc) return rc;
   if (B * S * H == 0) return REMORA_B200_OK;
   RB_CHECK_ARG(p.x && p.out, "rope: null pointer");
-  a.S = S;
-  a.q = Heads{p.x, p.out, p.x_b, p.x_s, p.x_h, p.out_b, p.out_s, p.out_h, (int32_t)H};
+  RB_CHECK_ARG(fits32(p.x_s) && fits32(p.x_h) && fits32(p.out_s) && fits32(p.out_h),
+               "rope: strides of tokens and heads must be below 2^31 elements");
+  a.S = (int32_t)S;
+  a.batch = Divisor((uint32_t)S);
+  a.q = Heads{p.x, p.out, p.x_b, p.out_b, (int32_t)p.x_s, (int32_t)p.x_h, (int32_t)p.out_s,
+              (int32_t)p.out_h, (int32_t)H};
   a.sign = p.inverse ? -1.0f : 1.0f;
   const int e = dtype_bytes(p.dtype);
   Fit f(e);
@@ -447,8 +520,8 @@ extern "C" int remora_b200_rope_kv_append(const remora_b200_rope_kv_append_args*
   RB_CHECK_ARG(p.block_size >= 1 && p.num_blocks >= 1 && p.block_size <= 0x7fffffff &&
                    p.num_blocks <= 0x7fffffff / p.block_size,
                "rope_kv_append: num_blocks * block_size must be in [1, 2^31)");
-  RB_CHECK_ARG(std::isfinite(p.k_scale) && p.k_scale > 0 && std::isfinite(p.v_scale) && p.v_scale > 0,
-               "rope_kv_append: the scales must be positive and finite");
+  RB_CHECK_ARG(scale_ok(p.k_scale) && scale_ok(p.v_scale),
+               "rope_kv_append: the scales must lie in [1e-30, 1e30]");
   RB_CHECK_ARG(p.cache_dtype == REMORA_B200_E4M3 || (p.k_scale == 1.0f && p.v_scale == 1.0f),
                "rope_kv_append: the scales must be 1 unless the cache is E4M3");
   Args a = {};
@@ -457,10 +530,14 @@ extern "C" int remora_b200_rope_kv_append(const remora_b200_rope_kv_append_args*
   if (T == 0) return REMORA_B200_OK;
   RB_CHECK_ARG((Hq == 0 || (p.q && p.q_out)) && p.k && p.v && p.slots && p.k_cache && p.v_cache,
                "rope_kv_append: null pointer");
-  a.S = T;
-  a.q = Heads{p.q, p.q_out, 0, p.q_t, p.q_h, 0, p.q_out_t, p.q_out_h, (int32_t)Hq};
-  a.k = Heads{p.k, p.k_cache, 0, p.k_t, p.k_h, 0, 0, 0, (int32_t)Hkv};
-  a.v = Heads{p.v, p.v_cache, 0, p.v_t, p.v_h, 0, 0, 0, (int32_t)Hkv};
+  RB_CHECK_ARG(fits32(p.q_t) && fits32(p.q_h) && fits32(p.k_t) && fits32(p.k_h) &&
+                   fits32(p.v_t) && fits32(p.v_h) && fits32(p.q_out_t) && fits32(p.q_out_h),
+               "rope_kv_append: strides of tokens and heads must be below 2^31 elements");
+  a.S = (int32_t)T;
+  a.q = Heads{p.q, p.q_out, 0, 0, (int32_t)p.q_t, (int32_t)p.q_h, (int32_t)p.q_out_t,
+              (int32_t)p.q_out_h, (int32_t)Hq};
+  a.k = Heads{p.k, p.k_cache, 0, 0, (int32_t)p.k_t, (int32_t)p.k_h, 0, 0, (int32_t)Hkv};
+  a.v = Heads{p.v, p.v_cache, 0, 0, (int32_t)p.v_t, (int32_t)p.v_h, 0, 0, (int32_t)Hkv};
   a.slots = p.slots;
   a.num_blocks = (int32_t)p.num_blocks;
   a.bs = (int32_t)p.block_size;
@@ -472,6 +549,8 @@ extern "C" int remora_b200_rope_kv_append(const remora_b200_rope_kv_append_args*
   a.c_head_v = p.vc_head;
   a.k_scale = p.k_scale;
   a.v_scale = p.v_scale;
+  a.k_inverse = 1.0f / p.k_scale;
+  a.v_inverse = 1.0f / p.v_scale;
   a.sign = 1.0f;
   const int c = dtype_bytes(p.cache_dtype);
   Fit f(2);

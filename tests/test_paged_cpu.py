@@ -61,7 +61,8 @@ def rope(L, **c):
     dict(x=None), dict(out=None), dict(dt=rb.E4M3), dict(dt=9), dict(B=-1), dict(S=-1), dict(H=-1),
     dict(D=0), dict(D=2048), dict(pos=None), dict(ld=3, axes=2), dict(axes=0), dict(axes=9),
     dict(freq=None), dict(ax=AXES), dict(rot=3), dict(rot=130), dict(rot=258, D=512),
-    dict(x=A + 1), dict(freq=NAN), dict(freq=INF)])
+    dict(x=A + 1), dict(freq=NAN), dict(freq=INF), dict(xs=2 ** 31),
+    dict(oh=-2 ** 31), dict(S=2 ** 30 + 1, ld=2 ** 31), dict(B=2 ** 20, S=2 ** 20, ld=2 ** 41)])
 def test_rope_refuses(L, bad):
     assert rope(L, **bad) == rb.ERR_INVALID and "rope" in rb.last_error()
 
@@ -85,6 +86,7 @@ def append(L, **c):
     dict(vc=None), dict(pos=None), dict(dt=rb.F32), dict(cdt=rb.F16), dict(T=-1), dict(Hkv=0),
     dict(nb=0), dict(bs=0), dict(nb=2 ** 28), dict(ks=0.0), dict(vs=-1.0), dict(ks=2.0),
     dict(cdt=rb.E4M3, ks=float("nan")), dict(cdt=rb.E4M3, vs=float("inf")), dict(rot=200),
+    dict(cdt=rb.E4M3, ks=1e-31), dict(cdt=rb.E4M3, vs=1e31), dict(qt=2 ** 31), dict(T=2 ** 31),
     dict(kc=A + 1)])
 def test_append_refuses(L, bad):
     assert append(L, **bad) == rb.ERR_INVALID and "rope_kv_append" in rb.last_error()
@@ -105,7 +107,7 @@ def attention(L, **c):
     dict(wsb=0), dict(dt=rb.F32), dict(cdt=rb.F16), dict(R=-1), dict(R=8193), dict(Hq=7),
     dict(Hkv=0), dict(Hq=0), dict(D=96), dict(nb=0), dict(bs=0), dict(nb=2 ** 28), dict(mb=0),
     dict(ld=7), dict(mb=2 ** 28, ld=2 ** 28), dict(scale=float("nan")), dict(scale=float("inf")),
-    dict(window=-1), dict(ks=0.5), dict(vs=2.0), dict(cdt=rb.E4M3, ks=0.0),
+    dict(window=-1), dict(ks=0.5), dict(vs=2.0), dict(cdt=rb.E4M3, ks=0.0), dict(cdt=rb.E4M3, vs=1e31),
     dict(cdt=rb.E4M3, kt=264), dict(qt=1020), dict(oh=4), dict(kt=12), dict(vb=4)])
 def test_attention_refuses(L, bad):
     assert attention(L, **bad) == rb.ERR_INVALID and "paged_attention" in rb.last_error()

@@ -294,6 +294,25 @@ def test_append_e4m3_saturates_and_keeps_nan(rb):
     np.testing.assert_array_equal(vc.float().cpu().view(-1).numpy(), np.array(want, np.float32))
 
 
+@pytest.mark.parametrize("scale", [0.031, 1.7e-30, 9.1e29, 3.0, 448.0])
+def test_append_e4m3_rounds_as_the_division(rb, scale):
+    """Values over the whole of bf16 (every exponent and mantissa, both signs): the stored byte
+    is that of the exact quotient x / scale, rounded once."""
+    bits = torch.arange(0, 1 << 16, 1, dtype=torch.int32)
+    x = bits.to(torch.int16).view(torch.bfloat16)
+    x = x[x.isfinite()][:65024].view(-1, 1, 64)
+    T = x.shape[0]
+    kc = torch.zeros(T, 1, 1, 64, dtype=torch.float8_e4m3fn, device="cuda")
+    vc = kc.clone()
+    rb.rope_kv_append(x.cuda(), x.cuda(), x.cuda(), i32(np.zeros(T)), i32(np.arange(T)), freqs(0),
+                      kc, vc, k_scale=scale, v_scale=scale)
+    # the quotient in 64 bits, rounded to 32 as the division is, then to 8
+    s32 = float(np.float32(scale))
+    want = (x.double() / s32).float().clamp(-448, 448).to(torch.float8_e4m3fn)
+    for c in (kc, vc):
+        assert torch.equal(c.view(T, 1, 64).cpu().float(), want.float())
+
+
 def test_append_reports_bad_slots(rb):
     x = torch.ones(3, 1, 64, dtype=torch.bfloat16, device="cuda")
     kc = torch.zeros(2, 4, 1, 64, dtype=torch.bfloat16, device="cuda")
