@@ -21,7 +21,9 @@ namespace paged {
 
 constexpr int kMaxRequests = 8192;
 constexpr int kRingBytes = 196608;  // shared memory of a CTA's rings
-constexpr int kMinTiles = 2;        // tiles of a warp at least
+constexpr int kItemCost = 2;         // what starting and ending an item costs, in tiles
+constexpr int kMinShare = 4;        // tiles and items' costs of a warp at least
+constexpr int kMostWarps = 8;
 
 struct Args {
   const void *q, *kc, *vc;
@@ -31,7 +33,11 @@ struct Args {
   int64_t q_t, q_h, o_t, o_h;
   int64_t kc_b, kc_t, kc_h, vc_b, vc_t, vc_h;
   int64_t ld_table, window;
+  int64_t k_step, v_step;  // bytes between the rows of a warp's consecutive copies
   int32_t R, Hq, Hkv, D, num_blocks, bs, max_blocks;
+  int32_t gq;        // query heads of a kv head
+  Divisor page;      // bs
+  int32_t whole16;   // 16 keys from a multiple of 16 on share a block
   float scale2, v_scale;  // scale2 = scale * log2(e) * the keys' scale
 };
 
@@ -112,10 +118,12 @@ struct Shape {
   static constexpr int CH = RB / 16;                // 16-byte pieces of a row
   static constexpr int KT = RB <= 128 ? 32 : 16;    // keys of a tile
   static constexpr int SB = 2 * KT * RB;            // a tile's keys and values
-  static constexpr int W = SB > 8192 ? 4 : 8;       // warps
+  static constexpr int W = SB > 8192 ? 4 : SB > 4096 ? 8 : kMostWarps;  // warps
   static constexpr int S = kRingBytes / (W * SB) > 6 ? 6 : kRingBytes / (W * SB);
   static constexpr size_t kSmem = (size_t)W * S * SB;
   static_assert(S >= 2 && kSmem <= kRingBytes, "ring");
+  // a warp's two parts, 16 heads each at most, fit into its ring
+  static_assert(2 * (D == 256 ? 8 : 16) * (D + 2) * 4 <= S * SB, "parts");
 };
 
 // Piece c of row `row` lies at piece c ^ swz(row): the eight rows of an ldmatrix
@@ -134,18 +142,47 @@ __device__ __forceinline__ void tiles_of(const Args& a, int32_t len, int KT, int
   t1 = (int)(((int64_t)n + KT - 1) / KT);
 }
 
+// 16 bytes into shared memory at `dst`; zeros, and nothing read, if there is nothing.
+__device__ __forceinline__ void copy16(uint32_t dst, const char* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy16(uint32_t dst, const char* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src),
+               "r"(there ? 16 : 0)
+               : "memory");
+}
+
+// 2^x; results below 2^-126 are 0.
+__device__ __forceinline__ float exp2_ftz(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 struct Stage {  // what the reader of a tile needs to know
   uint32_t mask;   // keys that count
-  int32_t r, h;    // the item
+  int32_t r, h;    // the item; r < 0: no tile, the walk is over
   uint32_t flags;  // 1: first tile of this worker's part, 2: first of the item, 4: last of the
-                   // item; the item's tiles behind this one << 3
+                   // item, 8: last of the worker
 };
 
+// Shares of this lane's request: its tiles and an item's cost, or 0.  For one item.
+__device__ __forceinline__ int32_t shares_of(const Args& a, int32_t len, int KT) {
+  int t0, t1;
+  tiles_of(a, len, KT, t0, t1);
+  return t0 < t1 ? t1 - t0 + kItemCost : 0;
+}
+// The sum over a warp of values below 2^28.
+__device__ __forceinline__ int64_t warp_sum(int32_t v) {
+  return (int64_t)__reduce_add_sync(~0u, (unsigned)v & 0xffffu) +
+         ((int64_t)__reduce_add_sync(~0u, (unsigned)v >> 16) << 16);
+}
+
 // A warp's walk over its tiles, as it fetches them.
-template <typename C, int D>
+template <typename T, typename C, int D, int kHeads>
 struct Walk {
   using X = Shape<C, D>;
-  int64_t left;        // tiles not fetched yet
+  int64_t at, end;     // the tile to come and the end of the walk, in shares
   int32_t g, r, h;     // group of 32 requests, request, item of the request
   int32_t t, t0, t1;   // tile, and the request's
   int32_t n, start;    // the request's keys [start, n)
@@ -171,21 +208,23 @@ struct Walk {
     id = -1;
     off = 0;
     if (ok) {
-      const int32_t page = key / a.bs;
+      const int32_t page = a.page.div(key);
       off = key - page * a.bs;
       id = __ldg(a.table + (int64_t)r * a.ld_table + page);
     }
   }
   __device__ __forceinline__ void next(const Args& a, int Hg, int lane) {
     ++t;
+    ++at;
     fresh = false;
     if (t == t1) {
       fresh = true;
+      at += kItemCost;
       if (++h == Hg) {
         h = 0;
         do {
-          if (++r >= a.R) {  // only if the lengths changed under the call: end, do not spin
-            left = 0;
+          if (++r >= a.R) {  // the last item is done
+            at = end;
             return;
           }
           if ((r & 31) == 0) {
@@ -197,38 +236,76 @@ struct Walk {
       }
       t = t0;
     }
+    if (at < end) look_up(a, lane);
   }
-  // Starts the copies of the next tile into `ring` (a stage), or commits nothing.
+  // Starts the copies of the next tile into `ring` (a stage), or commits nothing.  With the
+  // walk's last tile, *item_end = the share of its item's last tile.
   __device__ __forceinline__ void fetch(const Args& a, int Hg, int ngr, char* ring, Stage* st,
-                                        int lane) {
-    if (left > 0) {
+                                        int64_t* item_end, int lane) {
+    if (at < end) {
       const bool in = ok && id >= 0 && id < a.num_blocks;
       if (ok && !in) atomicExch(&g_device_error, 3);
-      const uint32_t mask = __ballot_sync(~0u, in) & (X::KT == 32 ? ~0u : 0xffffu);
-      const int hk = h / ngr;
-      int64_t ko = 0, vo = 0;
-      if (in) {
-        ko = id * a.kc_b + off * a.kc_t + hk * a.kc_h;
-        vo = id * a.vc_b + off * a.vc_t + hk * a.vc_h;
+      constexpr uint32_t kAll = X::KT == 32 ? ~0u : 0xffffu;
+      const uint32_t mask = __ballot_sync(~0u, in) & kAll;
+      const int hk = ngr == 1 ? h : h / ngr;
+      const Stage about{mask, r, h,
+                        (fresh ? 1u : 0u) | (t == t0 ? 2u : 0u) | (t == t1 - 1 ? 4u : 0u)};
+      const int64_t ends_at = at + (t1 - 1 - t);
+      if (fresh) {  // the item's queries are read when its first tile has come
+        constexpr int kLines = D * 2 / 128;
+        const T* qp = (const T*)a.q + r * a.q_t + (hk * a.gq + (h - hk * ngr) * kHeads) * a.q_h;
+        for (int i = lane; i < kHeads * kLines; i += 32)
+          if ((h - hk * ngr) * kHeads + i / kLines < a.gq)
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(qp + i / kLines * a.q_h +
+                                                          i % kLines * 64));
       }
-      if (lane == 0) {
-        const uint32_t f = (fresh ? 1u : 0u) | (t == t0 ? 2u : 0u) | (t == t1 - 1 ? 4u : 0u);
-        *st = Stage{mask, r, h, f | (uint32_t)(t1 - 1 - t) << 3};
-      }
-      char* kd = ring;
-      char* vd = ring + X::KT * X::RB;
+      // a warp's copy instruction: kRows rows, lane / CH the row, lane % CH its piece
+      constexpr int kRows = 32 / X::CH, kSteps = X::KT / kRows;
+      const int lr = lane / X::CH, c = lane % X::CH;
+      const uint32_t kd = smem_u32(ring) + lr * X::RB, vd = kd + X::KT * X::RB;
+      if (a.whole16 && mask == kAll) {
+        // every key counts, and the rows of 16 keys follow one another in their block: one
+        // address for each 16, then steps of kRows rows
 #pragma unroll
-      for (int i = 0; i < X::KT * X::CH / 32; ++i) {
-        const int p = i * 32 + lane, row = p / X::CH, c = p % X::CH;
-        const int64_t k1 = __shfl_sync(~0u, ko, row), v1 = __shfl_sync(~0u, vo, row);
-        const bool there = mask >> row & 1;
-        const int at = row * X::RB + ((c ^ swz<X::RB>(row)) << 4);
-        cp_async16(kd + at, (const char*)a.kc + k1 * (int64_t)sizeof(C) + c * 16, there);
-        cp_async16(vd + at, (const char*)a.vc + v1 * (int64_t)sizeof(C) + c * 16, there);
+        for (int g16 = 0; g16 < X::KT / 16; ++g16) {
+          const int64_t b = __shfl_sync(~0u, id, 16 * g16), o = __shfl_sync(~0u, off, 16 * g16) + lr;
+          const char* ks = (const char*)a.kc +
+                           (b * a.kc_b + o * a.kc_t + (int64_t)hk * a.kc_h) * (int)sizeof(C) + c * 16;
+          const char* vs = (const char*)a.vc +
+                           (b * a.vc_b + o * a.vc_t + (int64_t)hk * a.vc_h) * (int)sizeof(C) + c * 16;
+#pragma unroll
+          for (int i = 0; i < 16 / kRows; ++i) {
+            const int row = 16 * g16 + i * kRows;  // and lr more
+            const int at = row * X::RB + ((c ^ swz<X::RB>(row + lr)) << 4);
+            copy16(kd + at, ks);
+            copy16(vd + at, vs);
+            ks += a.k_step;
+            vs += a.v_step;
+          }
+        }
+      } else {
+        int64_t ko = 0, vo = 0;
+        if (in) {
+          ko = id * a.kc_b + off * a.kc_t + hk * a.kc_h;
+          vo = id * a.vc_b + off * a.vc_t + hk * a.vc_h;
+        }
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+          const int row = i * kRows + lr;
+          const int64_t k1 = __shfl_sync(~0u, ko, row), v1 = __shfl_sync(~0u, vo, row);
+          const bool there = mask >> row & 1;
+          const int at = i * kRows * X::RB + ((c ^ swz<X::RB>(row)) << 4);
+          copy16(kd + at, (const char*)a.kc + k1 * (int)sizeof(C) + c * 16, there);
+          copy16(vd + at, (const char*)a.vc + v1 * (int)sizeof(C) + c * 16, there);
+        }
       }
-      if (--left > 0) {
-        next(a, Hg, lane);
-        if (left > 0) look_up(a, lane);
+      next(a, Hg, lane);
+      if (lane == 0) {
+        *st = about;
+        if (at >= end) {
+          st->flags |= 8u;
+          *item_end = ends_at;
+        }
       }
     } else if (lane == 0) {
       st->r = -1;
@@ -268,7 +345,7 @@ __device__ __forceinline__ float lse_of(float m, float l) {
 }
 // 2^(m - top), where top may be -inf (then so is m: nothing was seen).
 __device__ __forceinline__ float weight(float m, float top) {
-  return exp2f(m - (top == -INFINITY ? 0.0f : top));
+  return exp2_ftz(m - (top == -INFINITY ? 0.0f : top));
 }
 
 // A partial result: fragments [nt][j][lane] as float4, then m[8 NT], l[8 NT].
@@ -299,28 +376,28 @@ __global__ void __launch_bounds__(Shape<C, D>::W * 32, 1)
   __shared__ int64_t before[kMaxRequests / 32 + 1];
   __shared__ Stage stages[W][S];
   __shared__ int32_t p_item[2 * W], p_flag[2 * W];
-  __shared__ uint32_t p_rest;
+  __shared__ int64_t p_end[W];
+  __shared__ float p_w[2 * W][8 * NT], p_m[2 * W][8 * NT], p_l[2 * W][8 * NT];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t4 = lane & 3;
-  const int gq = a.Hq / a.Hkv, ngr = (gq + 8 * NT - 1) / (8 * NT), Hg = a.Hkv * ngr;
+  const int gq = a.gq, ngr = (gq + 8 * NT - 1) / (8 * NT), Hg = a.Hkv * ngr;
 
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the kernel before is done
 
-  // tiles before each group of 32 requests
+  // The work in shares: each tile one, and kItemCost for each item (request and group of heads)
+  // in front of its tiles.  Every worker (warp) gets the same number of shares, a range of them,
+  // and with it the tiles in that range.  Shares before each group of 32 requests:
   const int groups = (a.R + 31) / 32;
   for (int i = warp; i < groups; i += W) {
     const int r = i * 32 + lane;
-    int t0 = 0, t1 = 0;
-    if (r < a.R) tiles_of(a, a.lens[r], KT, t0, t1);
-    int64_t c = (int64_t)max(t1 - t0, 0) * Hg;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) c += __shfl_xor_sync(~0u, c, o);
+    const int64_t c = warp_sum(r < a.R ? shares_of(a, a.lens[r], KT) : 0) * Hg;
     if (lane == 0) before[i + 1] = c;
   }
   if (threadIdx.x < 2 * W) p_item[threadIdx.x] = -1;
-  if (threadIdx.x == 0) { before[0] = 0; p_rest = 0; }
+  if (threadIdx.x == 0) before[0] = 0;
   __syncthreads();
-  if (warp == 0) {
+  if (groups > 1 && warp == 0) {
     int64_t sum = 0;
     for (int i = 0; i < groups; i += 32) {
       int64_t c = i + lane < groups ? before[i + lane + 1] : 0;
@@ -333,11 +410,11 @@ __global__ void __launch_bounds__(Shape<C, D>::W * 32, 1)
       sum += __shfl_sync(~0u, c, 31);
     }
   }
-  __syncthreads();
+  if (groups > 1) __syncthreads();
   const int64_t total = before[groups];
   const int64_t workers = (int64_t)gridDim.x * W, worker = (int64_t)blockIdx.x * W + warp;
-  const int64_t quota = max((total + workers - 1) / workers, (int64_t)kMinTiles);
-  const int64_t begin = min(worker * quota, total), tiles = min(begin + quota, total) - begin;
+  const int64_t quota = max((total + workers - 1) / workers, (int64_t)kMinShare);
+  const int64_t begin = worker * quota;
 
   // requests without keys; lengths that are out of range
   for (int64_t r = worker; r < a.R; r += workers) {
@@ -358,9 +435,9 @@ __global__ void __launch_bounds__(Shape<C, D>::W * 32, 1)
   }
 
   char* ring = ring_all + (size_t)warp * S * X::SB;
-  if (tiles > 0) {
-    Walk<C, D> w;
-    w.left = tiles;
+  if (begin < total) {
+    Walk<T, C, D, 8 * NT> w;
+    w.at = w.end = min(begin + quota, total);
     {
       int lo = 0, hi = groups;  // before[lo] <= begin < before[hi]
       while (hi - lo > 1) {
@@ -370,53 +447,62 @@ __global__ void __launch_bounds__(Shape<C, D>::W * 32, 1)
       }
       w.g = lo;
       w.load_group(a, lane);
-      int t0, t1;
-      tiles_of(a, w.glen, KT, t0, t1);
-      int64_t c = (int64_t)max(t1 - t0, 0) * Hg;
+      int64_t c = (int64_t)shares_of(a, w.glen, KT) * Hg;
+      const int64_t mine = c;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int64_t y = __shfl_up_sync(~0u, c, o);
         if (lane >= o) c += y;
       }
-      const int64_t at = begin - before[lo];
-      // (a request that covers the tile: there is one unless the lengths change under the call)
-      const int l = max(__ffs(__ballot_sync(~0u, c > at)) - 1, 0);
-      const int64_t prev = __shfl_sync(~0u, c, l > 0 ? l - 1 : 0);
+      const int64_t want = begin - before[lo];
+      // (a request that holds the share: there is one unless the lengths change under the call)
+      const int l = max(__ffs(__ballot_sync(~0u, c > want)) - 1, 0);
+      const int64_t in = want - __shfl_sync(~0u, c - mine, l);
       w.r = lo * 32 + l;
       w.set_request(a);
-      const int64_t in = at - (l > 0 ? prev : 0), each = max(w.t1 - w.t0, 1);
-      w.h = (int)(in / each);
-      w.t = w.t0 + (int)(in - w.h * each);
+      // in / each, below 2^16: the float quotient is off by less than one
+      const int64_t each = max(w.t1 - w.t0, 1) + kItemCost;
+      w.h = (int)__fdividef((float)in, (float)each);
+      if (w.h * each > in) --w.h;
+      else if ((w.h + 1) * each <= in) ++w.h;
+      const int skip = max((int)(in - w.h * each) - kItemCost, 0);  // tiles of earlier workers
+      w.t = w.t0 + skip;
       w.fresh = true;
-      if (w.r < a.R && w.t < w.t1 && in >= 0 && w.h < Hg) w.look_up(a, lane);
-      else w.left = 0;
+      const int64_t at = begin - in + w.h * each + kItemCost + skip;
+      if (w.r < a.R && w.t < w.t1 && in >= 0 && w.h >= 0 && w.h < Hg && at < w.end) {
+        w.at = at;
+        w.look_up(a, lane);
+      }
     }
 #pragma unroll
-    for (int s = 0; s < S - 1; ++s) w.fetch(a, Hg, ngr, ring + s * X::SB, &stages[warp][s], lane);
+    for (int s = 0; s < S - 1; ++s) 
+      w.fetch(a, Hg, ngr, ring + s * X::SB, &stages[warp][s], &p_end[warp], lane);
 
     uint32_t q[D / 16][2 * NT];
     float o[NT][D / 16][4];
     float m[NT], l[NT], sc[NT];
     bool began = false;
+    int head0 = 0, heads = 0;  // the item's query heads
     const int lrow = lane & 7, lhalf = (lane >> 3) & 1, lsec = lane >> 4;
     // where this lane points ldmatrix: 16-bit rows (keys by lsec, d's by lhalf), 8-bit the reverse
     const int frow = (F8 ? lhalf : lsec) * 8 + lrow, fpiece = F8 ? lsec : lhalf;
     const int fswz = swz<X::RB>(lrow);
     int rs = 0, ws = S - 1;  // stage to read, stage to fill
-    for (int64_t i = 0; i < tiles; ++i) {
+    while (true) {
       cp_async_wait<S - 2>();
       __syncwarp();
-      w.fetch(a, Hg, ngr, ring + ws * X::SB, &stages[warp][ws], lane);
+      w.fetch(a, Hg, ngr, ring + ws * X::SB, &stages[warp][ws], &p_end[warp], lane);
       ws = ws + 1 == S ? 0 : ws + 1;
       const Stage st = stages[warp][rs];
       const uint32_t kb = smem_u32(ring + rs * X::SB), vb = kb + KT * X::RB;
       rs = rs + 1 == S ? 0 : rs + 1;
       if (st.r < 0) break;
-      const int sub = st.h % ngr, head0 = st.h / ngr * gq + sub * 8 * NT;
-      const int heads = min(8 * NT, gq - sub * 8 * NT);
 
       if (st.flags & 1) {  // a new item: its queries, and nothing seen
+        const int sub = st.h % ngr;
         began = st.flags & 2;
+        head0 = st.h / ngr * gq + sub * 8 * NT;
+        heads = min(8 * NT, gq - sub * 8 * NT);
         const T* qp = (const T*)a.q + st.r * a.q_t + head0 * a.q_h;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -521,7 +607,7 @@ __global__ void __launch_bounds__(Shape<C, D>::W * 32, 1)
         top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
         top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
         base[n] = top == -INFINITY ? 0.0f : top;
-        c[n] = exp2f(m[n] - base[n]);
+        c[n] = exp2_ftz(m[n] - base[n]);
         grew |= top > m[n];
         m[n] = top;
       }
@@ -547,7 +633,8 @@ __global__ void __launch_bounds__(Shape<C, D>::W * 32, 1)
       for (int n = 0; n < NT; ++n)
 #pragma unroll
         for (int k = 0; k < KT / 8; ++k) {
-          const float x = exp2f(s[k][2 * n] - base[n]), y = exp2f(s[k][2 * n + 1] - base[n]);
+          const float x = exp2_ftz(s[k][2 * n] - base[n]);
+          const float y = exp2_ftz(s[k][2 * n + 1] - base[n]);
           l[n] += x + y;
           ph[n][k] = pack2<M>(x, y);
           const float2 w = unpack2<M>(ph[n][k]);
@@ -585,8 +672,8 @@ __global__ void __launch_bounds__(Shape<C, D>::W * 32, 1)
         }
       }
 
-      const bool ends = st.flags & 4;
-      if (ends || i == tiles - 1) {  // the end of this warp's part of the item
+      const bool ends = st.flags & 4, last = st.flags & 8;
+      if (ends || last) {  // the end of this warp's part of the item
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           l[n] += __shfl_xor_sync(~0u, l[n], 1);
@@ -609,7 +696,6 @@ __global__ void __launch_bounds__(Shape<C, D>::W * 32, 1)
         } else {
           // a part: the first of several is put aside in the workspace, the last one in this
           // warp's ring, which is then free
-          const bool last = i == tiles - 1;
           if (last) {
             cp_async_wait<0>();
             __syncwarp();
@@ -630,55 +716,76 @@ __global__ void __launch_bounds__(Shape<C, D>::W * 32, 1)
             const int e = 2 * warp + (last ? 1 : 0);
             p_item[e] = st.r * Hg + st.h;
             p_flag[e] = (began ? 1 : 0) | (ends ? 2 : 0);
-            if (last && !ends && warp == W - 1) p_rest = st.flags >> 3;
           }
         }
       }
+      if (last) break;
+    }
+    if (p_item[2 * warp] >= 0) {  // the first part joins the last in the ring
+      cp_async_wait<0>();
+      __syncwarp();
+      const float4* from = reinterpret_cast<const float4*>(room.first + worker * PF);
+      float4* to = reinterpret_cast<float4*>(ring) + PF / 4;
+#pragma unroll
+      for (int i = 0; i < (PF / 4 + 31) / 32; ++i)
+        if (i * 32 + lane < PF / 4) to[i * 32 + lane] = from[i * 32 + lane];
     }
   }
   cp_async_wait<0>();
   __syncthreads();
 
-  // Join the CTA's own parts.  Parts of one item are neighbours in the order of the warps; a
-  // run that lacks the item's first or last tile crosses into another CTA.
+  // Join the CTA's own parts: entry 2w is warp w's first part, 2w + 1 its last.  Parts of one
+  // item are neighbours in that order; a run that lacks the item's first or last tile crosses
+  // into another CTA.
+  auto part = [&](int e) {
+    return reinterpret_cast<const float*>(ring_all + (size_t)(e >> 1) * S * X::SB) +
+           (e & 1 ? 0 : PF);
+  };
+  const int my_item = lane < 2 * W ? p_item[lane] : -1;
+  const uint32_t same = __match_any_sync(~0u, my_item);
+  uint32_t leads = __ballot_sync(~0u, my_item >= 0 && (same & ((1u << lane) - 1)) == 0);
+  if (leads) {  // (the same in all warps)
+    const int we = threadIdx.x / (8 * NT), wh = threadIdx.x % (8 * NT);
+    const uint32_t peers = __shfl_sync(~0u, same, we & 31);
+    static_assert(2 * W * 8 * NT <= W * 32 && 32 % (8 * NT) == 0, "a thread per entry and head");
+    if (we < 2 * W && p_item[we] >= 0) {
+      float top = -INFINITY;
+      for (uint32_t b = peers; b; b &= b - 1) top = fmaxf(top, part(__ffs(b) - 1)[NT * 8 * D + wh]);
+      p_w[we][wh] = weight(part(we)[NT * 8 * D + wh], top);
+      if ((peers & ((1u << we) - 1)) == 0) {
+        float sum = 0;
+        for (uint32_t b = peers; b; b &= b - 1) {
+          const float* p = part(__ffs(b) - 1) + NT * 8 * D + wh;
+          sum += weight(p[0], top) * p[8 * NT];
+        }
+        p_m[we][wh] = top;
+        p_l[we][wh] = sum;
+      }
+    }
+  }
+  __syncthreads();
   Cross cross{-1, 0, {0, 0}};
-  for (int e0 = 0; e0 < 2 * W;) {
-    const int item = p_item[e0];
-    if (item < 0) { ++e0; continue; }
-    int e1 = e0, tail = e0;
-    for (int e = e0; e < 2 * W && (p_item[e] == item || p_item[e] < 0); ++e)
-      if (p_item[e] == item) { tail = e; e1 = e + 1; }
+  for (; leads; leads &= leads - 1) {
+    const int e0 = __ffs(leads) - 1;
+    const uint32_t run = __shfl_sync(~0u, same, e0);
+    const int tail = 31 - __clz(run), item = p_item[e0];
     const bool has0 = p_flag[e0] & 1, has1 = p_flag[tail] & 2;
     const int r = item / Hg, h = item - r * Hg, sub = h % ngr, head0 = h / ngr * gq + sub * 8 * NT;
     const int heads = min(8 * NT, gq - sub * 8 * NT);
-    auto part = [&](int e) {
-      return e & 1 ? reinterpret_cast<const float*>(ring_all + (size_t)(e >> 1) * S * X::SB)
-                   : room.first + ((int64_t)blockIdx.x * W + (e >> 1)) * PF;
-    };
     float* to = room.cross + ((int64_t)blockIdx.x * 2 + (has0 ? 1 : 0)) * PF;
     for (int f = warp; f < NT * (D / 16); f += W) {
       const int n = f / (D / 16), j = f % (D / 16), hh = n * 8 + 2 * t4;
-      float m0 = -INFINITY, m1 = -INFINITY;
-      for (int e = e0; e < e1; ++e)
-        if (p_item[e] == item) {
-          const float* p = part(e) + NT * 8 * D;
-          m0 = fmaxf(m0, p[hh]);
-          m1 = fmaxf(m1, p[hh + 1]);
-        }
       float4 c = make_float4(0, 0, 0, 0);
-      float l0 = 0, l1 = 0;
-      for (int e = e0; e < e1; ++e)
-        if (p_item[e] == item) {
-          const float* p = part(e);
-          const float w0 = weight(p[NT * 8 * D + hh], m0), w1 = weight(p[NT * 8 * D + hh + 1], m1);
-          const float4 v = reinterpret_cast<const float4*>(p)[f * 32 + lane];
-          c.x += w0 * v.x;
-          c.y += w1 * v.y;
-          c.z += w0 * v.z;
-          c.w += w1 * v.w;
-          l0 += w0 * p[NT * 8 * (D + 1) + hh];
-          l1 += w1 * p[NT * 8 * (D + 1) + hh + 1];
-        }
+      for (uint32_t b = run; b; b &= b - 1) {
+        const int e = __ffs(b) - 1;
+        const float2 w = *reinterpret_cast<const float2*>(&p_w[e][hh]);
+        const float4 v = reinterpret_cast<const float4*>(part(e))[f * 32 + lane];
+        c.x += w.x * v.x;
+        c.y += w.y * v.y;
+        c.z += w.x * v.z;
+        c.w += w.y * v.w;
+      }
+      const float m0 = p_m[e0][hh], m1 = p_m[e0][hh + 1], l0 = p_l[e0][hh], l1 = p_l[e0][hh + 1];
       if (has0 && has1) {
         const float i0 = l0 == 0.0f ? 0.0f : a.v_scale / l0;
         const float i1 = l1 == 0.0f ? 0.0f : a.v_scale / l1;
@@ -691,19 +798,15 @@ __global__ void __launch_bounds__(Shape<C, D>::W * 32, 1)
       } else {
         reinterpret_cast<float4*>(to)[f * 32 + lane] = c;
         if (j == 0 && g == 0) {
-          to[NT * 8 * D + hh] = m0;
-          to[NT * 8 * D + hh + 1] = m1;
-          to[NT * 8 * (D + 1) + hh] = l0;
-          to[NT * 8 * (D + 1) + hh + 1] = l1;
+          *reinterpret_cast<float2*>(to + NT * 8 * D + hh) = make_float2(m0, m1);
+          *reinterpret_cast<float2*>(to + NT * 8 * (D + 1) + hh) = make_float2(l0, l1);
         }
       }
     }
     if (has0 && !has1) {
-      const int64_t end = min(total, (int64_t)(blockIdx.x + 1) * W * quota);
       cross.item = item;
-      cross.last = (int)((end + p_rest - 1) / (W * quota));
+      cross.last = (int)(p_end[tail >> 1] / (W * quota));
     }
-    e0 = e1;
   }
   if (threadIdx.x == 0) room.about[blockIdx.x] = cross;
 }
@@ -719,8 +822,9 @@ __global__ void __launch_bounds__(kJoinWarps * 32)
   __shared__ float4 sc[kJoinWarps][32];
   __shared__ float sm[kJoinWarps][32][2], sl[kJoinWarps][32][2];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int gq = a.Hq / a.Hkv, ngr = (gq + 8 * NT - 1) / (8 * NT), Hg = a.Hkv * ngr;
+  const int gq = a.gq, ngr = (gq + 8 * NT - 1) / (8 * NT), Hg = a.Hkv * ngr;
   const int cta = blockIdx.x, f = blockIdx.y;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int item = __ldcg(&room.about[cta].item), last = __ldcg(&room.about[cta].last);
   if (item < 0) return;
@@ -787,8 +891,10 @@ inline int64_t part_floats(int64_t Hq, int64_t Hkv, int64_t D) {
 }
 
 template <typename T, typename C, int D, int NT>
-int launch(const Args& a, void* workspace, cudaStream_t st) {
+int launch(Args& a, void* workspace, cudaStream_t st) {
   using X = Shape<C, D>;
+  a.k_step = a.kc_t * (int64_t)sizeof(C) * (32 / X::CH);
+  a.v_step = a.vc_t * (int64_t)sizeof(C) * (32 / X::CH);
   constexpr int PF = kPartFloats<D, NT>;
   auto split = k_paged_split<T, C, D, NT>;
   RB_CUDA(cudaFuncSetAttribute(split, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -796,31 +902,36 @@ int launch(const Args& a, void* workspace, cudaStream_t st) {
   // no more CTAs than the tables' room has tiles for
   const int ngr = (a.Hq / a.Hkv + 8 * NT - 1) / (8 * NT);
   const int64_t room_tiles = ((int64_t)a.max_blocks * a.bs + X::KT - 1) / X::KT + 1;
-  const int64_t most = (room_tiles * a.R * a.Hkv * ngr + kMinTiles * X::W - 1) / (kMinTiles * X::W);
+  const int64_t most =
+      (room_tiles + kItemCost) * a.R * a.Hkv * ngr / (kMinShare * X::W) + 1;
   const int sms = num_sms();
   const int grid = (int)std::min<int64_t>(sms, std::max<int64_t>(most, 1));
   Room room;
   room.first = static_cast<float*>(workspace);
   room.cross = room.first + (int64_t)sms * X::W * PF;
   room.about = reinterpret_cast<Cross*>(room.cross + (int64_t)sms * 2 * PF);
-  split<<<grid, X::W * 32, X::kSmem, st>>>(a, room);
-  RB_LAUNCH_CHECK();
-  if (grid == 1) return REMORA_B200_OK;  // nothing crosses
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid, NT * (D / 16));
-  cfg.blockDim = dim3(kJoinWarps * 32);
-  cfg.stream = st;
+  // both may be set up while the kernel before is ending; they wait for its end themselves
   cudaLaunchAttribute at;
   at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(X::W * 32);
+  cfg.dynamicSmemBytes = X::kSmem;
+  cfg.stream = st;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
+  RB_CUDA(cudaLaunchKernelEx(&cfg, split, a, room));
+  if (grid == 1) return REMORA_B200_OK;  // nothing crosses
+  cfg.gridDim = dim3(grid, NT * (D / 16));
+  cfg.blockDim = dim3(kJoinWarps * 32);
+  cfg.dynamicSmemBytes = 0;
   RB_CUDA(cudaLaunchKernelEx(&cfg, k_paged_join<T, C, D, NT>, a, room));
   return REMORA_B200_OK;
 }
 
 template <typename T, typename C>
-int launch_shape(const Args& a, void* ws, cudaStream_t st) {
+int launch_shape(Args& a, void* ws, cudaStream_t st) {
   const int nt = head_tiles(a.Hq, a.Hkv, a.D);
   if (a.D == 64) return nt == 2 ? launch<T, C, 64, 2>(a, ws, st) : launch<T, C, 64, 1>(a, ws, st);
   if (a.D == 128)
@@ -841,7 +952,7 @@ extern "C" size_t remora_b200_paged_attention_workspace_bytes(int64_t R, int64_t
   using namespace rb::paged;
   if (!shape_ok(R, Hq, Hkv, D)) return 0;
   const int64_t sms = rb::num_sms();
-  return (size_t)(sms * (8 + 2) * part_floats(Hq, Hkv, D) * 4 + sms * (int64_t)sizeof(Cross));
+  return (size_t)(sms * (kMostWarps + 2) * part_floats(Hq, Hkv, D) * 4 + sms * (int64_t)sizeof(Cross));
 }
 
 extern "C" int remora_b200_paged_attention(const remora_b200_paged_attention_args* args,
@@ -885,10 +996,38 @@ extern "C" int remora_b200_paged_attention(const remora_b200_paged_attention_arg
   const size_t need = remora_b200_paged_attention_workspace_bytes(R, Hq, Hkv, D);
   RB_CHECK_ARG(p.workspace && p.workspace_bytes >= need && aligned16(p.workspace),
                "paged_attention: workspace of %zu bytes, 16-byte aligned, is needed", need);
-  Args a{p.q, p.k_cache, p.v_cache, p.block_table, p.lens, p.out, p.lse, p.q_t, p.q_h, p.out_t, p.out_h, p.kc_block,
-         p.kc_token, p.kc_head, p.vc_block, p.vc_token, p.vc_head, p.ld_table, p.window, (int32_t)R, (int32_t)Hq,
-         (int32_t)Hkv, (int32_t)D, (int32_t)p.num_blocks, (int32_t)p.block_size, (int32_t)p.max_blocks,
-         p.scale * 1.4426950408889634f * p.k_scale, p.v_scale};
+  Args a = {};
+  a.q = p.q;
+  a.kc = p.k_cache;
+  a.vc = p.v_cache;
+  a.table = p.block_table;
+  a.lens = p.lens;
+  a.out = p.out;
+  a.lse = p.lse;
+  a.q_t = p.q_t;
+  a.q_h = p.q_h;
+  a.o_t = p.out_t;
+  a.o_h = p.out_h;
+  a.kc_b = p.kc_block;
+  a.kc_t = p.kc_token;
+  a.kc_h = p.kc_head;
+  a.vc_b = p.vc_block;
+  a.vc_t = p.vc_token;
+  a.vc_h = p.vc_head;
+  a.ld_table = p.ld_table;
+  a.window = p.window;
+  a.R = (int32_t)R;
+  a.Hq = (int32_t)Hq;
+  a.Hkv = (int32_t)Hkv;
+  a.D = (int32_t)D;
+  a.gq = (int32_t)(Hq / Hkv);
+  a.num_blocks = (int32_t)p.num_blocks;
+  a.bs = (int32_t)p.block_size;
+  a.max_blocks = (int32_t)p.max_blocks;
+  a.page = Divisor((uint32_t)p.block_size);
+  a.whole16 = p.block_size % 16 == 0;
+  a.scale2 = p.scale * 1.4426950408889634f * p.k_scale;
+  a.v_scale = p.v_scale;
   cudaStream_t st = as_stream(stream);
   const bool f8 = p.cache_dtype == REMORA_B200_E4M3;
   if (p.dtype == REMORA_B200_BF16)

@@ -57,20 +57,6 @@ struct Heads {
   int32_t H;
 };
 
-// Division of n < 2^31 by d, as a multiplication: m = floor(2^(31 + s) / d) + 1 with 2^s >= d
-// is off by at most 2^s / d < 1 per n / 2^31, which never carries into the quotient.
-struct Divisor {
-  uint32_t d, m, s;
-  Divisor() = default;
-  explicit Divisor(uint32_t d_) : d(d_), s(0) {
-    while ((1ull << s) < d) ++s;
-    m = (uint32_t)((1ull << (31 + s)) / d + 1);
-  }
-  __device__ __forceinline__ int div(int n) const {
-    return (int)((uint64_t)(uint32_t)n * m >> (31 + s));
-  }
-};
-
 struct Args {
   Heads q, k, v;  // k and v: out is the cache, addressed by slot
   const int32_t* pos;

@@ -55,6 +55,20 @@ inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// Division of n < 2^31 by d, as a multiplication: m = floor(2^(31 + s) / d) + 1 with 2^s >= d
+// is off by at most 2^s / d < 1 per n / 2^31, which never carries into the quotient.
+struct Divisor {
+  uint32_t d, m, s;
+  Divisor() = default;
+  explicit Divisor(uint32_t d_) : d(d_), s(0) {
+    while ((1ull << s) < d) ++s;
+    m = (uint32_t)((1ull << (31 + s)) / d + 1);
+  }
+  __device__ __forceinline__ int div(int n) const {
+    return (int)((uint64_t)(uint32_t)n * m >> (31 + s));
+  }
+};
+
 // ---------------------------------------------------------- tensor maps
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
                                    const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
