@@ -22,7 +22,7 @@ namespace paged {
 constexpr int kMaxRequests = 8192;
 constexpr int kRingBytes = 196608;  // shared memory of a CTA's rings
 constexpr int kItemCost = 2;         // what starting and ending an item costs, in tiles
-constexpr int kMinShare = 4;        // tiles and items' costs of a warp at least
+constexpr int kMinShare = 2;        // tiles and items' costs of a warp at least
 constexpr int kMostWarps = 8;
 
 struct Args {
@@ -121,7 +121,7 @@ struct Shape {
   static constexpr int W = SB > 8192 ? 4 : SB > 4096 ? 8 : kMostWarps;  // warps
   static constexpr int S = kRingBytes / (W * SB) > 6 ? 6 : kRingBytes / (W * SB);
   static constexpr size_t kSmem = (size_t)W * S * SB;
-  static_assert(S >= 2 && kSmem <= kRingBytes, "ring");
+  static_assert(S >= 3 && kSmem <= kRingBytes, "ring");
   // a warp's two parts, 16 heads each at most, fit into its ring
   static_assert(2 * (D == 256 ? 8 : 16) * (D + 2) * 4 <= S * SB, "parts");
 };
@@ -289,7 +289,7 @@ struct Walk {
           ko = id * a.kc_b + off * a.kc_t + hk * a.kc_h;
           vo = id * a.vc_b + off * a.vc_t + hk * a.vc_h;
         }
-#pragma unroll
+#pragma unroll 1
         for (int i = 0; i < kSteps; ++i) {
           const int row = i * kRows + lr;
           const int64_t k1 = __shfl_sync(~0u, ko, row), v1 = __shfl_sync(~0u, vo, row);
@@ -474,10 +474,6 @@ __global__ void __launch_bounds__(Shape<C, D>::W * 32, 1)
         w.look_up(a, lane);
       }
     }
-#pragma unroll
-    for (int s = 0; s < S - 1; ++s) 
-      w.fetch(a, Hg, ngr, ring + s * X::SB, &stages[warp][s], &p_end[warp], lane);
-
     uint32_t q[D / 16][2 * NT];
     float o[NT][D / 16][4];
     float m[NT], l[NT], sc[NT];
@@ -487,75 +483,94 @@ __global__ void __launch_bounds__(Shape<C, D>::W * 32, 1)
     // where this lane points ldmatrix: 16-bit rows (keys by lsec, d's by lhalf), 8-bit the reverse
     const int frow = (F8 ? lhalf : lsec) * 8 + lrow, fpiece = F8 ? lsec : lhalf;
     const int fswz = swz<X::RB>(lrow);
-    int rs = 0, ws = S - 1;  // stage to read, stage to fill
-    while (true) {
-      cp_async_wait<S - 2>();
-      __syncwarp();
-      w.fetch(a, Hg, ngr, ring + ws * X::SB, &stages[warp][ws], &p_end[warp], lane);
-      ws = ws + 1 == S ? 0 : ws + 1;
-      const Stage st = stages[warp][rs];
-      const uint32_t kb = smem_u32(ring + rs * X::SB), vb = kb + KT * X::RB;
-      rs = rs + 1 == S ? 0 : rs + 1;
-      if (st.r < 0) break;
-
-      if (st.flags & 1) {  // a new item: its queries, and nothing seen
-        const int sub = st.h % ngr;
-        began = st.flags & 2;
-        head0 = st.h / ngr * gq + sub * 8 * NT;
-        heads = min(8 * NT, gq - sub * 8 * NT);
-        const T* qp = (const T*)a.q + st.r * a.q_t + head0 * a.q_h;
+    // an item's queries, as they are
+    auto load_queries = [&](const Stage& st) {
+      const int sub = st.h % ngr;
+      head0 = st.h / ngr * gq + sub * 8 * NT;
+      heads = min(8 * NT, gq - sub * 8 * NT);
+      const T* qp = (const T*)a.q + st.r * a.q_t + head0 * a.q_h;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const int row = g + 8 * n;
-          const bool on = row < heads;
-          const T* qr = qp + (on ? row : 0) * a.q_h;
-          float fac = 1.0f;
+      for (int n = 0; n < NT; ++n) {
+        const int row = g + 8 * n;
+        const T* qr = qp + row * a.q_h;
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j) q[j][2 * n] = q[j][2 * n + 1] = 0;
+        if (row < heads) {
 #pragma unroll
           for (int j = 0; j < D / 16; ++j) {
             if constexpr (F8) {  // pairs in the order of the keys' 8-bit pieces
               const uint2 v = *reinterpret_cast<const uint2*>(qr + 16 * j + 4 * t4);
-              q[j][2 * n] = on ? v.x : 0;
-              q[j][2 * n + 1] = on ? v.y : 0;
+              q[j][2 * n] = v.x;
+              q[j][2 * n + 1] = v.y;
             } else {
               const uint32_t* p = reinterpret_cast<const uint32_t*>(qr + 16 * j + 2 * t4);
-              q[j][2 * n] = on ? p[0] : 0;
-              q[j][2 * n + 1] = on ? p[4] : 0;
+              q[j][2 * n] = p[0];
+              q[j][2 * n + 1] = p[4];
             }
           }
-          if constexpr (F8 && !std::is_same<T, __half>::value) {
-            // bf16 queries against keys widened to f16: the row is brought to [1, 2) by a
-            // power of two (put back on the scores), so that f16 holds all of a bf16's 8 bits
-            uint32_t top = 0;
+        }
+      }
+    };
+    // nothing seen of the item yet; its queries as the product takes them
+    auto start_item = [&](const Stage& st) {
+      began = st.flags & 2;
 #pragma unroll
-            for (int j = 0; j < D / 16; ++j)
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const uint32_t v = q[j][2 * n + e] & 0x7fff7fffu;
-                top = max(top, max(v & 0xffffu, v >> 16));
-              }
-            top = max(top, __shfl_xor_sync(~0u, top, 1));
-            top = max(top, __shfl_xor_sync(~0u, top, 2));
-            const uint32_t ex = min(max(top << 16 & 0x7f800000u, 0x00800000u), 0x7e800000u);
-            fac = __uint_as_float(ex);
-            const float inv = __uint_as_float(0x7f000000u - ex);
-#pragma unroll
-            for (int j = 0; j < D / 16; ++j)
-#pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const uint32_t v = q[j][2 * n + e];
-                q[j][2 * n + e] = pack2<__half>(__uint_as_float(v << 16) * inv,
-                                                __uint_as_float(v & 0xffff0000u) * inv);
-              }
-          }
-          sc[n] = a.scale2 * fac;
-          m[n] = -INFINITY;
-          l[n] = 0.0f;
+      for (int n = 0; n < NT; ++n) {
+        float fac = 1.0f;
+        if constexpr (F8 && !std::is_same<T, __half>::value) {
+          // bf16 queries against keys widened to f16: the row is brought to [1, 2) by a
+          // power of two (put back on the scores), so that f16 holds all of a bf16's 8 bits
+          uint32_t top = 0;
 #pragma unroll
           for (int j = 0; j < D / 16; ++j)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[n][j][e] = 0.0f;
+            for (int e = 0; e < 2; ++e) {
+              const uint32_t v = q[j][2 * n + e] & 0x7fff7fffu;
+              top = max(top, max(v & 0xffffu, v >> 16));
+            }
+          top = max(top, __shfl_xor_sync(~0u, top, 1));
+          top = max(top, __shfl_xor_sync(~0u, top, 2));
+          const uint32_t ex = min(max(top << 16 & 0x7f800000u, 0x00800000u), 0x7e800000u);
+          fac = __uint_as_float(ex);
+          const float inv = __uint_as_float(0x7f000000u - ex);
+#pragma unroll
+          for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const uint32_t v = q[j][2 * n + e];
+              q[j][2 * n + e] = pack2<__half>(__uint_as_float(v << 16) * inv,
+                                              __uint_as_float(v & 0xffff0000u) * inv);
+            }
         }
+        sc[n] = a.scale2 * fac;
+        m[n] = -INFINITY;
+        l[n] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[n][j][e] = 0.0f;
       }
+    };
+    int rs = 0, ws = 0;        // stage to read, stage to fill
+    Stage st{0, -1, 0, 0};     // the tile at hand
+    for (int ahead = S - 1;; ahead -= ahead > 0) {  // tiles to start before the first is awaited
+      if (ahead == 0) {
+        cp_async_wait<S - 2>();
+        __syncwarp();
+      }
+      w.fetch(a, Hg, ngr, ring + ws * X::SB, &stages[warp][ws], &p_end[warp], lane);
+      ws = ws + 1 == S ? 0 : ws + 1;
+      if (ahead > 1) continue;
+      if (ahead == 1) {  // the first tile is under way: its queries
+        __syncwarp();
+        st = stages[warp][rs];
+        if (st.r < 0) break;
+        load_queries(st);
+        continue;
+      }
+      const uint32_t kb = smem_u32(ring + rs * X::SB), vb = kb + KT * X::RB;
+      rs = rs + 1 == S ? 0 : rs + 1;
+      if (st.flags & 1) start_item(st);
 
       // scores: rows = heads, columns = keys
       float s[KT / 8][4];
@@ -720,6 +735,9 @@ __global__ void __launch_bounds__(Shape<C, D>::W * 32, 1)
         }
       }
       if (last) break;
+      st = stages[warp][rs];  // written two fetches ago
+      if (st.r < 0) break;
+      if (st.flags & 1) load_queries(st);
     }
     if (p_item[2 * warp] >= 0) {  // the first part joins the last in the ring
       cp_async_wait<0>();
@@ -741,25 +759,42 @@ __global__ void __launch_bounds__(Shape<C, D>::W * 32, 1)
     return reinterpret_cast<const float*>(ring_all + (size_t)(e >> 1) * S * X::SB) +
            (e & 1 ? 0 : PF);
   };
-  const int my_item = lane < 2 * W ? p_item[lane] : -1;
-  const uint32_t same = __match_any_sync(~0u, my_item);
-  uint32_t leads = __ballot_sync(~0u, my_item >= 0 && (same & ((1u << lane) - 1)) == 0);
+  static_assert(2 * W <= 16, "a lane per entry");
+  int my_item = lane < 2 * W ? p_item[lane] : -1;
+  const bool real = my_item >= 0;
+  const uint32_t reals = __ballot_sync(~0u, real), upto = reals & ((2u << lane) - 1);
+  const int known = __shfl_sync(~0u, my_item, upto ? 31 - __clz(upto) : 0);
+  if (!real && lane < 2 * W) my_item = upto ? known : -1;  // an empty entry goes with its run
+  const uint32_t same = __match_any_sync(~0u, my_item) & reals;
+  uint32_t leads = __ballot_sync(~0u, real && (same & ((1u << lane) - 1)) == 0);
   if (leads) {  // (the same in all warps)
-    const int we = threadIdx.x / (8 * NT), wh = threadIdx.x % (8 * NT);
-    const uint32_t peers = __shfl_sync(~0u, same, we & 31);
-    static_assert(2 * W * 8 * NT <= W * 32 && 32 % (8 * NT) == 0, "a thread per entry and head");
-    if (we < 2 * W && p_item[we] >= 0) {
-      float top = -INFINITY;
-      for (uint32_t b = peers; b; b &= b - 1) top = fmaxf(top, part(__ffs(b) - 1)[NT * 8 * D + wh]);
-      p_w[we][wh] = weight(part(we)[NT * 8 * D + wh], top);
-      if ((peers & ((1u << we) - 1)) == 0) {
-        float sum = 0;
-        for (uint32_t b = peers; b; b &= b - 1) {
-          const float* p = part(__ffs(b) - 1) + NT * 8 * D + wh;
-          sum += weight(p[0], top) * p[8 * NT];
+#pragma unroll 1
+    for (int h = warp; h < 8 * NT; h += W) {
+      const float* p = part(lane & (2 * W - 1)) + NT * 8 * D + h;
+      const float pm = real ? p[0] : -INFINITY;
+      float top = pm, sum;
+#pragma unroll
+      for (int o = 1; o < 2 * W; o <<= 1) {  // up the run, then from its end
+        const float y = __shfl_up_sync(~0u, top, o);
+        const int it = __shfl_up_sync(~0u, my_item, o);
+        if (lane >= o && it == my_item) top = fmaxf(top, y);
+      }
+      const int tail = same ? 31 - __clz(same) : lane;
+      top = __shfl_sync(~0u, top, tail);
+      const float wgt = real ? weight(pm, top) : 0.0f;
+      sum = real ? wgt * p[8 * NT] : 0.0f;
+#pragma unroll
+      for (int o = 1; o < 2 * W; o <<= 1) {
+        const float y = __shfl_up_sync(~0u, sum, o);
+        const int it = __shfl_up_sync(~0u, my_item, o);
+        if (lane >= o && it == my_item) sum += y;
+      }
+      if (real) {
+        p_w[lane][h] = wgt;
+        if (lane == tail) {
+          p_m[__ffs(same) - 1][h] = top;
+          p_l[__ffs(same) - 1][h] = sum;
         }
-        p_m[we][wh] = top;
-        p_l[we][wh] = sum;
       }
     }
   }
