@@ -384,10 +384,13 @@ def kv_block_table(lens: torch.Tensor, new_tokens: torch.Tensor, block_table: to
     if N < 0:
         raise ValueError("max_tokens must not be negative")
     guard, index = _on(lens, new_tokens, block_table, free_blocks, free_count)
-    if out is None:  # one allocation, cut up
-        sizes = (R, 1, R + 1, N, N, N, R)
-        out = KvStep(*torch.empty(sum(sizes), dtype=torch.int32,
-                                  device=lens.device).split_with_sizes(sizes))
+    if out is None:  # one allocation, cut up; the tokens' rows first, each 16-byte aligned
+        pad = -N % 4
+        sizes = (N, pad, N, pad, N, pad, R, 1, R + 1, R) if pad else (N, N, N, R, 1, R + 1, R)
+        cut = torch.empty(3 * (N + pad) + 3 * R + 2, dtype=torch.int32,
+                          device=lens.device).split_with_sizes(sizes)
+        s, p, t = cut[0:6:2] if pad else cut[:3]
+        out = KvStep(*cut[-4:-1], s, p, t, cut[-1])
     else:
         for name, n in zip(KvStep._fields, (R, 1, R + 1, N, N, N, R)):
             _ints(name, getattr(out, name), (n,))

@@ -16,6 +16,8 @@
 // 8192 lengths), the CTAs meet at a cluster barrier before anything is written,
 // and tokens are then spread over all threads, each finding its request by
 // binary search in the shared-memory prefix sums.
+#include <algorithm>
+
 #include "runtime.cuh"
 
 namespace rb {
@@ -30,6 +32,8 @@ struct TableArgs {
   int32_t *free_blocks, *lens_out, *free_out, *cu, *slots, *positions, *requests, *status;
   const int32_t* free_count;
   int32_t R, max_blocks, num_blocks, bs, max_tokens;
+  Divisor by_bs;
+  int32_t vectors;  // slots, positions and requests are 16-byte aligned
 };
 
 __device__ __forceinline__ void cluster_barrier() {
@@ -59,20 +63,35 @@ struct Ask {
   bool bad;
 };
 
+// Blocks of n tokens, n in [0, 2^31).
+__device__ __forceinline__ int32_t blocks_of(const TableArgs& a, int32_t n) {
+  return n > 0 ? a.by_bs.div(n - 1) + 1 : 0;
+}
+
 __device__ __forceinline__ Ask ask_of(const TableArgs& a, int32_t len, int32_t n) {
   Ask q{0, 0, 0, false};
-  const int64_t room = (int64_t)a.max_blocks * a.bs;
+  const int64_t room = (int64_t)a.max_blocks * a.bs;  // below 2^31
   const bool held = len >= 0 && len <= room;
-  const int32_t own = held ? (int32_t)(((int64_t)len + a.bs - 1) / a.bs) : 0;
+  const int32_t own = held ? blocks_of(a, len) : 0;
   if (n >= 0) {
     q.tokens = n;
     q.bad = !held || (int64_t)len + n > room;
-    if (!q.bad) q.need = ((int64_t)len + n + a.bs - 1) / a.bs - own;
+    if (!q.bad) q.need = blocks_of(a, len + n) - own;
   } else {
     q.bad = n != REMORA_B200_KV_RELEASE || !held;
     if (!q.bad) q.back = own;
   }
   return q;
+}
+
+// Inclusive sum over the lanes of a warp.
+__device__ __forceinline__ int64_t warp_scan(int64_t x, int lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t y = __shfl_up_sync(~0u, x, o);
+    if (lane >= o) x += y;
+  }
+  return x;
 }
 
 // Largest i with prefix[i] <= v, over prefix[0..n] (prefix[0] = 0, v >= 0).
@@ -97,58 +116,47 @@ __global__ void __launch_bounds__(1024) k_block_table(const TableArgs a) {
   const int tid = threadIdx.x, nt = blockDim.x, lane = tid & 31, warp = tid >> 5;
   const int nw = nt >> 5;
   if (tid == 0) taken = 0;
+  const int32_t count_in = *a.free_count;
 
-  // prefix sums: each thread sums a run of requests, then warps, then the block
+  // prefix sums: each thread sums a run of requests, then warps, then the block.  A request
+  // whose tokens pass max_tokens is refused and its blocks are not counted, so the tokens are
+  // summed first.
   const int c = (a.R + nt - 1) / nt;
   const int r0 = min(tid * c, a.R), r1 = min(r0 + c, a.R);
+  const int32_t len_r0 = r0 < r1 ? a.lens[r0] : 0, n_r0 = r0 < r1 ? a.fresh[r0] : 0;
+  const Ask ask_r0 = ask_of(a, len_r0, n_r0);
+  auto ask = [&](int r) { return r == r0 ? ask_r0 : ask_of(a, a.lens[r], a.fresh[r]); };
   int64_t s0 = 0, s1 = 0, s2 = 0;
-  int64_t before = 0;  // tokens: a request whose tokens pass max_tokens is refused, so its
-                       // blocks are not counted; that needs the token sum first
-  for (int r = r0; r < r1; ++r) {
-    const Ask q = ask_of(a, a.lens[r], a.fresh[r]);
-    s0 += q.tokens;
-  }
-  int64_t x = s0;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int64_t y = __shfl_up_sync(~0u, x, o);
-    if (lane >= o) x += y;
-  }
-  if (lane == 31) part[0][warp] = x;
+  for (int r = r0; r < r1; ++r) s0 += ask(r).tokens;
+  const int64_t x0 = warp_scan(s0, lane);
+  if (lane == 31) part[0][warp] = x0;
   __syncthreads();
-  int64_t base = 0;
-  for (int w = 0; w < warp; ++w) base += part[0][w];
-  before = base + x - s0;
+  const int64_t w0 = lane < nw ? part[0][lane] : 0, i0 = warp_scan(w0, lane);
+  const int64_t before = __shfl_sync(~0u, i0 - w0, warp) + x0 - s0;
   {
     int64_t t = before;
     for (int r = r0; r < r1; ++r) {
-      const Ask q = ask_of(a, a.lens[r], a.fresh[r]);
+      const Ask q = ask(r);
       t += q.tokens;
       if (t <= a.max_tokens) s1 += q.need;
       s2 += q.back;
     }
   }
-  int64_t x1 = s1, x2 = s2;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int64_t y1 = __shfl_up_sync(~0u, x1, o), y2 = __shfl_up_sync(~0u, x2, o);
-    if (lane >= o) { x1 += y1; x2 += y2; }
-  }
+  const int64_t x1 = warp_scan(s1, lane), x2 = warp_scan(s2, lane);
   if (lane == 31) { part[1][warp] = x1; part[2][warp] = x2; }
   __syncthreads();
-  int64_t b1 = 0, b2 = 0, all2 = 0;
-  for (int w = 0; w < nw; ++w) {
-    if (w < warp) { b1 += part[1][w]; b2 += part[2][w]; }
-    all2 += part[2][w];
-  }
-  const int32_t count_in = *a.free_count;
+  const int64_t w1 = lane < nw ? part[1][lane] : 0, w2 = lane < nw ? part[2][lane] : 0;
+  const int64_t i1 = warp_scan(w1, lane), i2 = warp_scan(w2, lane);
+  const int64_t b1 = __shfl_sync(~0u, i1 - w1, warp), b2 = __shfl_sync(~0u, i2 - w2, warp);
+  const int64_t all2 = __shfl_sync(~0u, i2, 31);
   const int32_t count0 = min(max(count_in, 0), a.num_blocks);
   const int32_t have = (int32_t)min((int64_t)count0 + all2, (int64_t)a.num_blocks);
   {
     int64_t t = before, p1 = b1 + x1 - s1, p2 = b2 + x2 - s2;
+    int32_t top = 0;
     for (int r = r0; r < r1; ++r) {
-      const int32_t len = a.lens[r];
-      const Ask q = ask_of(a, len, a.fresh[r]);
+      const int32_t len = r == r0 ? len_r0 : a.lens[r];
+      const Ask q = ask(r);
       cu[r] = sat32(t);
       need[r] = sat32(p1);
       back[r] = sat32(p2);
@@ -157,7 +165,7 @@ __global__ void __launch_bounds__(1024) k_block_table(const TableArgs a) {
       if (t <= a.max_tokens) p1 += q.need;
       p2 += q.back;
       const bool dry = !bad && q.need > 0 && p1 > have;
-      if (!bad && !dry && q.need > 0) atomicMax(&taken, (int32_t)p1);
+      if (!bad && !dry && q.need > 0) top = (int32_t)p1;
       len0[r] = (len & 0x7fffffff) | (bad || dry ? 0x80000000 : 0);
     }
     if (r1 == a.R) {  // several threads when R is short of the block: the same values
@@ -165,6 +173,7 @@ __global__ void __launch_bounds__(1024) k_block_table(const TableArgs a) {
       need[a.R] = sat32(p1);
       back[a.R] = sat32(p2);
     }
+    if (top > 0) atomicMax(&taken, top);
   }
   const uint32_t rank = cluster_rank(), ctas = cluster_size();
   const int me = rank * nt + tid, step = ctas * nt;
@@ -184,32 +193,57 @@ __global__ void __launch_bounds__(1024) k_block_table(const TableArgs a) {
     cluster_barrier();
   }
 
-  // each token's slot; the token that opens a block enters it into the table
+  // each token's slot, four neighbours to a thread (mostly of one request and one block); the
+  // token that opens a block enters it into the table
   const int32_t total = cu[a.R];
-  for (int64_t i = me; i < a.max_tokens; i += step) {
-    const int32_t t = (int32_t)i;
-    int32_t slot = -1, pos = 0, req = -1;
-    if (t < total) {
-      req = find_le(cu, a.R, t);
-      const int32_t l = len0[req];
-      if (l >= 0) {
-        pos = l + (t - cu[req]);
-        const int32_t page = pos / a.bs, off = pos - page * a.bs;
-        const int32_t own = (int32_t)(((int64_t)l + a.bs - 1) / a.bs);
-        int32_t id;
+  const int64_t quads = ((int64_t)a.max_tokens + 3) / 4;
+  for (int64_t i = me; i < quads; i += step) {
+    const int32_t t4 = (int32_t)(4 * i);
+    int32_t slot[4], pos[4], req[4];
+    int32_t r = t4 < total ? find_le(cu, a.R, t4) : a.R, seen_r = -1, seen_page = -1, id = -1;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int64_t t = (int64_t)t4 + e;
+      slot[e] = -1;
+      pos[e] = 0;
+      req[e] = -1;
+      if (t >= min(total, a.max_tokens)) continue;
+      while (t >= cu[r + 1]) ++r;
+      req[e] = r;
+      const int32_t l = len0[r];
+      if (l < 0) continue;
+      pos[e] = l + (int32_t)(t - cu[r]);
+      const int32_t page = a.by_bs.div(pos[e]), off = pos[e] - page * a.bs;
+      if (r != seen_r || page != seen_page) {
+        const int32_t own = blocks_of(a, l);
         if (page < own) {
-          id = a.table[(int64_t)req * a.ld_table + page];
+          id = a.table[(int64_t)r * a.ld_table + page];
         } else {
-          id = __ldcg(a.free_blocks + (have - 1 - (need[req] + page - own)));
-          if (off == 0) a.table[(int64_t)req * a.ld_table + page] = id;
+          id = __ldcg(a.free_blocks + (have - 1 - (need[r] + page - own)));
+          if (off == 0) a.table[(int64_t)r * a.ld_table + page] = id;
         }
-        if (id >= 0 && id < a.num_blocks) slot = id * a.bs + off;
-        else atomicExch(&g_device_error, 3);
+        if (id < 0 || id >= a.num_blocks) {
+          atomicExch(&g_device_error, 3);
+          id = -1;
+        }
+        seen_r = r;
+        seen_page = page;
       }
+      if (id >= 0) slot[e] = id * a.bs + off;
     }
-    a.slots[t] = slot;
-    a.positions[t] = pos;
-    a.requests[t] = req;
+    if (a.vectors && t4 + 3 < a.max_tokens) {
+      *reinterpret_cast<int4*>(a.slots + t4) = make_int4(slot[0], slot[1], slot[2], slot[3]);
+      *reinterpret_cast<int4*>(a.positions + t4) = make_int4(pos[0], pos[1], pos[2], pos[3]);
+      *reinterpret_cast<int4*>(a.requests + t4) = make_int4(req[0], req[1], req[2], req[3]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if ((int64_t)t4 + e < a.max_tokens) {
+          a.slots[t4 + e] = slot[e];
+          a.positions[t4 + e] = pos[e];
+          a.requests[t4 + e] = req[e];
+        }
+    }
   }
 
   for (int r = me; r < a.R; r += step) {
@@ -258,12 +292,16 @@ extern "C" int remora_b200_kv_block_table(const remora_b200_kv_block_table_args*
   TableArgs a{x.lens, x.new_tokens, x.block_table, x.ld_table, x.free_blocks, x.lens_out,
               x.free_count_out, x.cu_tokens, x.slots, x.positions, x.requests, x.status,
               x.free_count, (int32_t)x.R, (int32_t)x.max_blocks, (int32_t)x.num_blocks,
-              (int32_t)x.block_size, (int32_t)x.max_tokens};
+              (int32_t)x.block_size, (int32_t)x.max_tokens, Divisor((uint32_t)x.block_size),
+              aligned16(x.slots) && aligned16(x.positions) && aligned16(x.requests)};
   const size_t smem = (4 * (size_t)x.R + 3) * sizeof(int32_t);
   if (smem > 48 * 1024)
     RB_CUDA(cudaFuncSetAttribute(k_block_table, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                  (4 * kMaxRequests + 3) * (int)sizeof(int32_t)));
-  const int threads = 1024, ctas = x.max_tokens > 4096 ? 8 : 1;
+  // a thread for each request or four tokens, in one CTA while 1024 are enough
+  const int64_t wide = std::max<int64_t>(x.R, (x.max_tokens + 3) / 4);
+  const int ctas = wide > 1024 ? 8 : 1;
+  const int threads = (int)std::min<int64_t>(1024, std::max<int64_t>(128, (wide + 31) / 32 * 32));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas);
   cfg.blockDim = dim3(threads);
