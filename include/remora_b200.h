@@ -95,7 +95,9 @@ typedef struct remora_b200_report {
 
 /* 1 if `test` (the --test= kind) is handled by this library, else 0.
  * Kinds: "elementwise" (gpu_tests.cpp:35-95), "projection"
- * (cpu_tests.cpp:65-97), "elementwise_chain", "gemm", "attention", "moe"
+ * (cpu_tests.cpp:65-97), "elementwise_chain", "gemm", "attention", "decode"
+ * (a serving step over a paged cache: tables, append and attention; config
+ * "RxHqxHkvxS", requests, heads, kv heads and keys), "moe"
  * (configs "4", "5", "mixtral" = mixtral_moe_layer.mlir:8, "simple" =
  * simple_moe.mlir:16, "hetero" = heterogeneous_moe_layer.mlir:66, with
  * bf16 operands). */

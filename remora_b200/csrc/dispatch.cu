@@ -312,6 +312,216 @@ static int run_attention(const remora_b200_opts* o, remora_b200_report* r, cudaS
   return REMORA_B200_OK;
 }
 
+// "RxHqxHkvxS": requests, heads, kv heads, keys; default 64x32x8x4096.
+static bool decode_config(const char* c, int64_t* R, int64_t* Hq, int64_t* Hkv, int64_t* S) {
+  long long r = 64, q = 32, k = 8, n = 4096;
+  if (c && *c && sscanf(c, "%lldx%lldx%lldx%lld", &r, &q, &k, &n) != 4) return false;
+  *R = r;
+  *Hq = q;
+  *Hkv = k;
+  *S = n;
+  return r >= 1 && r <= paged::kMaxRequests && k >= 1 && q >= k && q % k == 0 && q <= 1024 &&
+         n >= 1 && n <= (1 << 20) && r * n <= (1 << 26);
+}
+
+// --test=decode (no counterpart in the reference): a step of a serving loop over a paged bf16
+// cache, head_dim 128, blocks of 16 tokens.  The requests' prompts (lengths S - 37 r mod S/2)
+// are put into the cache by kv_block_table and rope_kv_append; then one token each is timed:
+// tables, append, attention.  Validation: 32 (request, head) rows of the output against a
+// double-precision softmax over the rotated keys on the host, normwise per row.
+static int run_decode(const remora_b200_opts* o, remora_b200_report* r, cudaStream_t st) {
+  int64_t R, Hq, Hkv, S;
+  if (!decode_config(o ? o->config : nullptr, &R, &Hq, &Hkv, &S))
+    return fail(REMORA_B200_ERR_INVALID, "decode: unknown config '%s'", o->config);
+  const int64_t D = 128, bs = 16, mb = (S + 1 + bs - 1) / bs, row = Hkv * D;
+  const uint64_t seed = o && o->seed ? o->seed : 42;
+  std::vector<int32_t> len(R), ones(R, 1), zero(R, 0);
+  int64_t N = 0, nb = 8;
+  for (int64_t i = 0; i < R; ++i) {
+    len[i] = (int32_t)(S - (37 * i) % (S / 2 + 1));
+    N += len[i];
+    nb += (len[i] + 1 + bs - 1) / bs;
+  }
+  std::vector<int32_t> ids(nb);
+  for (int64_t i = 0; i < nb; ++i) ids[i] = (int32_t)i;
+  for (int64_t i = nb - 1; i > 0; --i)  // the free blocks in no order
+    std::swap(ids[i], ids[host_mix64(stream_key(seed, 97) + (uint64_t)i) % (uint64_t)(i + 1)]);
+  std::vector<double> freq(D / 2);
+  for (int64_t i = 0; i < D / 2; ++i) freq[i] = std::pow(10000.0, -2.0 * (double)i / (double)D);
+
+  DevBuf lens, fresh, table, free_blocks, count, cu, slots, positions, requests, status, q, k, v, q1,
+      k1, v1, out, kc, vc, ws;
+  const size_t wsb = remora_b200_paged_attention_workspace_bytes(R, Hq, Hkv, D);
+  int rc;
+  if ((rc = lens.alloc(3 * R * 4)) || (rc = fresh.alloc(R * 4)) || (rc = table.alloc(R * mb * 4)) ||
+      (rc = free_blocks.alloc(nb * 4)) || (rc = count.alloc(3 * 4)) || (rc = cu.alloc((R + 1) * 4)) ||
+      (rc = slots.alloc(N * 4)) || (rc = positions.alloc(N * 4)) || (rc = requests.alloc(N * 4)) ||
+      (rc = status.alloc(R * 4)) || (rc = q.alloc(R * Hq * D * 2)) || (rc = k.alloc(N * row * 2)) ||
+      (rc = v.alloc(N * row * 2)) || (rc = q1.alloc(R * Hq * D * 2)) ||
+      (rc = k1.alloc(R * row * 2)) || (rc = v1.alloc(R * row * 2)) ||
+      (rc = out.alloc(R * Hq * D * 2)) || (rc = kc.alloc(nb * bs * row * 2)) ||
+      (rc = vc.alloc(nb * bs * row * 2)) || (rc = ws.alloc(wsb)))
+    return rc;
+  if ((rc = remora_b200_fill_normal(q.p, R * Hq * D, 1, stream_key(seed, 50), 0, 1, st)) ||
+      (rc = remora_b200_fill_normal(k.p, N * row, 1, stream_key(seed, 51), 0, 1, st)) ||
+      (rc = remora_b200_fill_normal(v.p, N * row, 1, stream_key(seed, 52), 0, 1, st)) ||
+      (rc = remora_b200_fill_normal(k1.p, R * row, 1, stream_key(seed, 53), 0, 1, st)) ||
+      (rc = remora_b200_fill_normal(v1.p, R * row, 1, stream_key(seed, 54), 0, 1, st)))
+    return rc;
+  const int32_t n_free = (int32_t)nb;
+  int32_t* l = (int32_t*)lens.p;  // [3][R]: empty, prompts, prompts and a token
+  int32_t* c = (int32_t*)count.p;
+  RB_CUDA(cudaMemcpyAsync(l, zero.data(), R * 4, cudaMemcpyHostToDevice, st));
+  RB_CUDA(cudaMemcpyAsync(fresh.p, len.data(), R * 4, cudaMemcpyHostToDevice, st));
+  RB_CUDA(cudaMemcpyAsync(free_blocks.p, ids.data(), nb * 4, cudaMemcpyHostToDevice, st));
+  RB_CUDA(cudaMemcpyAsync(c, &n_free, 4, cudaMemcpyHostToDevice, st));
+  RB_CUDA(cudaStreamSynchronize(st));
+
+  remora_b200_kv_block_table_args t = {};
+  t.lens = l;
+  t.new_tokens = (const int32_t*)fresh.p;
+  t.block_table = (int32_t*)table.p;
+  t.free_blocks = (int32_t*)free_blocks.p;
+  t.free_count = c;
+  t.lens_out = l + R;
+  t.free_count_out = c + 1;
+  t.cu_tokens = (int32_t*)cu.p;
+  t.slots = (int32_t*)slots.p;
+  t.positions = (int32_t*)positions.p;
+  t.requests = (int32_t*)requests.p;
+  t.status = (int32_t*)status.p;
+  t.R = R;
+  t.ld_table = t.max_blocks = mb;
+  t.num_blocks = nb;
+  t.block_size = bs;
+  t.max_tokens = N;
+  remora_b200_rope_kv_append_args e = {};
+  e.k = k.p;
+  e.v = v.p;
+  e.k_cache = kc.p;
+  e.v_cache = vc.p;
+  e.positions = (const int32_t*)positions.p;
+  e.slots = (const int32_t*)slots.p;
+  e.freq = freq.data();
+  e.T = N;
+  e.Hkv = Hkv;
+  e.D = e.rot = D;
+  e.q_t = e.q_out_t = Hq * D;
+  e.k_t = e.v_t = row;
+  e.q_h = e.k_h = e.v_h = e.q_out_h = D;
+  e.ld_pos = N;
+  e.num_blocks = nb;
+  e.block_size = bs;
+  e.kc_block = e.vc_block = bs * row;
+  e.kc_token = e.vc_token = row;
+  e.kc_head = e.vc_head = D;
+  e.k_scale = e.v_scale = 1.0f;
+  e.dtype = e.cache_dtype = REMORA_B200_BF16;
+  e.n_axes = 1;
+  if ((rc = remora_b200_kv_block_table(&t, st)) || (rc = remora_b200_rope_kv_append(&e, st)))
+    return rc;  // the prompts' keys and values
+
+  RB_CUDA(cudaMemcpyAsync(fresh.p, ones.data(), R * 4, cudaMemcpyHostToDevice, st));
+  t.lens = l + R;
+  t.lens_out = l + 2 * R;
+  t.free_count = c + 1;
+  t.free_count_out = c + 2;
+  t.max_tokens = R;
+  e.q = q.p;
+  e.q_out = q1.p;
+  e.k = k1.p;
+  e.v = v1.p;
+  e.T = R;
+  e.Hq = Hq;
+  e.ld_pos = R;
+  remora_b200_paged_attention_args a = {};
+  a.q = q1.p;
+  a.k_cache = kc.p;
+  a.v_cache = vc.p;
+  a.block_table = (const int32_t*)table.p;
+  a.lens = l + 2 * R;
+  a.out = out.p;
+  a.workspace = ws.p;
+  a.workspace_bytes = wsb;
+  a.R = R;
+  a.Hq = Hq;
+  a.Hkv = Hkv;
+  a.D = D;
+  a.q_t = a.out_t = Hq * D;
+  a.q_h = a.out_h = D;
+  a.num_blocks = nb;
+  a.block_size = bs;
+  a.kc_block = a.vc_block = bs * row;
+  a.kc_token = a.vc_token = row;
+  a.kc_head = a.vc_head = D;
+  a.ld_table = a.max_blocks = mb;
+  a.scale = 1.0f / sqrtf((float)D);
+  a.k_scale = a.v_scale = 1.0f;
+  a.dtype = a.cache_dtype = REMORA_B200_BF16;
+  double ms = 0;
+  rc = time_iters(o, st, [&] {
+    int s;
+    if ((s = remora_b200_kv_block_table(&t, st)) || (s = remora_b200_rope_kv_append(&e, st)))
+      return s;
+    return remora_b200_paged_attention(&a, st);
+  }, &ms);
+  if (rc) return rc;
+
+  ErrStat err;
+  if (o && o->validate) {
+    std::vector<uint16_t> hq(R * Hq * D), ho(R * Hq * D), kr, vr, k1h(R * row), v1h(R * row);
+    RB_CUDA(cudaMemcpy(hq.data(), q.p, hq.size() * 2, cudaMemcpyDeviceToHost));
+    RB_CUDA(cudaMemcpy(ho.data(), out.p, ho.size() * 2, cudaMemcpyDeviceToHost));
+    RB_CUDA(cudaMemcpy(k1h.data(), k1.p, k1h.size() * 2, cudaMemcpyDeviceToHost));
+    RB_CUDA(cudaMemcpy(v1h.data(), v1.p, v1h.size() * 2, cudaMemcpyDeviceToHost));
+    // one head turned at position p, rounded to bf16 as the kernels store it
+    auto turn = [&](const uint16_t* x, int64_t p, std::vector<double>& y) {
+      for (int64_t i = 0; i < D / 2; ++i) {
+        const double s = std::sin(p * freq[i]), w = std::cos(p * freq[i]);
+        const double x0 = bf16_to_f32(x[i]), x1 = bf16_to_f32(x[i + D / 2]);
+        y[i] = __bfloat162float(__float2bfloat16_rn((float)(x0 * w - x1 * s)));
+        y[i + D / 2] = __bfloat162float(__float2bfloat16_rn((float)(x0 * s + x1 * w)));
+      }
+    };
+    std::vector<double> qd(D), kd(D), pr, acc(D);
+    const uint64_t key = stream_key(seed, 96);
+    for (int s2 = 0; s2 < 32; ++s2) {
+      const uint64_t hsh = host_mix64(key + (uint64_t)s2 * 0x9E3779B97F4A7C15ull);
+      const int64_t i = (int64_t)(hsh % (uint64_t)R), h = (int64_t)((hsh >> 32) % (uint64_t)Hq);
+      const int64_t hk = h / (Hq / Hkv), n = len[i];
+      int64_t first = 0;
+      for (int64_t x = 0; x < i; ++x) first += len[x];
+      kr.resize(n * D);
+      vr.resize(n * D);
+      RB_CUDA(cudaMemcpy2D(kr.data(), D * 2, (const uint16_t*)k.p + first * row + hk * D, row * 2,
+                           D * 2, n, cudaMemcpyDeviceToHost));
+      RB_CUDA(cudaMemcpy2D(vr.data(), D * 2, (const uint16_t*)v.p + first * row + hk * D, row * 2,
+                           D * 2, n, cudaMemcpyDeviceToHost));
+      turn(&hq[(i * Hq + h) * D], n, qd);
+      pr.assign(n + 1, 0);
+      double m = -1e300, sum = 0;
+      for (int64_t j = 0; j <= n; ++j) {
+        turn(j < n ? &kr[j * D] : &k1h[i * row + hk * D], j, kd);
+        for (int64_t x = 0; x < D; ++x) pr[j] += qd[x] * kd[x];
+        pr[j] *= a.scale;
+        m = std::max(m, pr[j]);
+      }
+      for (double& x : pr) sum += (x = std::exp(x - m));
+      std::fill(acc.begin(), acc.end(), 0.0);
+      for (int64_t j = 0; j <= n; ++j) {
+        const uint16_t* y = j < n ? &vr[j * D] : &v1h[i * row + hk * D];
+        for (int64_t x = 0; x < D; ++x) acc[x] += pr[j] / sum * bf16_to_f32(y[x]);
+      }
+      double mx = 1e-6;
+      for (double x : acc) mx = std::max(mx, std::fabs(x));
+      for (int64_t x = 0; x < D; ++x) err.add(bf16_to_f32(ho[(i * Hq + h) * D + x]), acc[x], mx);
+    }
+  }
+  finish(r, ms, 2.0 * (double)(N + R) * row * 2, err, 2e-2, o ? o->validate : 0,
+         "decode step (tables, append, attention)", "TB/s");
+  return REMORA_B200_OK;
+}
+
 // --test=moe: the MoE layer of mlir/stablehlo/mixtral_moe_layer.mlir:8-68
 // with bf16 operands.  config "4" (default: T=8192 D=4096 F=14336 E=8 top-2),
 // "5" (T=65536 D=2048 F=1536 E=64 top-8), "mixtral" (the program's own
@@ -483,7 +693,7 @@ extern "C" int remora_b200_recognise(const char* test) {
   if (!test) return 0;
   std::string t = test;
   return t == "elementwise" || t == "projection" || t == "elementwise_chain" || t == "gemm" ||
-         t == "attention" || t == "moe";
+         t == "attention" || t == "decode" || t == "moe";
 }
 
 extern "C" int remora_b200_run_test(const char* test, const remora_b200_opts* o,
@@ -507,6 +717,8 @@ extern "C" int remora_b200_run_test(const char* test, const remora_b200_opts* o,
     rc = run_gemm(o, r, st);
   else if (t == "attention")
     rc = run_attention(o, r, st);
+  else if (t == "decode")
+    rc = run_decode(o, r, st);
   else if (t == "moe")
     rc = run_moe(o, r, st);
   else

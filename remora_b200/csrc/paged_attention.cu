@@ -112,14 +112,28 @@ __device__ __forceinline__ float2 unpack2(uint32_t x) {
 }
 
 // ------------------------------------------------------------------ shapes
+// By the bytes of a row (head_dim elements of the cache): the keys of a tile, a tile's keys and
+// values in bytes, the warps of a CTA and the tiles of a warp's ring.  8 KB tiles and 24 KB rings
+// for 8 warps, so that 16 KB are in flight per warp while it computes.  12 or 16 warps of half
+// the keys measured slower: 128 ragged requests of 64-element f16 rows 60 and 67 us against 56
+// (more instructions per key, the same bytes in flight).
+constexpr int tile_keys(int rb) { return rb <= 128 ? 32 : 16; }
+constexpr int tile_bytes(int rb) { return 2 * tile_keys(rb) * rb; }
+constexpr int split_warps(int rb) { return tile_bytes(rb) > 8192 ? 4 : kMostWarps; }
+constexpr int ring_tiles(int rb) {
+  return kRingBytes / (split_warps(rb) * tile_bytes(rb)) > 6
+             ? 6
+             : kRingBytes / (split_warps(rb) * tile_bytes(rb));
+}
+
 template <typename C, int D>
 struct Shape {
-  static constexpr int RB = D * (int)sizeof(C);     // bytes of a row
-  static constexpr int CH = RB / 16;                // 16-byte pieces of a row
-  static constexpr int KT = RB <= 128 ? 32 : 16;    // keys of a tile
-  static constexpr int SB = 2 * KT * RB;            // a tile's keys and values
-  static constexpr int W = SB > 8192 ? 4 : SB > 4096 ? 8 : kMostWarps;  // warps
-  static constexpr int S = kRingBytes / (W * SB) > 6 ? 6 : kRingBytes / (W * SB);
+  static constexpr int RB = D * (int)sizeof(C);  // bytes of a row
+  static constexpr int CH = RB / 16;             // 16-byte pieces of a row
+  static constexpr int KT = tile_keys(RB);
+  static constexpr int SB = tile_bytes(RB);
+  static constexpr int W = split_warps(RB);
+  static constexpr int S = ring_tiles(RB);
   static constexpr size_t kSmem = (size_t)W * S * SB;
   static_assert(S >= 3 && kSmem <= kRingBytes, "ring");
   // a warp's two parts, 16 heads each at most, fit into its ring
@@ -920,6 +934,14 @@ __global__ void __launch_bounds__(kJoinWarps * 32)
 
 inline int head_tiles(int64_t Hq, int64_t Hkv, int64_t D) { return Hq / Hkv > 8 && D <= 128 ? 2 : 1; }
 
+// One CTA per SM, but no more than the block tables' room could have tiles for.
+inline int split_grid(int64_t R, int64_t Hq, int64_t Hkv, int64_t D, int rb, int64_t room) {
+  const int nt = head_tiles(Hq, Hkv, D), ngr = (int)((Hq / Hkv + 8 * nt - 1) / (8 * nt));
+  const int64_t tiles = (room + tile_keys(rb) - 1) / tile_keys(rb) + 1;
+  const int64_t most = (tiles + kItemCost) * R * Hkv * ngr / (kMinShare * split_warps(rb)) + 1;
+  return (int)std::min<int64_t>(num_sms(), most);
+}
+
 // Floats of one partial result.
 inline int64_t part_floats(int64_t Hq, int64_t Hkv, int64_t D) {
   return head_tiles(Hq, Hkv, D) * 8 * (D + 2);
@@ -934,13 +956,8 @@ int launch(Args& a, void* workspace, cudaStream_t st) {
   auto split = k_paged_split<T, C, D, NT>;
   RB_CUDA(cudaFuncSetAttribute(split, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                (int)X::kSmem));
-  // no more CTAs than the tables' room has tiles for
-  const int ngr = (a.Hq / a.Hkv + 8 * NT - 1) / (8 * NT);
-  const int64_t room_tiles = ((int64_t)a.max_blocks * a.bs + X::KT - 1) / X::KT + 1;
-  const int64_t most =
-      (room_tiles + kItemCost) * a.R * a.Hkv * ngr / (kMinShare * X::W) + 1;
   const int sms = num_sms();
-  const int grid = (int)std::min<int64_t>(sms, std::max<int64_t>(most, 1));
+  const int grid = split_grid(a.R, a.Hq, a.Hkv, D, X::RB, (int64_t)a.max_blocks * a.bs);
   Room room;
   room.first = static_cast<float*>(workspace);
   room.cross = room.first + (int64_t)sms * X::W * PF;

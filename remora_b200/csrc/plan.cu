@@ -88,6 +88,31 @@ void hetero_plan(Text& t) {
   t.add("  rb::moe::k_combine<2>  grid 64 x block 256\n");
 }
 
+// One decoding step: tables, append and attention of R requests of up to S keys.
+void decode_plan(Text& t, int64_t R, int64_t Hq, int64_t Hkv, int64_t S) {
+  const int64_t D = 128, bs = 16, mb = (S + 1 + bs - 1) / bs;
+  const int nt = paged::head_tiles(Hq, Hkv, D), rb = (int)D * 2;
+  const int grid = paged::split_grid(R, Hq, Hkv, D, rb, mb * bs);
+  t.add("remora_b200_kv_block_table(lens i32[%lld], table i32[%lld,%lld], %lld tokens)\n",
+        (long long)R, (long long)R, (long long)mb, (long long)R);
+  const kv::Launch l = kv::launch_of(R, R);
+  t.add("  rb::kv::k_block_table  grid %d x block %d, one cluster, smem %zu B\n", l.ctas, l.threads,
+        l.smem);
+  t.add("remora_b200_rope_kv_append(q bf16[%lld,%lld,128], k/v bf16[%lld,%lld,128], cache blocks of "
+        "%lld tokens)\n", (long long)R, (long long)Hq, (long long)R, (long long)Hkv, (long long)bs);
+  t.add("  rb::rope::k_rope  grid %lld x block %d (whole heads in units of 8 pairs)\n",
+        (long long)std::min<int64_t>(R, (int64_t)num_sms() * 16), rope::kThreads);
+  t.add("remora_b200_paged_attention(q bf16[%lld,%lld,128], %lld kv heads, up to %lld keys)\n",
+        (long long)R, (long long)Hq, (long long)Hkv, (long long)S + 1);
+  t.add("  rb::paged::k_paged_split  grid %d x block %d, smem %d B (tiles of %d keys, %d in a "
+        "warp's ring, %d heads to a warp)\n", grid, paged::split_warps(rb) * 32,
+        paged::split_warps(rb) * paged::ring_tiles(rb) * paged::tile_bytes(rb),
+        paged::tile_keys(rb), paged::ring_tiles(rb), 8 * nt);
+  if (grid > 1)
+    t.add("  rb::paged::k_paged_join  grid %d x %lld x block %d\n", grid, (long long)(nt * D / 16),
+          paged::kJoinWarps * 32);
+}
+
 }  // namespace plan
 }  // namespace rb
 
@@ -137,6 +162,11 @@ extern "C" int remora_b200_launch_plan(const char* test, const char* config, cha
     t.add("  rb::attnp::k_attention_persist  grid %lld x block %d, smem %u B (persistent: %lld "
           "work items of one (b,h) and 256 query rows)\n",
           std::min<long long>(items, num_sms()), attnp::kThreads, attn::kSmemBytes, items);
+  } else if (kind == "decode") {
+    int64_t R, Hq, Hkv, S;
+    if (!decode_config(c.c_str(), &R, &Hq, &Hkv, &S))
+      return fail(REMORA_B200_ERR_INVALID, "launch_plan: unknown decode config '%s'", c.c_str());
+    decode_plan(t, R, Hq, Hkv, S);
   } else if (kind == "moe") {
     if (c.empty() || c == "4")
       moe_plan(t, 8192, 4096, 14336, 8, 2);

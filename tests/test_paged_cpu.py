@@ -152,6 +152,18 @@ def test_attention_without_requests_is_done_and_workspace_sizes(L):
         assert L.remora_b200_paged_attention_workspace_bytes(*bad) == 0
 
 
+def test_decode_program_is_recognised_and_planned(L):
+    assert rb.recognise("decode")
+    plan = rb.launch_plan("decode")
+    for word in ("remora_b200_kv_block_table", "k_block_table", "remora_b200_rope_kv_append",
+                 "k_rope", "remora_b200_paged_attention", "k_paged_split", "k_paged_join", "grid"):
+        assert word in plan
+    assert "k_paged_join" not in rb.launch_plan("decode", "1x1x1x1")  # one CTA: nothing to join
+    for bad in ("64", "0x8x2x16", "4x7x2x16", "9000x8x2x16", "4x8x2x0", "8192x8x2x1048576"):
+        with pytest.raises(rb.RemoraError, match="decode config"):
+            rb.launch_plan("decode", bad)
+
+
 def test_python_mirrors_refuse_host_tensors_and_bad_shapes():
     i = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
     b = lambda *s: torch.zeros(s, dtype=torch.bfloat16)  # noqa: E731

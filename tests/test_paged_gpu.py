@@ -551,6 +551,26 @@ def test_attention_past_32_bit_offsets(rb):
 
 
 # ------------------------------------------------------------- the step together
+@pytest.mark.parametrize("config", [None, "3x8x2x100", "1x16x1x5000", "40x4x4x33"])
+def test_run_test_decode(rb, config):
+    rep = rb.run_test("decode", iters=2, warmup=1, config=config)
+    assert rep["passed"] and rep["checked"] == 32 * 128 and rep["max_rel_err"] <= 2e-2
+
+
+def test_cli_decode(rb, tmp_path):
+    import os
+    import subprocess
+
+    from remora_b200 import build
+
+    prog = tmp_path / "prog.mlir"
+    prog.write_text("func.func public @main()\n")
+    r = subprocess.run([build.CLI, str(prog), "--run-gpu", "--test=decode",
+                        "--config=2x8x4x300"], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "Validation: PASS" in r.stdout and "decode step" in r.stdout
+    assert os.path.exists(build.CLI)
+
+
 @pytest.mark.parametrize("dtype,cache", TYPES)
 def test_serving_steps(rb, dtype, cache):
     """Prompts, then decoding steps, a release and a newcomer: tables, append and attention in
