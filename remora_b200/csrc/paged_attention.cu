@@ -23,7 +23,7 @@ constexpr int kMaxRequests = 8192;
 constexpr int kRingBytes = 196608;  // shared memory of a CTA's rings
 constexpr int kItemCost = 2;         // what starting and ending an item costs, in tiles
 constexpr int kMinShare = 2;        // tiles and items' costs of a warp at least
-constexpr int kMostWarps = 8;
+constexpr int kMostWarps = 12;
 
 struct Args {
   const void *q, *kc, *vc;
@@ -112,32 +112,37 @@ __device__ __forceinline__ float2 unpack2(uint32_t x) {
 }
 
 // ------------------------------------------------------------------ shapes
-// By the bytes of a row (head_dim elements of the cache): the keys of a tile, a tile's keys and
-// values in bytes, the warps of a CTA and the tiles of a warp's ring.  8 KB tiles and 24 KB rings
-// for 8 warps, so that 16 KB are in flight per warp while it computes.  12 or 16 warps of half
-// the keys measured slower: 128 ragged requests of 64-element f16 rows 60 and 67 us against 56
-// (more instructions per key, the same bytes in flight).
-constexpr int tile_keys(int rb) { return rb <= 128 ? 32 : 16; }
-constexpr int tile_bytes(int rb) { return 2 * tile_keys(rb) * rb; }
-constexpr int split_warps(int rb) { return tile_bytes(rb) > 8192 ? 4 : kMostWarps; }
-constexpr int ring_tiles(int rb) {
-  return kRingBytes / (split_warps(rb) * tile_bytes(rb)) > 6
+// By the bytes of a row (head_dim elements of the cache) and of an element: the keys of a tile, a
+// tile's keys and values in bytes, the warps of a CTA and the tiles of a warp's ring.  8 KB tiles
+// and rings of 3 for 8 warps keep 16 KB in flight per warp while it computes.  8-bit rows of 128
+// elements take the most instructions per byte (every element is widened), and 8 warps do not
+// hide their latencies: 12 with rings of 2 take 121 us where 8 take 129 (3 requests of 90 to 131
+// thousand keys); for 16-bit rows of the same size 12 warps measure alike (53.2 and 52.6 us, 128
+// ragged requests), and 12 or 16 warps of half the keys slower (60 and 67 us against 56: more
+// instructions per key).
+__host__ __device__ constexpr int tile_keys(int rb) { return rb <= 128 ? 32 : 16; }
+__host__ __device__ constexpr int tile_bytes(int rb) { return 2 * tile_keys(rb) * rb; }
+__host__ __device__ constexpr int split_warps(int rb, int elem) {
+  return tile_bytes(rb) > 8192 ? 4 : elem == 1 && rb == 128 ? kMostWarps : 8;
+}
+__host__ __device__ constexpr int ring_tiles(int rb, int elem) {
+  return kRingBytes / (split_warps(rb, elem) * tile_bytes(rb)) > 6
              ? 6
-             : kRingBytes / (split_warps(rb) * tile_bytes(rb));
+             : kRingBytes / (split_warps(rb, elem) * tile_bytes(rb));
 }
 
-template <typename C, int D>
+template <typename C, int D, int NT>
 struct Shape {
   static constexpr int RB = D * (int)sizeof(C);  // bytes of a row
   static constexpr int CH = RB / 16;             // 16-byte pieces of a row
   static constexpr int KT = tile_keys(RB);
   static constexpr int SB = tile_bytes(RB);
-  static constexpr int W = split_warps(RB);
-  static constexpr int S = ring_tiles(RB);
-  static constexpr size_t kSmem = (size_t)W * S * SB;
-  static_assert(S >= 3 && kSmem <= kRingBytes, "ring");
-  // a warp's two parts, 16 heads each at most, fit into its ring
-  static_assert(2 * (D == 256 ? 8 : 16) * (D + 2) * 4 <= S * SB, "parts");
+  static constexpr int W = split_warps(RB, sizeof(C));
+  static constexpr int S = ring_tiles(RB, sizeof(C));
+  // a warp's ring; its two parts, in 32 bits, lie there in the end
+  static constexpr int kRing = S * SB > 2 * NT * 8 * (D + 2) * 4 ? S * SB : 2 * NT * 8 * (D + 2) * 4;
+  static constexpr size_t kSmem = (size_t)W * kRing;
+  static_assert(S >= 2 && kSmem <= 200 * 1024, "ring");
 };
 
 // Piece c of row `row` lies at piece c ^ swz(row): the eight rows of an ldmatrix
@@ -195,7 +200,7 @@ __device__ __forceinline__ int64_t warp_sum(int32_t v) {
 // A warp's walk over its tiles, as it fetches them.
 template <typename T, typename C, int D, int kHeads>
 struct Walk {
-  using X = Shape<C, D>;
+  using X = Shape<C, D, kHeads / 8>;
   int64_t at, end;     // the tile to come and the end of the walk, in shares
   int32_t g, r, h;     // group of 32 requests, request, item of the request
   int32_t t, t0, t1;   // tile, and the request's
@@ -354,8 +359,15 @@ __device__ __forceinline__ void store_fragment(T* out, int64_t o_h, int heads, i
   }
 }
 
+// The weights 2^(s - m) are kept times 2^kLift: with f16 pieces 2^14, so that weights down to
+// 2^-38 of the largest are seen (131072 keys of 2^-24 each may outweigh it); l and the products
+// carry the same factor, so only the logarithm takes it off.
+template <typename T, typename C>
+constexpr float kLift = sizeof(C) == 1 || std::is_same<T, __half>::value ? 14.0f : 0.0f;
+
+template <typename T, typename C>
 __device__ __forceinline__ float lse_of(float m, float l) {
-  return l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+  return l == 0.0f ? -INFINITY : (m - kLift<T, C> + log2f(l)) * 0.6931471805599453f;
 }
 // 2^(m - top), where top may be -inf (then so is m: nothing was seen).
 __device__ __forceinline__ float weight(float m, float top) {
@@ -380,9 +392,9 @@ struct Room {
 };
 
 template <typename T, typename C, int D, int NT>
-__global__ void __launch_bounds__(Shape<C, D>::W * 32, 1)
+__global__ void __launch_bounds__(Shape<C, D, NT>::W * 32, 1)
     k_paged_split(const __grid_constant__ Args a, const Room room) {
-  using X = Shape<C, D>;
+  using X = Shape<C, D, NT>;
   using M = typename std::conditional<sizeof(C) == 1, __half, T>::type;  // the product's type
   constexpr int W = X::W, S = X::S, KT = X::KT, PF = kPartFloats<D, NT>;
   constexpr bool F8 = sizeof(C) == 1;
@@ -448,7 +460,7 @@ __global__ void __launch_bounds__(Shape<C, D>::W * 32, 1)
     }
   }
 
-  char* ring = ring_all + (size_t)warp * S * X::SB;
+  char* ring = ring_all + (size_t)warp * X::kRing;
   if (begin < total) {
     Walk<T, C, D, 8 * NT> w;
     w.at = w.end = min(begin + quota, total);
@@ -637,6 +649,7 @@ __global__ void __launch_bounds__(Shape<C, D>::W * 32, 1)
         top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
         base[n] = top == -INFINITY ? 0.0f : top;
         c[n] = exp2_ftz(m[n] - base[n]);
+        base[n] -= kLift<T, C>;
         grew |= top > m[n];
         m[n] = top;
       }
@@ -720,7 +733,7 @@ __global__ void __launch_bounds__(Shape<C, D>::W * 32, 1)
                                    make_float4(o[n][j][0] * i0, o[n][j][1] * i1, o[n][j][2] * i0,
                                                o[n][j][3] * i1));
             if (a.lse && t4 == 0 && g + 8 * n < heads)
-              a.lse[(int64_t)st.r * a.Hq + head0 + g + 8 * n] = lse_of(m[n], l[n]);
+              a.lse[(int64_t)st.r * a.Hq + head0 + g + 8 * n] = lse_of<T, C>(m[n], l[n]);
           }
         } else {
           // a part: the first of several is put aside in the workspace, the last one in this
@@ -749,7 +762,8 @@ __global__ void __launch_bounds__(Shape<C, D>::W * 32, 1)
         }
       }
       if (last) break;
-      st = stages[warp][rs];  // written two fetches ago
+      if (S == 2) __syncwarp();  // written in this turn; with more tiles, before the last wait
+      st = stages[warp][rs];
       if (st.r < 0) break;
       if (st.flags & 1) load_queries(st);
     }
@@ -770,10 +784,10 @@ __global__ void __launch_bounds__(Shape<C, D>::W * 32, 1)
   // item are neighbours in that order; a run that lacks the item's first or last tile crosses
   // into another CTA.
   auto part = [&](int e) {
-    return reinterpret_cast<const float*>(ring_all + (size_t)(e >> 1) * S * X::SB) +
+    return reinterpret_cast<const float*>(ring_all + (size_t)(e >> 1) * X::kRing) +
            (e & 1 ? 0 : PF);
   };
-  static_assert(2 * W <= 16, "a lane per entry");
+  static_assert(2 * W <= 32, "a lane per entry");
   int my_item = lane < 2 * W ? p_item[lane] : -1;
   const bool real = my_item >= 0;
   const uint32_t reals = __ballot_sync(~0u, real), upto = reals & ((2u << lane) - 1);
@@ -784,7 +798,7 @@ __global__ void __launch_bounds__(Shape<C, D>::W * 32, 1)
   if (leads) {  // (the same in all warps)
 #pragma unroll 1
     for (int h = warp; h < 8 * NT; h += W) {
-      const float* p = part(lane & (2 * W - 1)) + NT * 8 * D + h;
+      const float* p = part(min(lane, 2 * W - 1)) + NT * 8 * D + h;
       const float pm = real ? p[0] : -INFINITY;
       float top = pm, sum;
 #pragma unroll
@@ -841,8 +855,8 @@ __global__ void __launch_bounds__(Shape<C, D>::W * 32, 1)
         store_fragment<T, C>((T*)a.out + r * a.o_t + head0 * a.o_h, a.o_h, heads, n, j, lane,
                              make_float4(c.x * i0, c.y * i1, c.z * i0, c.w * i1));
         if (a.lse && j == 0 && g == 0) {
-          if (hh < heads) a.lse[(int64_t)r * a.Hq + head0 + hh] = lse_of(m0, l0);
-          if (hh + 1 < heads) a.lse[(int64_t)r * a.Hq + head0 + hh + 1] = lse_of(m1, l1);
+          if (hh < heads) a.lse[(int64_t)r * a.Hq + head0 + hh] = lse_of<T, C>(m0, l0);
+          if (hh + 1 < heads) a.lse[(int64_t)r * a.Hq + head0 + hh + 1] = lse_of<T, C>(m1, l1);
         }
       } else {
         reinterpret_cast<float4*>(to)[f * 32 + lane] = c;
@@ -927,18 +941,19 @@ __global__ void __launch_bounds__(kJoinWarps * 32)
   store_fragment<T, C>((T*)a.out + r * a.o_t + head0 * a.o_h, a.o_h, heads, n, j, lane,
                        make_float4(c.x * i0, c.y * i1, c.z * i0, c.w * i1));
   if (a.lse && j == 0 && (lane >> 2) == 0) {
-    if (hh < heads) a.lse[(int64_t)r * a.Hq + head0 + hh] = lse_of(m0, l0);
-    if (hh + 1 < heads) a.lse[(int64_t)r * a.Hq + head0 + hh + 1] = lse_of(m1, l1);
+    if (hh < heads) a.lse[(int64_t)r * a.Hq + head0 + hh] = lse_of<T, C>(m0, l0);
+    if (hh + 1 < heads) a.lse[(int64_t)r * a.Hq + head0 + hh + 1] = lse_of<T, C>(m1, l1);
   }
 }
 
 inline int head_tiles(int64_t Hq, int64_t Hkv, int64_t D) { return Hq / Hkv > 8 && D <= 128 ? 2 : 1; }
 
 // One CTA per SM, but no more than the block tables' room could have tiles for.
-inline int split_grid(int64_t R, int64_t Hq, int64_t Hkv, int64_t D, int rb, int64_t room) {
+inline int split_grid(int64_t R, int64_t Hq, int64_t Hkv, int64_t D, int elem, int64_t room) {
   const int nt = head_tiles(Hq, Hkv, D), ngr = (int)((Hq / Hkv + 8 * nt - 1) / (8 * nt));
+  const int rb = (int)D * elem;
   const int64_t tiles = (room + tile_keys(rb) - 1) / tile_keys(rb) + 1;
-  const int64_t most = (tiles + kItemCost) * R * Hkv * ngr / (kMinShare * split_warps(rb)) + 1;
+  const int64_t most = (tiles + kItemCost) * R * Hkv * ngr / (kMinShare * split_warps(rb, elem)) + 1;
   return (int)std::min<int64_t>(num_sms(), most);
 }
 
@@ -949,7 +964,7 @@ inline int64_t part_floats(int64_t Hq, int64_t Hkv, int64_t D) {
 
 template <typename T, typename C, int D, int NT>
 int launch(Args& a, void* workspace, cudaStream_t st) {
-  using X = Shape<C, D>;
+  using X = Shape<C, D, NT>;
   a.k_step = a.kc_t * (int64_t)sizeof(C) * (32 / X::CH);
   a.v_step = a.vc_t * (int64_t)sizeof(C) * (32 / X::CH);
   constexpr int PF = kPartFloats<D, NT>;
@@ -957,7 +972,7 @@ int launch(Args& a, void* workspace, cudaStream_t st) {
   RB_CUDA(cudaFuncSetAttribute(split, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                (int)X::kSmem));
   const int sms = num_sms();
-  const int grid = split_grid(a.R, a.Hq, a.Hkv, D, X::RB, (int64_t)a.max_blocks * a.bs);
+  const int grid = split_grid(a.R, a.Hq, a.Hkv, D, sizeof(C), (int64_t)a.max_blocks * a.bs);
   Room room;
   room.first = static_cast<float*>(workspace);
   room.cross = room.first + (int64_t)sms * X::W * PF;

@@ -92,7 +92,7 @@ void hetero_plan(Text& t) {
 void decode_plan(Text& t, int64_t R, int64_t Hq, int64_t Hkv, int64_t S) {
   const int64_t D = 128, bs = 16, mb = (S + 1 + bs - 1) / bs;
   const int nt = paged::head_tiles(Hq, Hkv, D), rb = (int)D * 2;
-  const int grid = paged::split_grid(R, Hq, Hkv, D, rb, mb * bs);
+  const int grid = paged::split_grid(R, Hq, Hkv, D, 2, mb * bs);
   t.add("remora_b200_kv_block_table(lens i32[%lld], table i32[%lld,%lld], %lld tokens)\n",
         (long long)R, (long long)R, (long long)mb, (long long)R);
   const kv::Launch l = kv::launch_of(R, R);
@@ -105,9 +105,9 @@ void decode_plan(Text& t, int64_t R, int64_t Hq, int64_t Hkv, int64_t S) {
   t.add("remora_b200_paged_attention(q bf16[%lld,%lld,128], %lld kv heads, up to %lld keys)\n",
         (long long)R, (long long)Hq, (long long)Hkv, (long long)S + 1);
   t.add("  rb::paged::k_paged_split  grid %d x block %d, smem %d B (tiles of %d keys, %d in a "
-        "warp's ring, %d heads to a warp)\n", grid, paged::split_warps(rb) * 32,
-        paged::split_warps(rb) * paged::ring_tiles(rb) * paged::tile_bytes(rb),
-        paged::tile_keys(rb), paged::ring_tiles(rb), 8 * nt);
+        "warp's ring, %d heads to a warp)\n", grid, paged::split_warps(rb, 2) * 32,
+        paged::split_warps(rb, 2) * paged::ring_tiles(rb, 2) * paged::tile_bytes(rb),
+        paged::tile_keys(rb), paged::ring_tiles(rb, 2), 8 * nt);
   if (grid > 1)
     t.add("  rb::paged::k_paged_join  grid %d x %lld x block %d\n", grid, (long long)(nt * D / 16),
           paged::kJoinWarps * 32);
