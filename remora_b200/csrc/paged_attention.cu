@@ -122,13 +122,13 @@ __device__ __forceinline__ float2 unpack2(uint32_t x) {
 // instructions per key).
 __host__ __device__ constexpr int tile_keys(int rb) { return rb <= 128 ? 32 : 16; }
 __host__ __device__ constexpr int tile_bytes(int rb) { return 2 * tile_keys(rb) * rb; }
-__host__ __device__ constexpr int split_warps(int rb, int elem) {
-  return tile_bytes(rb) > 8192 ? 4 : elem == 1 && rb == 128 ? kMostWarps : 8;
+__host__ __device__ constexpr int split_warps(int rb, int elem, int nt) {
+  return tile_bytes(rb) > 8192 ? 4 : elem == 1 && rb <= 128 && nt == 1 ? kMostWarps : 8;
 }
-__host__ __device__ constexpr int ring_tiles(int rb, int elem) {
-  return kRingBytes / (split_warps(rb, elem) * tile_bytes(rb)) > 6
+__host__ __device__ constexpr int ring_tiles(int rb, int elem, int nt) {
+  return kRingBytes / (split_warps(rb, elem, nt) * tile_bytes(rb)) > 6
              ? 6
-             : kRingBytes / (split_warps(rb, elem) * tile_bytes(rb));
+             : kRingBytes / (split_warps(rb, elem, nt) * tile_bytes(rb));
 }
 
 template <typename C, int D, int NT>
@@ -137,8 +137,8 @@ struct Shape {
   static constexpr int CH = RB / 16;             // 16-byte pieces of a row
   static constexpr int KT = tile_keys(RB);
   static constexpr int SB = tile_bytes(RB);
-  static constexpr int W = split_warps(RB, sizeof(C));
-  static constexpr int S = ring_tiles(RB, sizeof(C));
+  static constexpr int W = split_warps(RB, sizeof(C), NT);
+  static constexpr int S = ring_tiles(RB, sizeof(C), NT);
   // a warp's ring; its two parts, in 32 bits, lie there in the end
   static constexpr int kRing = S * SB > 2 * NT * 8 * (D + 2) * 4 ? S * SB : 2 * NT * 8 * (D + 2) * 4;
   static constexpr size_t kSmem = (size_t)W * kRing;
@@ -226,7 +226,7 @@ struct Walk {
     ok = key >= start && key < n;
     id = -1;
     off = 0;
-    if (ok) {
+    if (key < n) {  // (a key in front of the window may share its block with one that counts)
       const int32_t page = a.page.div(key);
       off = key - page * a.bs;
       id = __ldg(a.table + (int64_t)r * a.ld_table + page);
@@ -282,12 +282,15 @@ struct Walk {
       constexpr int kRows = 32 / X::CH, kSteps = X::KT / kRows;
       const int lr = lane / X::CH, c = lane % X::CH;
       const uint32_t kd = smem_u32(ring) + lr * X::RB, vd = kd + X::KT * X::RB;
-      if (a.whole16 && mask == kAll) {
-        // every key counts, and the rows of 16 keys follow one another in their block: one
-        // address for each 16, then steps of kRows rows
+      // the rows of 16 keys follow one another in their block: one address for each 16, then
+      // steps of kRows rows (what does not count is zeros; 16 keys that share a block with one
+      // that counts lie in the cache)
+      auto rows = [&](auto every) {
 #pragma unroll
         for (int g16 = 0; g16 < X::KT / 16; ++g16) {
-          const int64_t b = __shfl_sync(~0u, id, 16 * g16), o = __shfl_sync(~0u, off, 16 * g16) + lr;
+          int64_t b = __shfl_sync(~0u, id, 16 * g16);
+          const int64_t o = __shfl_sync(~0u, off, 16 * g16) + lr;
+          if (!every.value && (mask >> 16 * g16 & 0xffffu) == 0) b = 0;  // no address to take
           const char* ks = (const char*)a.kc +
                            (b * a.kc_b + o * a.kc_t + (int64_t)hk * a.kc_h) * (int)sizeof(C) + c * 16;
           const char* vs = (const char*)a.vc +
@@ -296,12 +299,23 @@ struct Walk {
           for (int i = 0; i < 16 / kRows; ++i) {
             const int row = 16 * g16 + i * kRows;  // and lr more
             const int at = row * X::RB + ((c ^ swz<X::RB>(row + lr)) << 4);
-            copy16(kd + at, ks);
-            copy16(vd + at, vs);
+            if constexpr (every.value) {
+              copy16(kd + at, ks);
+              copy16(vd + at, vs);
+            } else {
+              const bool there = mask >> (row + lr) & 1;
+              copy16(kd + at, ks, there);
+              copy16(vd + at, vs, there);
+            }
             ks += a.k_step;
             vs += a.v_step;
           }
         }
+      };
+      if (a.whole16 && mask == kAll) {
+        rows(std::true_type());
+      } else if (a.whole16) {
+        rows(std::false_type());
       } else {
         int64_t ko = 0, vo = 0;
         if (in) {
@@ -511,8 +525,8 @@ __global__ void __launch_bounds__(Shape<C, D, NT>::W * 32, 1)
     const int fswz = swz<X::RB>(lrow);
     // an item's queries, as they are
     auto load_queries = [&](const Stage& st) {
-      const int sub = st.h % ngr;
-      head0 = st.h / ngr * gq + sub * 8 * NT;
+      const int hk = ngr == 1 ? st.h : st.h / ngr, sub = st.h - hk * ngr;
+      head0 = hk * gq + sub * 8 * NT;
       heads = min(8 * NT, gq - sub * 8 * NT);
       const T* qp = (const T*)a.q + st.r * a.q_t + head0 * a.q_h;
 #pragma unroll
@@ -953,7 +967,7 @@ inline int split_grid(int64_t R, int64_t Hq, int64_t Hkv, int64_t D, int elem, i
   const int nt = head_tiles(Hq, Hkv, D), ngr = (int)((Hq / Hkv + 8 * nt - 1) / (8 * nt));
   const int rb = (int)D * elem;
   const int64_t tiles = (room + tile_keys(rb) - 1) / tile_keys(rb) + 1;
-  const int64_t most = (tiles + kItemCost) * R * Hkv * ngr / (kMinShare * split_warps(rb, elem)) + 1;
+  const int64_t most = (tiles + kItemCost) * R * Hkv * ngr / (kMinShare * split_warps(rb, elem, nt)) + 1;
   return (int)std::min<int64_t>(num_sms(), most);
 }
 

@@ -105,9 +105,9 @@ void decode_plan(Text& t, int64_t R, int64_t Hq, int64_t Hkv, int64_t S) {
   t.add("remora_b200_paged_attention(q bf16[%lld,%lld,128], %lld kv heads, up to %lld keys)\n",
         (long long)R, (long long)Hq, (long long)Hkv, (long long)S + 1);
   t.add("  rb::paged::k_paged_split  grid %d x block %d, smem %d B (tiles of %d keys, %d in a "
-        "warp's ring, %d heads to a warp)\n", grid, paged::split_warps(rb, 2) * 32,
-        paged::split_warps(rb, 2) * paged::ring_tiles(rb, 2) * paged::tile_bytes(rb),
-        paged::tile_keys(rb), paged::ring_tiles(rb, 2), 8 * nt);
+        "warp's ring, %d heads to a warp)\n", grid, paged::split_warps(rb, 2, nt) * 32,
+        paged::split_warps(rb, 2, nt) * paged::ring_tiles(rb, 2, nt) * paged::tile_bytes(rb),
+        paged::tile_keys(rb), paged::ring_tiles(rb, 2, nt), 8 * nt);
   if (grid > 1)
     t.add("  rb::paged::k_paged_join  grid %d x %lld x block %d\n", grid, (long long)(nt * D / 16),
           paged::kJoinWarps * 32);
