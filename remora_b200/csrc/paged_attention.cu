@@ -64,13 +64,13 @@ template <typename M>
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
                                          uint32_t a3, uint32_t b0, uint32_t b1) {
   if constexpr (std::is_same<M, __half>::value)
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
         "{%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   else
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
         "{%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -297,8 +297,8 @@ struct Walk {
                            (b * a.vc_b + o * a.vc_t + (int64_t)hk * a.vc_h) * (int)sizeof(C) + c * 16;
 #pragma unroll
           for (int i = 0; i < 16 / kRows; ++i) {
-            const int row = 16 * g16 + i * kRows;  // and lr more
-            const int at = row * X::RB + ((c ^ swz<X::RB>(row + lr)) << 4);
+            const int row = 16 * g16 + i * kRows;  // and lr more: swz is a xor of the two
+            const int at = row * X::RB + ((c ^ swz<X::RB>(lr) ^ swz<X::RB>(row)) << 4);
             if constexpr (every.value) {
               copy16(kd + at, ks);
               copy16(vd + at, vs);
@@ -411,7 +411,7 @@ __global__ void __launch_bounds__(Shape<C, D, NT>::W * 32, 1)
   using X = Shape<C, D, NT>;
   using M = typename std::conditional<sizeof(C) == 1, __half, T>::type;  // the product's type
   constexpr int W = X::W, S = X::S, KT = X::KT, PF = kPartFloats<D, NT>;
-  constexpr bool F8 = sizeof(C) == 1;
+  constexpr bool F8 = sizeof(C) == 1, kTwo = !F8 || std::is_same<T, __half>::value;
   extern __shared__ __align__(128) char ring_all[];
   __shared__ int64_t before[kMaxRequests / 32 + 1];
   __shared__ Stage stages[W][S];
@@ -516,13 +516,24 @@ __global__ void __launch_bounds__(Shape<C, D, NT>::W * 32, 1)
     }
     uint32_t q[D / 16][2 * NT];
     float o[NT][D / 16][4];
-    float m[NT], l[NT], sc[NT];
+    float m[NT][2], l[NT][2], sc[NT][2];  // of heads 2 t4 and 2 t4 + 1 of each group of eight
     bool began = false;
     int head0 = 0, heads = 0;  // the item's query heads
     const int lrow = lane & 7, lhalf = (lane >> 3) & 1, lsec = lane >> 4;
-    // where this lane points ldmatrix: 16-bit rows (keys by lsec, d's by lhalf), 8-bit the reverse
-    const int frow = (F8 ? lhalf : lsec) * 8 + lrow, fpiece = F8 ? lsec : lhalf;
-    const int fswz = swz<X::RB>(lrow);
+    // where this lane points ldmatrix, from a tile's keys (values) on.  Four 8 x 8 matrices: the
+    // keys' are [keys 0-7 | 8-15] x [d's | the next], in that order (an A operand: keys x d's);
+    // the values' of 16 bits [d's | the next] x [keys 0-7 | 8-15] (its transpose: d's x keys), of
+    // 8 bits as the keys'.
+    constexpr int kStep = F8 ? 2 : 1;  // 16 d's of 8 bits are one 16-byte piece, of 16 bits two
+    uint32_t kpiece[D / 16 / kStep], vpiece[D / 16 / kStep];
+#pragma unroll
+    for (int j = 0; j < D / 16; j += kStep) {
+      const int base = F8 ? j : 2 * j;
+      kpiece[j / kStep] = (lhalf * 8 + lrow) * X::RB + (((base + lsec) ^ swz<X::RB>(lrow)) << 4);
+      vpiece[j / kStep] = F8 ? kpiece[j / kStep]
+                             : (lsec * 8 + lrow) * X::RB +
+                                   (((base + lhalf) ^ swz<X::RB>(lrow)) << 4);
+    }
     // an item's queries, as they are
     auto load_queries = [&](const Stage& st) {
       const int hk = ngr == 1 ? st.h : st.h / ngr, sub = st.h - hk * ngr;
@@ -582,9 +593,20 @@ __global__ void __launch_bounds__(Shape<C, D, NT>::W * 32, 1)
                                               __uint_as_float(v & 0xffff0000u) * inv);
             }
         }
-        sc[n] = a.scale2 * fac;
-        m[n] = -INFINITY;
-        l[n] = 0.0f;
+        // the scale's sign goes to the queries, so that the maximum is found before scaling; a
+        // scale of zero is queries of zero (a masked score stays -inf)
+        const float f = fmaxf(fabsf(a.scale2) * fac, 1.2e-38f);  // of this lane's row, head g
+        sc[n][0] = __shfl_sync(~0u, f, 8 * t4);
+        sc[n][1] = __shfl_sync(~0u, f, 8 * t4 + 4);
+        if (a.scale2 <= 0.0f) {
+#pragma unroll
+          for (int j = 0; j < D / 16; ++j)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              q[j][2 * n + e] = a.scale2 == 0.0f ? 0u : q[j][2 * n + e] ^ 0x80008000u;
+        }
+        m[n][0] = m[n][1] = -INFINITY;
+        l[n][0] = l[n][1] = 0.0f;
 #pragma unroll
         for (int j = 0; j < D / 16; ++j)
 #pragma unroll
@@ -608,117 +630,131 @@ __global__ void __launch_bounds__(Shape<C, D, NT>::W * 32, 1)
         load_queries(st);
         continue;
       }
-      const uint32_t kb = smem_u32(ring + rs * X::SB), vb = kb + KT * X::RB;
+      const uint32_t kb = smem_u32(ring + rs * X::SB);
       rs = rs + 1 == S ? 0 : rs + 1;
       if (st.flags & 1) start_item(st);
 
-      // scores: rows = heads, columns = keys
-      float s[KT / 8][4];
+      // scores: rows = keys, columns = heads
+      float s[KT / 16][NT][4];
 #pragma unroll
-      for (int n = 0; n < KT / 8; ++n)
+      for (int k2 = 0; k2 < KT / 16; ++k2)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[n][e] = 0.0f;
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-      for (int k2 = 0; k2 < KT / 16; ++k2) {
-        const uint32_t rowp = kb + (k2 * 16 + frow) * X::RB;
+          for (int e = 0; e < 4; ++e) s[k2][n][e] = 0.0f;
 #pragma unroll
-        for (int j = 0; j < D / 16; j += F8 ? 2 : 1) {
+      for (int j = 0; j < D / 16; j += kStep) {
+        const uint32_t at = kb + kpiece[j / kStep];
+#pragma unroll
+        for (int k2 = 0; k2 < KT / 16; ++k2) {
           uint32_t b[4];
+          ldm_x4(b, at + k2 * 16 * X::RB);
           if constexpr (F8) {
-            ldm_x4(b, rowp + (((j + fpiece) ^ fswz) << 4));
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-              const uint32_t* aq = q[j + (u >> 1)];
-              mma16816<M>(s[2 * k2 + (u & 1)], aq[0], NT == 2 ? aq[2 * NT - 2] : 0u, aq[1],
-                          NT == 2 ? aq[2 * NT - 1] : 0u, f16x2_lo(b[u]), f16x2_hi(b[u]));
+            for (int u = 0; u < 2; ++u) {
+              const uint32_t a0 = f16x2_lo(b[2 * u]), a1 = f16x2_lo(b[2 * u + 1]);
+              const uint32_t a2 = f16x2_hi(b[2 * u]), a3 = f16x2_hi(b[2 * u + 1]);
+#pragma unroll
+              for (int n = 0; n < NT; ++n)
+                mma16816<M>(s[k2][n], a0, a1, a2, a3, q[j + u][2 * n], q[j + u][2 * n + 1]);
             }
           } else {
-            ldm_x4(b, rowp + (((2 * j + fpiece) ^ fswz) << 4));
-            const uint32_t* aq = q[j];
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
-              mma16816<M>(s[2 * k2 + u], aq[0], NT == 2 ? aq[2 * NT - 2] : 0u, aq[1],
-                          NT == 2 ? aq[2 * NT - 1] : 0u, b[2 * u], b[2 * u + 1]);
+            for (int n = 0; n < NT; ++n)
+              mma16816<M>(s[k2][n], b[0], b[1], b[2], b[3], q[j][2 * n], q[j][2 * n + 1]);
           }
         }
       }
 
-      // softmax over the keys, per head
-      const bool all = st.mask == (KT == 32 ? ~0u : 0xffffu);
+      // softmax over the keys: this lane has keys g and g + 8 of each 16, and two heads
+      if (st.mask != (KT == 32 ? ~0u : 0xffffu)) {
+#pragma unroll
+        for (int k2 = 0; k2 < KT / 16; ++k2)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (!(st.mask >> (16 * k2 + g + 8 * (e >> 1)) & 1))
+#pragma unroll
+              for (int n = 0; n < NT; ++n) s[k2][n][e] = -INFINITY;
+      }
       bool grew = false;
-      float base[NT], c[NT];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        float top = m[n];
-#pragma unroll
-        for (int k = 0; k < KT / 8; ++k)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float v = s[k][2 * n + e] * sc[n];
-            if (!all && !(st.mask >> (8 * k + 2 * t4 + e) & 1)) v = -INFINITY;
-            s[k][2 * n + e] = v;
-            top = fmaxf(top, v);
-          }
-        top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-        base[n] = top == -INFINITY ? 0.0f : top;
-        c[n] = exp2_ftz(m[n] - base[n]);
-        base[n] -= kLift<T, C>;
-        grew |= top > m[n];
-        m[n] = top;
-      }
-      if (__any_sync(~0u, grew)) {  // a maximum rose: what was summed shrinks
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          l[n] *= c[n];
-          const float c0 = __shfl_sync(~0u, c[n], 8 * t4), c1 = __shfl_sync(~0u, c[n], 8 * t4 + 4);
-#pragma unroll
-          for (int j = 0; j < D / 16; ++j) {
-            o[n][j][0] *= c0;
-            o[n][j][1] *= c1;
-            o[n][j][2] *= c0;
-            o[n][j][3] *= c1;
-          }
-        }
-      }
-      // the weights enter the second product as two pieces of the 16-bit type: one piece
-      // alone would be off by as much as the output's own rounding (2^-9 for bf16, 2^-12 for
-      // f16), and the tensor pipe is idle most of the time
-      uint32_t ph[NT][KT / 8], pl[NT][KT / 8];
+      float base[NT][2], c[NT][2];
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
-        for (int k = 0; k < KT / 8; ++k) {
-          const float x = exp2_ftz(s[k][2 * n] - base[n]);
-          const float y = exp2_ftz(s[k][2 * n + 1] - base[n]);
-          l[n] += x + y;
-          ph[n][k] = pack2<M>(x, y);
-          const float2 w = unpack2<M>(ph[n][k]);
-          pl[n][k] = pack2<M>(x - w.x, y - w.y);
+        for (int h = 0; h < 2; ++h) {
+          float top = fmaxf(s[0][n][h], s[0][n][h + 2]);
+#pragma unroll
+          for (int k2 = 1; k2 < KT / 16; ++k2)
+            top = fmaxf(top, fmaxf(s[k2][n][h], s[k2][n][h + 2]));
+#pragma unroll
+          for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, x));
+          // sc > 0: the largest score is that of the largest product
+          top = fmaxf(m[n][h], top * sc[n][h]);
+          base[n][h] = top == -INFINITY ? 0.0f : top;
+          c[n][h] = exp2_ftz(m[n][h] - base[n][h]);
+          base[n][h] -= kLift<T, C>;
+          grew |= top > m[n][h];
+          m[n][h] = top;
+        }
+      if (__any_sync(~0u, grew)) {  // a maximum rose: what was summed shrinks
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          l[n][0] *= c[n][0];
+          l[n][1] *= c[n][1];
+#pragma unroll
+          for (int j = 0; j < D / 16; ++j) {
+            o[n][j][0] *= c[n][0];
+            o[n][j][1] *= c[n][1];
+            o[n][j][2] *= c[n][0];
+            o[n][j][3] *= c[n][1];
+          }
+        }
+      }
+      // The weights enter the second product as two pieces of the 16-bit type where one would be
+      // off by as much as the output's own rounding.  f16 weights of a bf16 output are one piece:
+      // off by 2^-11 of a weight at most, an eighth of the output's half step (the second piece
+      // costs a third of the tensor work: 127 us instead of 118 for 3 long requests at the clocks
+      // of a lasting load).
+      uint32_t ph[NT][KT / 8], pl[NT][KT / 8];
+#pragma unroll
+      for (int k = 0; k < KT / 8; ++k)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const float* p = &s[k / 2][n][k % 2 * 2];
+          const float x = exp2_ftz(fmaf(p[0], sc[n][0], -base[n][0]));
+          const float y = exp2_ftz(fmaf(p[1], sc[n][1], -base[n][1]));
+          l[n][0] += x;
+          l[n][1] += y;
+          const uint32_t w = pack2<M>(x, y);
+          ph[n][k] = transpose8x8(w);  // keys x heads -> a B operand's heads x keys
+          if constexpr (kTwo) {
+            const float2 r = unpack2<M>(w);
+            pl[n][k] = transpose8x8(pack2<M>(x - r.x, y - r.y));
+          }
         }
 
       // values: rows = d's, columns = heads
 #pragma unroll
       for (int k2 = 0; k2 < KT / 16; ++k2) {
-        const uint32_t rowp = vb + (k2 * 16 + frow) * X::RB;
 #pragma unroll
-        for (int j = 0; j < D / 16; j += F8 ? 2 : 1) {
+        for (int j = 0; j < D / 16; j += kStep) {
           uint32_t v[4];
+          ldm_x4_t(v, kb + vpiece[j / kStep] + KT * X::RB + k2 * 16 * X::RB);
           if constexpr (F8) {
-            ldm_x4_t(v, rowp + (((j + fpiece) ^ fswz) << 4));
 #pragma unroll
             for (int u = 0; u < 4; ++u) v[u] = __byte_perm(v[u], 0, 0x3120);
 #pragma unroll
-            for (int u = 0; u < 2; ++u)
+            for (int u = 0; u < 2; ++u) {
+              const uint32_t a0 = f16x2_lo(v[2 * u]), a1 = f16x2_hi(v[2 * u]);
+              const uint32_t a2 = f16x2_lo(v[2 * u + 1]), a3 = f16x2_hi(v[2 * u + 1]);
 #pragma unroll
               for (int n = 0; n < NT; ++n) {
-                const uint32_t a0 = f16x2_lo(v[2 * u]), a1 = f16x2_hi(v[2 * u]);
-                const uint32_t a2 = f16x2_lo(v[2 * u + 1]), a3 = f16x2_hi(v[2 * u + 1]);
                 mma16816<M>(o[n][j + u], a0, a1, a2, a3, ph[n][2 * k2], ph[n][2 * k2 + 1]);
-                mma16816<M>(o[n][j + u], a0, a1, a2, a3, pl[n][2 * k2], pl[n][2 * k2 + 1]);
+                if constexpr (kTwo)
+                  mma16816<M>(o[n][j + u], a0, a1, a2, a3, pl[n][2 * k2], pl[n][2 * k2 + 1]);
               }
+            }
           } else {
-            ldm_x4_t(v, rowp + (((2 * j + fpiece) ^ fswz) << 4));
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
               mma16816<M>(o[n][j], v[0], v[1], v[2], v[3], ph[n][2 * k2], ph[n][2 * k2 + 1]);
@@ -731,23 +767,25 @@ __global__ void __launch_bounds__(Shape<C, D, NT>::W * 32, 1)
       const bool ends = st.flags & 4, last = st.flags & 8;
       if (ends || last) {  // the end of this warp's part of the item
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          l[n] += __shfl_xor_sync(~0u, l[n], 1);
-          l[n] += __shfl_xor_sync(~0u, l[n], 2);
-        }
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) l[n][h] += __shfl_xor_sync(~0u, l[n][h], x);
         if (began && ends) {
           T* out = (T*)a.out + st.r * a.o_t + head0 * a.o_h;
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            const float inv = l[n] == 0.0f ? 0.0f : a.v_scale / l[n];
-            const float i0 = __shfl_sync(~0u, inv, 8 * t4), i1 = __shfl_sync(~0u, inv, 8 * t4 + 4);
+            const float i0 = l[n][0] == 0.0f ? 0.0f : a.v_scale / l[n][0];
+            const float i1 = l[n][1] == 0.0f ? 0.0f : a.v_scale / l[n][1];
 #pragma unroll
             for (int j = 0; j < D / 16; ++j)
               store_fragment<T, C>(out, a.o_h, heads, n, j, lane,
                                    make_float4(o[n][j][0] * i0, o[n][j][1] * i1, o[n][j][2] * i0,
                                                o[n][j][3] * i1));
-            if (a.lse && t4 == 0 && g + 8 * n < heads)
-              a.lse[(int64_t)st.r * a.Hq + head0 + g + 8 * n] = lse_of<T, C>(m[n], l[n]);
+            if (a.lse && g < 2 && 8 * n + 2 * t4 + g < heads)
+              a.lse[(int64_t)st.r * a.Hq + head0 + 8 * n + 2 * t4 + g] =
+                  g ? lse_of<T, C>(m[n][1], l[n][1]) : lse_of<T, C>(m[n][0], l[n][0]);
           }
         } else {
           // a part: the first of several is put aside in the workspace, the last one in this
@@ -763,9 +801,11 @@ __global__ void __launch_bounds__(Shape<C, D, NT>::W * 32, 1)
             for (int j = 0; j < D / 16; ++j)
               reinterpret_cast<float4*>(to)[(n * (D / 16) + j) * 32 + lane] =
                   make_float4(o[n][j][0], o[n][j][1], o[n][j][2], o[n][j][3]);
-            if (t4 == 0) {
-              to[NT * 8 * D + g + 8 * n] = m[n];
-              to[NT * 8 * (D + 1) + g + 8 * n] = l[n];
+            if (g == 0) {
+              *reinterpret_cast<float2*>(to + NT * 8 * D + 8 * n + 2 * t4) =
+                  make_float2(m[n][0], m[n][1]);
+              *reinterpret_cast<float2*>(to + NT * 8 * (D + 1) + 8 * n + 2 * t4) =
+                  make_float2(l[n][0], l[n][1]);
             }
           }
           if (lane == 0) {

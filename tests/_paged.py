@@ -120,7 +120,7 @@ def attention(q, k, v, scale):
     return out, lse, mag, size.amax(-1)
 
 
-def attention_bound(ref, lse, mag, size, n, D, dtype, vmax):
+def attention_bound(ref, lse, mag, size, n, D, dtype, vmax, cache=None):
     """(bound of out, bound of lse).
 
     Scores: D exact products summed in f32, off by at most D 2^-23 of the sum of
@@ -128,11 +128,15 @@ def attention_bound(ref, lse, mag, size, n, D, dtype, vmax):
     per step), then scaled (2^-23).  The exponential: 2 ulp and its argument's
     rounding, 2^-24 of a score's distance to the maximum (at most 2 size).
     Weights enter the second product as two pieces of the 16-bit type: 2^-17
-    left over (bf16), or 2^-25 of the largest (f16, a subnormal weight).  Sums
+    left over (bf16), or 2^-25 of the largest (f16, a subnormal weight).  With
+    a bf16 output over an 8-bit cache they are one f16 piece, rounded to at
+    most half a step: eps / 2 = 2^-11 of each weight.  Sums
     of n weights and values in f32: n 2^-23.  Each is relative to
     sum_j p_j |v_j|; the result is divided and rounded once."""
     ds = (D + 4) * 2.0 ** -23 * size
-    rel = torch.as_tensor(2 * ds + 2.0 ** -21 + 2.0 ** -17 + n * 2.0 ** -23)
+    piece = 2.0 ** -11 if dtype == torch.bfloat16 and cache == torch.float8_e4m3fn else 2.0 ** -17
+    rel = torch.as_tensor(2 * ds + 2.0 ** -21 + piece + n * 2.0 ** -23)
     b = rel[:, None] * mag + n * 2.0 ** -25 * vmax / max(1, n) + \
         torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
-    return half_step(dtype) * (ref.abs() + b) + b, rel + lse.abs() * 2.0 ** -22
+    return half_step(dtype) * (ref.abs() + b) + b, \
+        rel - piece + lse.abs() * 2.0 ** -22

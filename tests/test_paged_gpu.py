@@ -372,7 +372,7 @@ def check_attention(rb, lens, Hq, Hkv, D, bs, dtype, cache, layout="tokens", win
                 ((kf.double(), sc[0]), (vf.double(), sc[1])))
         o, l, mag, size = ref.attention(q[r], k, v, s)
         vmax = float(v.abs().max()) if len(j) else 0.0
-        b, bl = ref.attention_bound(o, l, mag, size, len(j), D, DT[dtype], vmax)
+        b, bl = ref.attention_bound(o, l, mag, size, len(j), D, DT[dtype], vmax, DT[cache])
         if len(j) == 0:
             assert not bool(out[r].any())
             assert not want_lse or bool((lse[r] == -math.inf).all())
@@ -617,5 +617,6 @@ def test_serving_steps(rb, dtype, cache):
             assert bool(((kk[h[-1]] - kw).abs() <= fi.eps / 2 * 1.01 * kw.abs() +
                          scales[0] * fi.smallest_normal * fi.eps + 2e-6).all())
             o, l, mag, size = ref.attention(qd[r].cpu(), kk[h], vv[h], D ** -0.5)
-            b = ref.attention_bound(o, l, mag, size, len(h), D, dt, float(vv[h].abs().max()))[0]
+            b = ref.attention_bound(o, l, mag, size, len(h), D, dt, float(vv[h].abs().max()),
+                                    DT[cache])[0]
             close(out[r], o, b, f"request {r}")
