@@ -199,7 +199,7 @@ int remora_b200_attention_fwd_bf16(const void* q, const void* k, const void* v, 
 /* Block tables, slots and positions of one step, from the requests' lengths.
  * Request r (r < R <= 8192) holds lens[r] tokens in the first
  * ceil(lens[r] / block_size) blocks of block_table[r * ld_table ...]
- * (max_blocks entries); free_blocks (num_blocks entries) is a stack of the
+ * (max_blocks entries; a block belongs to one request); free_blocks (num_blocks entries) is a stack of the
  * *free_count free block ids.  new_tokens[r] >= 0 appends that many tokens,
  * REMORA_B200_KV_RELEASE gives the request's blocks back (its table row is
  * left as it is, its length becomes 0).  Released blocks are pushed first, in
@@ -242,7 +242,8 @@ int remora_b200_kv_block_table(const remora_b200_kv_block_table_args* args, void
  * x_h (elements; out may be x).  positions: n_axes rows of B * S int32 on the
  * device.  freq (rot / 2 doubles) and axis_of (rot / 2 ints, NULL = all 0)
  * are HOST arrays, read before the call returns.  rot even, <= min(D, 256);
- * D <= 512; n_axes <= 8.  Angles are exact to 2^-25 of a quarter turn at
+ * D <= 512 (above 256, sizes, strides and bases in whole 4 elements); n_axes
+ * <= 8.  Angles are exact to 2^-25 of a quarter turn at
  * every 32-bit position.  Any strides (of tokens and heads below 2^31
  * elements), at most 2^30 tokens; sizes, strides and bases that are multiples
  * of 8 elements (and 16 bytes) move 8 pairs at a time. */

@@ -373,15 +373,19 @@ __device__ __forceinline__ void store_fragment(T* out, int64_t o_h, int heads, i
   }
 }
 
-// The weights 2^(s - m) are kept times 2^kLift: with f16 pieces 2^14, so that weights down to
-// 2^-38 of the largest are seen (131072 keys of 2^-24 each may outweigh it); l and the products
-// carry the same factor, so only the logarithm takes it off.
+// The exponent that a softmax's weights 2^(s - m) count from, for a largest score `top`.  For bf16
+// pieces top itself.  For f16 pieces 14 below it, so that weights lie below 2^15 and those down to
+// 2^-38 of the largest are seen (131072 keys of 2^-24 each may outweigh it); sums, products and
+// their joins all count from the same m, so nothing takes the factor off.  Scores that large that
+// 14 is lost in their rounding keep m = top.
 template <typename T, typename C>
-constexpr float kLift = sizeof(C) == 1 || std::is_same<T, __half>::value ? 14.0f : 0.0f;
+__device__ __forceinline__ float exponent_of(float top) {
+  constexpr bool kF16 = sizeof(C) == 1 || std::is_same<T, __half>::value;
+  return kF16 && fabsf(top) < 8388608.0f ? top - 14.0f : top;
+}
 
-template <typename T, typename C>
 __device__ __forceinline__ float lse_of(float m, float l) {
-  return l == 0.0f ? -INFINITY : (m - kLift<T, C> + log2f(l)) * 0.6931471805599453f;
+  return l == 0.0f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
 }
 // 2^(m - top), where top may be -inf (then so is m: nothing was seen).
 __device__ __forceinline__ float weight(float m, float top) {
@@ -689,12 +693,11 @@ __global__ void __launch_bounds__(Shape<C, D, NT>::W * 32, 1)
 #pragma unroll
           for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, x));
           // sc > 0: the largest score is that of the largest product
-          top = fmaxf(m[n][h], top * sc[n][h]);
-          base[n][h] = top == -INFINITY ? 0.0f : top;
+          const float now = fmaxf(m[n][h], exponent_of<T, C>(__fmul_rn(top, sc[n][h])));
+          base[n][h] = now == -INFINITY ? 0.0f : now;
           c[n][h] = exp2_ftz(m[n][h] - base[n][h]);
-          base[n][h] -= kLift<T, C>;
-          grew |= top > m[n][h];
-          m[n][h] = top;
+          grew |= now > m[n][h];
+          m[n][h] = now;
         }
       if (__any_sync(~0u, grew)) {  // a maximum rose: what was summed shrinks
 #pragma unroll
@@ -721,8 +724,10 @@ __global__ void __launch_bounds__(Shape<C, D, NT>::W * 32, 1)
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
           const float* p = &s[k / 2][n][k % 2 * 2];
-          const float x = exp2_ftz(fmaf(p[0], sc[n][0], -base[n][0]));
-          const float y = exp2_ftz(fmaf(p[1], sc[n][1], -base[n][1]));
+          // rounded as the largest was: fused, scores of 2^24 and more would be off it by their
+          // rounding, and their weights by any factor
+          const float x = exp2_ftz(__fsub_rn(__fmul_rn(p[0], sc[n][0]), base[n][0]));
+          const float y = exp2_ftz(__fsub_rn(__fmul_rn(p[1], sc[n][1]), base[n][1]));
           l[n][0] += x;
           l[n][1] += y;
           const uint32_t w = pack2<M>(x, y);
@@ -785,7 +790,7 @@ __global__ void __launch_bounds__(Shape<C, D, NT>::W * 32, 1)
                                                o[n][j][3] * i1));
             if (a.lse && g < 2 && 8 * n + 2 * t4 + g < heads)
               a.lse[(int64_t)st.r * a.Hq + head0 + 8 * n + 2 * t4 + g] =
-                  g ? lse_of<T, C>(m[n][1], l[n][1]) : lse_of<T, C>(m[n][0], l[n][0]);
+                  g ? lse_of(m[n][1], l[n][1]) : lse_of(m[n][0], l[n][0]);
           }
         } else {
           // a part: the first of several is put aside in the workspace, the last one in this
@@ -909,8 +914,8 @@ __global__ void __launch_bounds__(Shape<C, D, NT>::W * 32, 1)
         store_fragment<T, C>((T*)a.out + r * a.o_t + head0 * a.o_h, a.o_h, heads, n, j, lane,
                              make_float4(c.x * i0, c.y * i1, c.z * i0, c.w * i1));
         if (a.lse && j == 0 && g == 0) {
-          if (hh < heads) a.lse[(int64_t)r * a.Hq + head0 + hh] = lse_of<T, C>(m0, l0);
-          if (hh + 1 < heads) a.lse[(int64_t)r * a.Hq + head0 + hh + 1] = lse_of<T, C>(m1, l1);
+          if (hh < heads) a.lse[(int64_t)r * a.Hq + head0 + hh] = lse_of(m0, l0);
+          if (hh + 1 < heads) a.lse[(int64_t)r * a.Hq + head0 + hh + 1] = lse_of(m1, l1);
         }
       } else {
         reinterpret_cast<float4*>(to)[f * 32 + lane] = c;
@@ -922,7 +927,8 @@ __global__ void __launch_bounds__(Shape<C, D, NT>::W * 32, 1)
     }
     if (has0 && !has1) {
       cross.item = item;
-      cross.last = (int)(p_end[tail >> 1] / (W * quota));
+      // (no further than the last CTA, should the lengths change under the call)
+      cross.last = (int)min(p_end[tail >> 1] / (W * quota), (int64_t)gridDim.x - 1);
     }
   }
   if (threadIdx.x == 0) room.about[blockIdx.x] = cross;
@@ -995,8 +1001,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32)
   store_fragment<T, C>((T*)a.out + r * a.o_t + head0 * a.o_h, a.o_h, heads, n, j, lane,
                        make_float4(c.x * i0, c.y * i1, c.z * i0, c.w * i1));
   if (a.lse && j == 0 && (lane >> 2) == 0) {
-    if (hh < heads) a.lse[(int64_t)r * a.Hq + head0 + hh] = lse_of<T, C>(m0, l0);
-    if (hh + 1 < heads) a.lse[(int64_t)r * a.Hq + head0 + hh + 1] = lse_of<T, C>(m1, l1);
+    if (hh < heads) a.lse[(int64_t)r * a.Hq + head0 + hh] = lse_of(m0, l0);
+    if (hh + 1 < heads) a.lse[(int64_t)r * a.Hq + head0 + hh + 1] = lse_of(m1, l1);
   }
 }
 
@@ -1107,6 +1113,7 @@ extern "C" int remora_b200_paged_attention(const remora_b200_paged_attention_arg
   if (R == 0) return REMORA_B200_OK;
   RB_CHECK_ARG(p.q && p.k_cache && p.v_cache && p.block_table && p.lens && p.out,
                "paged_attention: null pointer");
+  RB_CHECK_ARG(p.q != p.out, "paged_attention: out must not be q");
   RB_CHECK_ARG(aligned16(p.q) && aligned16(p.k_cache) && aligned16(p.v_cache) && aligned16(p.out),
                "paged_attention: q, the caches and out must be 16-byte aligned");
   const int64_t ce = p.cache_dtype == REMORA_B200_E4M3 ? 16 : 8;

@@ -377,7 +377,10 @@ template <typename T, typename C, bool kAppend>
 int launch(Args& a, int v, int interleaved, cudaStream_t st) {
   a.rot_units = a.half / v;
   a.units = (a.D / v + 1) / 2;  // = rot_units + ceil of half the rest
-  a.pass = kThreads / a.units;  // D <= 512: at least one
+  RB_CHECK_ARG(a.units <= kThreads,
+               "rope: head_dim above %d needs sizes, strides and bases of whole 4 elements",
+               2 * kThreads);
+  a.pass = kThreads / a.units;
   const int heads = a.q.H + (kAppend ? a.k.H + a.v.H : 0);
   a.heads = Divisor((uint32_t)heads);
   // as many tokens as fill passes of kUnits heads a thread best (the fewest of those), within

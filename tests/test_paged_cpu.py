@@ -62,7 +62,7 @@ def rope(L, **c):
     dict(D=0), dict(D=2048), dict(pos=None), dict(ld=3, axes=2), dict(axes=0), dict(axes=9),
     dict(freq=None), dict(ax=AXES), dict(rot=3), dict(rot=130), dict(rot=258, D=512),
     dict(x=A + 1), dict(freq=NAN), dict(freq=INF), dict(xs=2 ** 31),
-    dict(oh=-2 ** 31), dict(S=2 ** 30 + 1, ld=2 ** 31), dict(B=2 ** 20, S=2 ** 20, ld=2 ** 41)])
+    dict(oh=-2 ** 31), dict(D=300, xs=601), dict(D=512, rot=2), dict(S=2 ** 30 + 1, ld=2 ** 31), dict(B=2 ** 20, S=2 ** 20, ld=2 ** 41)])
 def test_rope_refuses(L, bad):
     assert rope(L, **bad) == rb.ERR_INVALID and "rope" in rb.last_error()
 
@@ -93,7 +93,7 @@ def test_append_refuses(L, bad):
 
 
 def attention(L, **c):
-    d = dict(q=A, kc=A, vc=A, table=A, lens=A, out=A, lse=None, ws=A, wsb=1 << 40, R=2, Hq=8, Hkv=2,
+    d = dict(q=A, kc=A, vc=A, table=A, lens=A, out=2 * A, lse=None, ws=A, wsb=1 << 40, R=2, Hq=8, Hkv=2,
              D=128, qt=1024, qh=128, ot=1024, oh=128, nb=8, bs=16, kb=4096, kt=256, kh=128, vb=4096,
              vt=256, vh=128, ld=8, mb=8, window=0, scale=1.0, ks=1.0, vs=1.0, dt=rb.BF16,
              cdt=rb.BF16)
@@ -103,7 +103,7 @@ def attention(L, **c):
 
 @pytest.mark.parametrize("bad", [
     dict(q=None), dict(kc=None), dict(vc=None), dict(table=None), dict(lens=None), dict(out=None),
-    dict(q=ODD), dict(kc=ODD), dict(vc=ODD), dict(out=ODD), dict(ws=ODD), dict(ws=None),
+    dict(out=A), dict(q=ODD), dict(kc=ODD), dict(vc=ODD), dict(out=ODD), dict(ws=ODD), dict(ws=None),
     dict(wsb=0), dict(dt=rb.F32), dict(cdt=rb.F16), dict(R=-1), dict(R=8193), dict(Hq=7),
     dict(Hkv=0), dict(Hq=0), dict(D=96), dict(nb=0), dict(bs=0), dict(nb=2 ** 28), dict(mb=0),
     dict(ld=7), dict(mb=2 ** 28, ld=2 ** 28), dict(scale=float("nan")), dict(scale=float("inf")),

@@ -160,7 +160,7 @@ def close(got, want, bound, what=""):
 @pytest.mark.parametrize("inter", [False, True])
 @pytest.mark.parametrize("B,S,H,D,rot,axes", [
     (1, 1, 1, 64, 64, 1), (2, 37, 3, 128, 128, 3), (1, 130, 5, 80, 80, 2), (3, 11, 2, 72, 72, 2),
-    (2, 9, 4, 96, 32, 1), (1, 5, 2, 40, 6, 3), (2, 3, 1, 7, 2, 1), (1, 4, 2, 256, 256, 4),
+    (2, 9, 4, 96, 32, 1), (1, 5, 2, 40, 6, 3), (2, 3, 1, 7, 2, 1), (1, 4, 2, 256, 256, 4), (1, 5, 3, 512, 256, 2), (2, 4, 2, 255, 100, 2),
     (1, 3, 2, 64, 0, 1), (1, 300, 48, 128, 64, 1)])
 def test_rope_against_64_bits(rb, dtype, inter, B, S, H, D, rot, axes):
     g = gen(B * S + H)
@@ -480,6 +480,91 @@ def test_attention_reports_bad_pages_and_lengths(rb):
             rb.synchronize_and_check()
         assert torch.equal(got, rb.paged_attention(q, kc, vc, i32([[1, 3]]), i32([same])))
     rb.synchronize_and_check()
+
+
+@pytest.mark.parametrize("dtype,cache", TYPES)
+@pytest.mark.parametrize("size", [3e2, 3e4])
+def test_attention_huge_scores(rb, dtype, cache, size):
+    """Scores of 1e5 to 1e10, where their own rounding exceeds a factor of two of a weight: the
+    result stays a mean of the values, and where one key leads by far it is that key's value."""
+    D, n = 128, 70
+    g = gen(3)
+    k = torch.randn(n, 1, D, generator=g).sign() * (size if cache != "e4m3" else 448.0)
+    v = torch.randn(n, 1, D, generator=g)
+    q = torch.randn(1, 2, D, generator=g).sign() * size
+    q[0, 1] = k[17, 0] / k[17, 0].abs() * size  # head 1 is key 17's own direction
+    kc, vc = torch.zeros(5, 16, 1, D).to(DT[cache]), torch.zeros(5, 16, 1, D).to(DT[cache])
+    kc.view(80, 1, D)[:n], vc.view(80, 1, D)[:n] = k.to(DT[cache]), v.to(DT[cache])
+    out = rb.paged_attention(q.to(DT[dtype]).cuda(), kc.cuda(), vc.cuda(), i32([[0, 1, 2, 3, 4]]),
+                             i32([n]), scale=1.0)
+    vs = vc.view(80, D)[:n].float()
+    assert bool(out.isfinite().all()) and float(out.float().abs().max()) <= float(vs.abs().max())
+    assert torch.equal(out[0, 1].float().cpu(), vs[17].to(DT[dtype]).float())
+
+
+def test_attention_most_requests(rb):
+    """8192 requests, every other one empty, lengths of 0 to 3."""
+    R, D, bs = 8192, 64, 4
+    g = gen(2)
+    lens = torch.arange(R) % 4
+    kc = torch.randn(R, bs, 2, D, generator=g).to(torch.bfloat16).cuda()
+    vc = torch.randn(R, bs, 2, D, generator=g).to(torch.bfloat16).cuda()
+    q = torch.randn(R, 4, D, generator=g).to(torch.bfloat16).cuda()
+    out = rb.paged_attention(q, kc, vc, i32(np.arange(R))[:, None], i32(lens))
+    j = torch.arange(bs, device="cuda")
+    s = torch.einsum("rgd,rjgd->rgj", q.double().view(R, 2, 2, D).flatten(1, 2),
+                     kc.double().repeat_interleave(2, 2)) / 8
+    s = s.masked_fill(j >= lens.cuda()[:, None, None], -math.inf)
+    want = torch.einsum("rgj,rjgd->rgd", torch.softmax(s, -1).nan_to_num(0.0),
+                        vc.double().repeat_interleave(2, 2))
+    # half a step of bf16, and below it what four weights' roundings leave (2^-17 each) with room
+    assert bool(((out.double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -12).all())
+    assert not bool(out[::4].any())
+    rb.synchronize_and_check()
+
+
+def test_attention_window_over_freed_pages(rb):
+    """Table entries wholly in front of the window may be anything."""
+    out, args, kw = check_attention(rb, [100, 33, 64], 4, 2, 64, 16, "bf16", "bf16", window=20)
+    table = args[3].clone()
+    table[0, :5] = -1       # keys 80 on count
+    table[2, :2] = 1 << 30  # keys 44 on
+    got = rb.paged_attention(*args[:3], table, args[4], **kw)
+    assert torch.equal(got, out)
+    rb.synchronize_and_check()
+
+
+def test_attention_table_and_cache_strides(rb):
+    """A table that is a slice of a wider one; keys heads first, values tokens first."""
+    out, args, kw = check_attention(rb, [70, 300, 5], 8, 2, 128, 16, "f16", "f16")
+    q, kc, vc, table, lens = args
+    wide = torch.full((3, table.shape[1] + 5), -3, dtype=torch.int32, device="cuda")
+    wide[:, :table.shape[1]] = table
+    kh = kc.transpose(1, 2).contiguous().transpose(1, 2)
+    assert kh.stride() != vc.stride()
+    assert torch.equal(rb.paged_attention(q, kh, vc, wide[:, :table.shape[1]], lens, **kw), out)
+    rb.synchronize_and_check()
+
+
+def test_attention_in_a_graph_behind_copies(rb):
+    """Captured right behind a copy of its lengths and a fill of its output, each replay sees the
+    new lengths (the launch may be set up before the copy is done, but must wait for it)."""
+    out, args, kw = check_attention(rb, [900, 20, 7], 8, 2, 128, 16, "bf16", "bf16")
+    q, kc, vc, table, lens = args
+    room, src = torch.empty_like(out), lens.clone()
+    now = torch.zeros_like(lens)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        room.fill_(9)
+        now.copy_(src)
+        rb.paged_attention(q, kc, vc, table, now, out=room, **kw)
+        again = room.clone()
+    for new in ([900, 20, 7], [0, 20, 3], [899, 1, 0], [900, 20, 7]):
+        src.copy_(i32(new))
+        want = rb.paged_attention(q, kc, vc, table, src, **kw)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(again, want) and torch.equal(room, want)
 
 
 def test_attention_strided_q_and_out(rb):
