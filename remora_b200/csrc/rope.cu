@@ -19,7 +19,16 @@
 // Bound: HBM (each element read once and written once).  A block takes a few
 // tokens at a time, puts their cosines and sines into shared memory (one
 // sincos per pair and token, whatever the number of heads), and then moves
-// whole heads in vectors of up to 8 pairs.
+// whole heads in vectors of up to 8 pairs, the loads issued before the angles.
+//
+// B200, device time: 268.6 MB of bf16 [4,4096,32,128] (heads first, three
+// axes) 46.8 us = 5.74 TB/s, where a copy of the same bytes takes 42.6; 8192
+// tokens of 32 + 2 x 8 heads into an e4m3 cache (184.7 MB) 37.2 us = 4.96
+// TB/s.  What it took: a thread keeping its unit of the head and walking over
+// heads (65 -> 51 us with the angles read without bank conflicts), then one
+// multiply-add per stride and paired conversions (-> 47).  Blocks of 128
+// threads, 64 registers, 8 to an SM: 256 threads 50, more blocks (spills) 56
+// to 61, 3 or 4 units a thread 59 and 51.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>

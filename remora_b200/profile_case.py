@@ -2,7 +2,8 @@
 
     python -m remora_b200.profile_case <case> [--reps N] [--warmup W] [shape options]
 
-Cases: router, dispatch, gather, scatter, combine, swiglu, down, attention, gemm, layer, hetero.
+Cases: router, dispatch, gather, scatter, combine, swiglu, down, attention, gemm, layer, hetero,
+and of decoding: tables, rope, append, paged (R requests of S keys, H heads, --kv-heads, --dim).
 Each run fills its inputs with the seeded generator, launches the kernel
 `warmup` times, then `reps` times between CUDA events on the current
 stream, and prints one line: case, shape, time per launch, and the
@@ -115,7 +116,44 @@ def build_case(a):
         return (lambda: rb.moe_hetero_layer(x, wr, wg, wu, wd, k, out=out),
                 f"heterogeneous MoE layer T={T} D={D} F={Fs} top-{k}",
                 6.0 * T * k * D * sum(Fs) / len(Fs), "FLOP")
+    if a.case in ("tables", "rope", "append", "paged"):
+        return _decoding_case(a)
     raise SystemExit(f"unknown case {a.case}")
+
+
+def _decoding_case(a):
+    """A step of R requests that hold S tokens each, in blocks of 16."""
+    R, S, H, KV, D, bs = a.R, a.S, a.H, a.kv_heads, a.dim, 16
+    dev = dict(dtype=torch.int32, device="cuda")
+    mb = -(-(S + 1) // bs)
+    nb = R * mb + 1
+    lens, new = torch.full((R,), S, **dev), torch.ones(R, **dev)
+    table = torch.randperm(nb - 1, device="cuda").to(torch.int32).view(R, mb)
+    free, count = torch.full((nb,), nb - 1, **dev), torch.full((1,), nb, **dev)
+    if a.case == "tables":
+        return (lambda: rb.kv_block_table(lens, new, table, free, count, bs, R),
+                f"block tables R={R} S={S}", 32.0 * R, "B")
+    freq = 10000.0 ** (-2.0 * torch.arange(D // 2, dtype=torch.float64) / D)
+    if a.case == "rope":
+        x, pos = _bf16((a.B, S, H, D), 50), torch.arange(S, **dev).repeat(a.B, 1)
+        out = torch.empty_like(x)
+        return (lambda: rb.rope(x, pos, freq, out=out), f"rope [{a.B},{S},{H},{D}]",
+                4.0 * x.numel(), "B")
+    kc, vc = _bf16((nb, bs, KV, D), 51), _bf16((nb, bs, KV, D), 52)
+    if a.case == "append":
+        T = R * S
+        q, k, v = _bf16((T, H, D), 53), _bf16((T, KV, D), 54), _bf16((T, KV, D), 55)
+        pos = torch.arange(S, **dev).repeat(R)
+        slots = torch.randperm(nb * bs, device="cuda")[:T].to(torch.int32)
+        out = torch.empty_like(q)
+        return (lambda: rb.rope_kv_append(q, k, v, pos, slots, freq, kc, vc, q_out=out),
+                f"append {T} tokens, {H} + 2 x {KV} heads of {D}", 4.0 * T * (H + 2 * KV) * D, "B")
+    q = _bf16((R, H, D), 53)
+    out = torch.empty_like(q)
+    ws = torch.empty(rb.paged_attention_workspace_bytes(R, H, KV, D), dtype=torch.uint8,
+                     device="cuda")
+    return (lambda: rb.paged_attention(q, kc, vc, table, lens, out=out, workspace=ws),
+            f"paged attention R={R} S={S} heads {H}/{KV} x {D}", 4.0 * R * S * KV * D, "B")
 
 
 def main(argv=None):
@@ -132,6 +170,9 @@ def main(argv=None):
     ap.add_argument("--H", type=int, default=32)
     ap.add_argument("--S", type=int, default=4096)
     ap.add_argument("--n", type=int, default=8192)
+    ap.add_argument("--R", type=int, default=64)
+    ap.add_argument("--kv-heads", type=int, default=8)
+    ap.add_argument("--dim", type=int, default=128)
     a = ap.parse_args(argv)
     from remora_b200 import build
 
