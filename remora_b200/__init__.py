@@ -14,7 +14,6 @@ dispatcher that replaces its body.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import functools
 import os
@@ -164,12 +163,6 @@ def _stream(t: torch.Tensor) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
 
 
-def _raw_stream(device_index: int) -> int:
-    """torch's current stream on a device as its cudaStream_t (without the Stream object that
-    torch.cuda.current_stream makes: 1 us against 4 on the latency-bound calls)."""
-    return torch._C._cuda_getCurrentRawStream(device_index)
-
-
 def _dev(*ts: torch.Tensor) -> None:
     for t in ts:
         if not t.is_cuda:
@@ -315,27 +308,33 @@ _ROPE_ARGS = struct.Struct("=5Q12q4i")
 _APPEND_ARGS = struct.Struct("=10Q22q2f4i")
 _ATTENTION_ARGS = struct.Struct("=9Q19q3f2i4x")
 
-_HERE_ALREADY = contextlib.nullcontext()
+_INT32 = torch.int32
 
 
-def _on(*ts: torch.Tensor):
-    """Checks that all tensors are on one CUDA device.  Returns a context manager that makes it
-    current for the launch (nothing to do where it is current already) and its index."""
-    dev = ts[0].device
-    if dev.type != "cuda":
-        raise ValueError("remora_b200 operates on CUDA tensors only (no CPU fallback)")
+def _on(*ts: torch.Tensor) -> int:
+    """The index of the CUDA device that all tensors are on."""
+    index = ts[0].get_device()
     for t in ts:
-        if t.device != dev:
-            if not t.is_cuda:
+        if t.get_device() != index or index < 0:
+            if not (t.is_cuda and ts[0].is_cuda):
                 raise ValueError("remora_b200 operates on CUDA tensors only (no CPU fallback)")
-            raise ValueError(f"tensors are on different devices: {dev} and {t.device}")
-    if dev.index == torch._C._cuda_getDevice():
-        return _HERE_ALREADY, dev.index
-    return torch.cuda.device(dev), dev.index
+            raise ValueError(f"tensors are on different devices: {ts[0].device} and {t.device}")
+    return index
+
+
+def _launch(fn, args: bytes, index: int) -> None:
+    """Calls an entry point on torch's current stream of a device, made current for the call."""
+    if index == torch._C._cuda_getDevice():
+        rc = fn(args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(args, torch._C._cuda_getCurrentRawStream(index))
+    if rc != OK:
+        raise RemoraError(rc, last_error())
 
 
 def _ints(name: str, t: torch.Tensor, shape: tuple) -> None:
-    if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous():
+    if t.dtype is not _INT32 or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 tensor of shape {list(shape)}, got "
                          f"{t.dtype} {list(t.shape)}")
 
@@ -383,7 +382,7 @@ def kv_block_table(lens: torch.Tensor, new_tokens: torch.Tensor, block_table: to
         raise ValueError("block_table must be int32 with adjacent entries of a row")
     if N < 0:
         raise ValueError("max_tokens must not be negative")
-    guard, index = _on(lens, new_tokens, block_table, free_blocks, free_count)
+    index = _on(lens, new_tokens, block_table, free_blocks, free_count)
     if out is None:  # one allocation, cut up; the tokens' rows first, each 16-byte aligned
         pad = -N % 4
         sizes = (N, pad, N, pad, N, pad, R, 1, R + 1, R) if pad else (N, N, N, R, 1, R + 1, R)
@@ -395,12 +394,10 @@ def kv_block_table(lens: torch.Tensor, new_tokens: torch.Tensor, block_table: to
         for name, n in zip(KvStep._fields, (R, 1, R + 1, N, N, N, R)):
             _ints(name, getattr(out, name), (n,))
         _on(lens, *out)
-    with guard:
-        _check(lib().remora_b200_kv_block_table(_BLOCK_TABLE_ARGS.pack(
-            lens.data_ptr(), new_tokens.data_ptr(), block_table.data_ptr(),
-            free_blocks.data_ptr(), free_count.data_ptr(), *[t.data_ptr() for t in out], R,
-            block_table.stride(0) if R > 1 else max_blocks, max_blocks, num_blocks, block_size, N),
-            _raw_stream(index)))
+    _launch(lib().remora_b200_kv_block_table, _BLOCK_TABLE_ARGS.pack(
+        lens.data_ptr(), new_tokens.data_ptr(), block_table.data_ptr(),
+        free_blocks.data_ptr(), free_count.data_ptr(), *[t.data_ptr() for t in out], R,
+        block_table.stride(0) if R > 1 else max_blocks, max_blocks, num_blocks, block_size, N), index)
     return out
 
 
@@ -443,7 +440,7 @@ def rope(x: torch.Tensor, positions: torch.Tensor, freq: torch.Tensor,
     if x.dtype not in (torch.bfloat16, torch.float16, torch.float32):
         raise TypeError(f"rope takes bf16, f16 or f32, got {x.dtype}")
     n_axes, freq, axis_of, positions, rot = _rope_plan(freq, axis_of, positions, x.shape[:-2])
-    guard, index = _on(x, positions, x if out is None else out)
+    index = _on(x, positions, x if out is None else out)
     if out is None:
         out = torch.empty_like(x)
     elif out.shape != x.shape or out.dtype != x.dtype:
@@ -454,29 +451,28 @@ def rope(x: torch.Tensor, positions: torch.Tensor, freq: torch.Tensor,
     xs, os_ = x.stride(), out.stride()
     if x.dim() == 3:
         xs, os_ = (0,) + xs, (0,) + os_
-    with guard:
-        _check(lib().remora_b200_rope(_ROPE_ARGS.pack(
-            x.data_ptr(), out.data_ptr(), positions.data_ptr(), freq.data_ptr(),
-            0 if axis_of is None else axis_of.data_ptr(), B, S, x.shape[-2], x.shape[-1], rot,
-            *xs[:3], *os_[:3], B * S, _DTYPES[x.dtype], n_axes, interleaved, inverse),
-            _raw_stream(index)))
+    _launch(lib().remora_b200_rope, _ROPE_ARGS.pack(
+        x.data_ptr(), out.data_ptr(), positions.data_ptr(), freq.data_ptr(),
+        0 if axis_of is None else axis_of.data_ptr(), B, S, x.shape[-2], x.shape[-1], rot,
+        *xs[:3], *os_[:3], B * S, _DTYPES[x.dtype], n_axes, interleaved, inverse), index)
     return out
 
 
 def _cache(q, k_cache, v_cache, Hkv: int, D: int) -> tuple:
     """Checks a pair of caches against q; their element type, and their blocks and strides as
     the C ABI takes them."""
-    shape = k_cache.shape
-    if len(shape) != 4 or shape != v_cache.shape or shape[2:] != (Hkv, D):
+    shape, dtype = k_cache.shape, k_cache.dtype
+    if len(shape) != 4 or v_cache.shape != shape or shape[2] != Hkv or shape[3] != D:
         raise ValueError(f"the caches must be [num_blocks, block_size, {Hkv}, {D}] of one shape, "
                          f"got {list(k_cache.shape)} and {list(v_cache.shape)}")
-    if k_cache.dtype != v_cache.dtype or k_cache.dtype not in (q.dtype, torch.float8_e4m3fn):
+    if v_cache.dtype is not dtype or (dtype is not q.dtype and
+                                      dtype is not torch.float8_e4m3fn):
         raise TypeError(f"the caches must be {q.dtype} or float8_e4m3fn, got {k_cache.dtype} and "
                         f"{v_cache.dtype}")
     ks, vs = k_cache.stride(), v_cache.stride()
     if ks[3] != 1 or vs[3] != 1:
         raise ValueError("the elements of a cache row must be adjacent")
-    return _DTYPES[k_cache.dtype], (shape[0], shape[1], *ks[:3], *vs[:3])
+    return _DTYPES[dtype], (shape[0], shape[1], *ks[:3], *vs[:3])
 
 
 def rope_kv_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
@@ -502,7 +498,7 @@ def rope_kv_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions:
     cdt, cdims = _cache(q, k_cache, v_cache, Hkv, D)
     n_axes, freq, axis_of, positions, rot = _rope_plan(freq, axis_of, positions, (T,))
     _ints("slots", slots, (T,))
-    guard, index = _on(q, k, v, positions, slots, k_cache, v_cache)
+    index = _on(q, k, v, positions, slots, k_cache, v_cache)
     if q_out is None:
         q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif q_out.shape != q.shape or q_out.dtype != q.dtype or q_out.device != q.device:
@@ -510,13 +506,12 @@ def rope_kv_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions:
     qs, ks, vs, os_ = q.stride(), k.stride(), v.stride(), q_out.stride()
     if qs[2] != 1 or ks[2] != 1 or vs[2] != 1 or os_[2] != 1:
         raise ValueError("the elements of a head must be adjacent")
-    with guard:
-        _check(lib().remora_b200_rope_kv_append(_APPEND_ARGS.pack(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), q_out.data_ptr(), k_cache.data_ptr(),
-            v_cache.data_ptr(), positions.data_ptr(), slots.data_ptr(), freq.data_ptr(),
-            0 if axis_of is None else axis_of.data_ptr(), T, Hq, Hkv, D, rot, *qs[:2], *ks[:2],
-            *vs[:2], *os_[:2], T, *cdims, k_scale, v_scale, _DTYPES[q.dtype], cdt, n_axes,
-            interleaved), _raw_stream(index)))
+    _launch(lib().remora_b200_rope_kv_append, _APPEND_ARGS.pack(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), q_out.data_ptr(), k_cache.data_ptr(),
+        v_cache.data_ptr(), positions.data_ptr(), slots.data_ptr(), freq.data_ptr(),
+        0 if axis_of is None else axis_of.data_ptr(), T, Hq, Hkv, D, rot, *qs[:2], *ks[:2],
+        *vs[:2], *os_[:2], T, *cdims, k_scale, v_scale, _DTYPES[q.dtype], cdt, n_axes,
+        interleaved), index)
     return q_out
 
 
@@ -555,7 +550,7 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     if block_table.dtype != torch.int32 or block_table.shape[0] != R or \
             (max_blocks != 1 and block_table.stride(1) != 1):
         raise ValueError("block_table must be int32 [R, max_blocks] with adjacent entries")
-    guard, index = _on(q, k_cache, v_cache, block_table, lens)
+    index = _on(q, k_cache, v_cache, block_table, lens)
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device:
@@ -571,14 +566,12 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
                                 device=q.device)
     elif workspace.device != q.device or not workspace.is_contiguous():
         raise ValueError("workspace must be a contiguous tensor on q's device")
-    with guard:
-        _check(lib().remora_b200_paged_attention(_ATTENTION_ARGS.pack(
-            q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
-            lens.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
-            workspace.data_ptr(), workspace.nbytes, R, Hq, Hkv, D, *qs[:2], *os_[:2], *cdims,
-            block_table.stride(0) if R > 1 else max_blocks, max_blocks, window,
-            D ** -0.5 if scale is None else scale, k_scale, v_scale, _DTYPES[q.dtype], cdt),
-            _raw_stream(index)))
+    _launch(lib().remora_b200_paged_attention, _ATTENTION_ARGS.pack(
+        q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
+        lens.data_ptr(), out.data_ptr(), 0 if lse is None else lse.data_ptr(),
+        workspace.data_ptr(), workspace.nbytes, R, Hq, Hkv, D, *qs[:2], *os_[:2], *cdims,
+        block_table.stride(0) if R > 1 else max_blocks, max_blocks, window,
+        D ** -0.5 if scale is None else scale, k_scale, v_scale, _DTYPES[q.dtype], cdt), index)
     return out
 
 

@@ -433,7 +433,6 @@ constexpr int kPartFloats = NT * 8 * (D + 2);
 // The CTA's share of the join: what crosses into the next CTA.
 struct Cross {
   int32_t item, last;  // an item that goes on (-1: none), and the last CTA that has a part
-  int32_t pad[2];
 };
 
 // Workspace: [workers] first parts | [CTAs][2] parts that cross CTAs | [CTAs] Cross.
@@ -920,7 +919,7 @@ __global__ void __launch_bounds__(Shape<C, D, NT>::W * 32, 1)
     }
   }
   __syncthreads();
-  Cross cross{-1, 0, {0, 0}};
+  Cross cross{-1, 0};
   for (; leads; leads &= leads - 1) {
     const int e0 = __ffs(leads) - 1;
     const uint32_t run = __shfl_sync(~0u, same, e0);

@@ -75,7 +75,7 @@ struct Args {
   int32_t tokens, S;
   Divisor batch;      // S
   int32_t num_blocks, bs;
-  int32_t D, half, n_axes;
+  int32_t D, half;
   int32_t tile;       // tokens of a block's iteration
   int32_t rot_units;  // units of V pairs in a head
   int32_t units;      // those and the units of 2V plain elements behind them
@@ -443,7 +443,6 @@ inline int angles(const char* who, Args& a, const int32_t* positions, int64_t ld
   RB_CHECK_ARG(n_axes == 1 || ld_pos >= tokens, "%s: ld_pos must be at least the tokens", who);
   a.half = (int)(rot / 2);
   a.D = (int)D;
-  a.n_axes = n_axes;
   a.pos = positions;
   a.ld_pos = ld_pos;
   a.tokens = (int32_t)tokens;
@@ -452,8 +451,8 @@ inline int angles(const char* who, Args& a, const int32_t* positions, int64_t ld
     const int ax = axis_of ? axis_of[i] : 0;
     RB_CHECK_ARG(ax >= 0 && ax < n_axes, "%s: axis_of[%d] = %d is not in [0, %d)", who, i, ax,
                  n_axes);
-    long double t = (long double)freq[i] / 6.283185307179586476925286766559L;
-    t -= floorl(t);
+    long double t = (long double)freq[i] * 0.159154943091895335768883763373L;  // / (2 pi)
+    if (!(t >= 0 && t < 1)) t -= floorl(t);
     const long double f = t * 18446744073709551616.0L;
     a.turns.f[i] = f >= 18446744073709551615.0L ? 0 : (uint64_t)f;
     a.turns.axis[i] = (uint8_t)ax;
