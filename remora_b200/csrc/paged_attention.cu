@@ -261,7 +261,8 @@ struct Walk {
     if (key < n) {  // (a key in front of the window may share its block with one that counts)
       const int32_t page = a.page.div(key);
       off = key - page * a.bs;
-      id = __ldg(a.table + (int64_t)r * a.ld_table + page);
+      // (an ordinary load: the table may be written after this kernel was set up)
+      id = a.table[(int64_t)r * a.ld_table + page];
     }
   }
   __device__ __forceinline__ void next(const Args& a, int Hg, int lane) {
@@ -426,6 +427,22 @@ __device__ __forceinline__ float weight(float m, float top) {
   return exp2_ftz(m - (top == -INFINITY ? 0.0f : top));
 }
 
+// Adds a part (its maxima and sums of two heads, and its products) to the parts so far.
+__device__ __forceinline__ void join_part(float4& c, float& m0, float& m1, float& l0, float& l1,
+                                          float2 pm, float2 pl, float4 v) {
+  const float t0 = fmaxf(m0, pm.x), t1 = fmaxf(m1, pm.y);
+  const float a0 = weight(m0, t0), a1 = weight(m1, t1);
+  const float b0 = weight(pm.x, t0), b1 = weight(pm.y, t1);
+  c.x = c.x * a0 + v.x * b0;
+  c.y = c.y * a1 + v.y * b1;
+  c.z = c.z * a0 + v.z * b0;
+  c.w = c.w * a1 + v.w * b1;
+  l0 = l0 * a0 + pl.x * b0;
+  l1 = l1 * a1 + pl.y * b1;
+  m0 = t0;
+  m1 = t1;
+}
+
 // A partial result: fragments [nt][j][lane] as float4, then m[8 NT], l[8 NT].
 template <int D, int NT>
 constexpr int kPartFloats = NT * 8 * (D + 2);
@@ -454,7 +471,6 @@ __global__ void __launch_bounds__(Shape<C, D, NT>::W * 32, 1)
   __shared__ Stage stages[W][S];
   __shared__ int32_t p_item[2 * W], p_flag[2 * W];
   __shared__ int64_t p_end[W];
-  __shared__ float p_w[2 * W][8 * NT], p_m[2 * W][8 * NT], p_l[2 * W][8 * NT];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t4 = lane & 3;
   const int gq = a.gq, ngr = (gq + 8 * NT - 1) / (8 * NT), Hg = a.Hkv * ngr;
@@ -874,73 +890,43 @@ __global__ void __launch_bounds__(Shape<C, D, NT>::W * 32, 1)
 
   // Join the CTA's own parts: entry 2w is warp w's first part, 2w + 1 its last.  Parts of one
   // item are neighbours in that order; a run that lacks the item's first or last tile crosses
-  // into another CTA.
+  // into another CTA.  The code is met once a launch and comes from memory, so it is kept short:
+  // a warp takes a fragment of a run and sums the parts as they come, each with its maximum.
   auto part = [&](int e) {
     return reinterpret_cast<const float*>(ring_all + (size_t)(e >> 1) * X::kRing) +
            (e & 1 ? 0 : PF);
   };
   static_assert(2 * W <= 32, "a lane per entry");
-  int my_item = lane < 2 * W ? p_item[lane] : -1;
-  const bool real = my_item >= 0;
-  const uint32_t reals = __ballot_sync(~0u, real), upto = reals & ((2u << lane) - 1);
-  const int known = __shfl_sync(~0u, my_item, upto ? 31 - __clz(upto) : 0);
-  if (!real && lane < 2 * W) my_item = upto ? known : -1;  // an empty entry goes with its run
-  const uint32_t same = __match_any_sync(~0u, my_item) & reals;
-  uint32_t leads = __ballot_sync(~0u, real && (same & ((1u << lane) - 1)) == 0);
-  if (leads) {  // (the same in all warps)
-#pragma unroll 1
-    for (int h = warp; h < 8 * NT; h += W) {
-      const float* p = part(min(lane, 2 * W - 1)) + NT * 8 * D + h;
-      const float pm = real ? p[0] : -INFINITY;
-      float top = pm, sum;
-#pragma unroll
-      for (int o = 1; o < 2 * W; o <<= 1) {  // up the run, then from its end
-        const float y = __shfl_up_sync(~0u, top, o);
-        const int it = __shfl_up_sync(~0u, my_item, o);
-        if (lane >= o && it == my_item) top = fmaxf(top, y);
-      }
-      const int tail = same ? 31 - __clz(same) : lane;
-      top = __shfl_sync(~0u, top, tail);
-      const float wgt = real ? weight(pm, top) : 0.0f;
-      sum = real ? wgt * p[8 * NT] : 0.0f;
-#pragma unroll
-      for (int o = 1; o < 2 * W; o <<= 1) {
-        const float y = __shfl_up_sync(~0u, sum, o);
-        const int it = __shfl_up_sync(~0u, my_item, o);
-        if (lane >= o && it == my_item) sum += y;
-      }
-      if (real) {
-        p_w[lane][h] = wgt;
-        if (lane == tail) {
-          p_m[__ffs(same) - 1][h] = top;
-          p_l[__ffs(same) - 1][h] = sum;
-        }
-      }
-    }
-  }
-  __syncthreads();
+  constexpr int kFrags = NT * (D / 16);
+  const int entry = lane < 2 * W ? p_item[lane] : -1;
   Cross cross{-1, 0};
-  for (; leads; leads &= leads - 1) {
-    const int e0 = __ffs(leads) - 1;
-    const uint32_t run = __shfl_sync(~0u, same, e0);
-    const int tail = 31 - __clz(run), item = p_item[e0];
+  int turn = 0;  // fragments so far, of all runs
+  for (uint32_t todo = __ballot_sync(~0u, entry >= 0); todo; turn += kFrags) {
+    const int e0 = __ffs(todo) - 1, item = __shfl_sync(~0u, entry, e0);
+    const uint32_t run = __ballot_sync(~0u, entry == item);
+    todo &= ~run;
+    const int tail = 31 - __clz(run);
     const bool has0 = p_flag[e0] & 1, has1 = p_flag[tail] & 2;
-    const int r = item / Hg, h = item - r * Hg, sub = h % ngr, head0 = h / ngr * gq + sub * 8 * NT;
-    const int heads = min(8 * NT, gq - sub * 8 * NT);
-    float* to = room.cross + ((int64_t)blockIdx.x * 2 + (has0 ? 1 : 0)) * PF;
-    for (int f = warp; f < NT * (D / 16); f += W) {
+    if (has0 && !has1) {
+      cross.item = item;
+      // (no further than the last CTA, should the lengths change under the call)
+      cross.last = (int)min(p_end[tail >> 1] / (W * quota), (int64_t)gridDim.x - 1);
+    }
+#pragma unroll 1
+    for (int f = (warp + W * 32 - turn % W) % W; f < kFrags; f += W) {
       const int n = f / (D / 16), j = f % (D / 16), hh = n * 8 + 2 * t4;
       float4 c = make_float4(0, 0, 0, 0);
+      float m0 = -INFINITY, m1 = -INFINITY, l0 = 0, l1 = 0;
+#pragma unroll 1
       for (uint32_t b = run; b; b &= b - 1) {
-        const int e = __ffs(b) - 1;
-        const float2 w = *reinterpret_cast<const float2*>(&p_w[e][hh]);
-        const float4 v = reinterpret_cast<const float4*>(part(e))[f * 32 + lane];
-        c.x += w.x * v.x;
-        c.y += w.y * v.y;
-        c.z += w.x * v.z;
-        c.w += w.y * v.w;
+        const float* p = part(__ffs(b) - 1);
+        const float2 pm = *reinterpret_cast<const float2*>(p + NT * 8 * D + hh);
+        const float2 pl = *reinterpret_cast<const float2*>(p + NT * 8 * (D + 1) + hh);
+        const float4 v = reinterpret_cast<const float4*>(p)[f * 32 + lane];
+        join_part(c, m0, m1, l0, l1, pm, pl, v);
       }
-      const float m0 = p_m[e0][hh], m1 = p_m[e0][hh + 1], l0 = p_l[e0][hh], l1 = p_l[e0][hh + 1];
+      const int r = item / Hg, h = item - r * Hg, sub = h % ngr;
+      const int head0 = h / ngr * gq + sub * 8 * NT, heads = min(8 * NT, gq - sub * 8 * NT);
       if (has0 && has1) {
         const float i0 = l0 == 0.0f ? 0.0f : a.v_scale / l0;
         const float i1 = l1 == 0.0f ? 0.0f : a.v_scale / l1;
@@ -951,17 +937,13 @@ __global__ void __launch_bounds__(Shape<C, D, NT>::W * 32, 1)
           if (hh + 1 < heads) a.lse[(int64_t)r * a.Hq + head0 + hh + 1] = lse_of(m1, l1);
         }
       } else {
+        float* to = room.cross + ((int64_t)blockIdx.x * 2 + (has0 ? 1 : 0)) * PF;
         reinterpret_cast<float4*>(to)[f * 32 + lane] = c;
         if (j == 0 && g == 0) {
           *reinterpret_cast<float2*>(to + NT * 8 * D + hh) = make_float2(m0, m1);
           *reinterpret_cast<float2*>(to + NT * 8 * (D + 1) + hh) = make_float2(l0, l1);
         }
       }
-    }
-    if (has0 && !has1) {
-      cross.item = item;
-      // (no further than the last CTA, should the lengths change under the call)
-      cross.last = (int)min(p_end[tail >> 1] / (W * quota), (int64_t)gridDim.x - 1);
     }
   }
   if (threadIdx.x == 0) room.about[blockIdx.x] = cross;
@@ -993,17 +975,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32)
     const float2 pm = __ldcg(reinterpret_cast<const float2*>(p + NT * 8 * D + hh));
     const float2 pl = __ldcg(reinterpret_cast<const float2*>(p + NT * 8 * (D + 1) + hh));
     const float4 v = __ldcg(reinterpret_cast<const float4*>(p) + f * 32 + lane);
-    const float t0 = fmaxf(m0, pm.x), t1 = fmaxf(m1, pm.y);
-    const float a0 = weight(m0, t0), a1 = weight(m1, t1);
-    const float b0 = weight(pm.x, t0), b1 = weight(pm.y, t1);
-    c.x = c.x * a0 + v.x * b0;
-    c.y = c.y * a1 + v.y * b1;
-    c.z = c.z * a0 + v.z * b0;
-    c.w = c.w * a1 + v.w * b1;
-    l0 = l0 * a0 + pl.x * b0;
-    l1 = l1 * a1 + pl.y * b1;
-    m0 = t0;
-    m1 = t1;
+    join_part(c, m0, m1, l0, l1, pm, pl, v);
   }
   sc[warp][lane] = c;
   sm[warp][lane][0] = m0;
