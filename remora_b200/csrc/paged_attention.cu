@@ -30,10 +30,10 @@
 //     No atomics: the same inputs give the same bits.
 //
 // B200 (device time; the copy rate is 6462 GB/s): 64 requests of 7900 to 8190
-// keys, 8 kv heads of 128 bf16 elements, 2.11 GB: 325 to 335 us, 6.3 to 6.5
-// TB/s.  3 requests of 90 to 131 thousand keys over e4m3, 675 MB: 116 to 124 us
-// (the SM clock under power decides).  128 ragged requests, 272 MB: 52 us, of
-// which 9 are before the first and after the last tile.  700 keys: 9.9 us, two
+// keys, 8 kv heads of 128 bf16 elements, 2.11 GB: 321 to 338 us, 6.2 to 6.6
+// TB/s.  3 requests of 90 to 131 thousand keys over e4m3, 675 MB: 119 to 124 us
+// (the SM clock under power decides).  128 ragged requests, 272 MB: 51 us, of
+// which 7 are before the first and after the last tile.  700 keys: 9.1 us, two
 // launches of cold code.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
