@@ -22,13 +22,13 @@
 // whole heads in vectors of up to 8 pairs, the loads issued before the angles.
 //
 // B200, device time: 268.6 MB of bf16 [4,4096,32,128] (heads first, three
-// axes) 46.8 us = 5.74 TB/s, where a copy of the same bytes takes 42.6; 8192
-// tokens of 32 + 2 x 8 heads into an e4m3 cache (184.7 MB) 37.2 us = 4.96
+// axes) 45.8 us = 5.86 TB/s, where a copy of the same bytes takes 42.6; 8192
+// tokens of 32 + 2 x 8 heads into an e4m3 cache (184.7 MB) 36.6 us = 5.05
 // TB/s.  What it took: a thread keeping its unit of the head and walking over
-// heads (65 -> 51 us with the angles read without bank conflicts), then one
-// multiply-add per stride and paired conversions (-> 47).  Blocks of 128
-// threads, 64 registers, 8 to an SM: 256 threads 50, more blocks (spills) 56
-// to 61, 3 or 4 units a thread 59 and 51.
+// heads (65 -> 51 us with the angles read without bank conflicts), one
+// multiply-add per stride and paired conversions (-> 47), streaming stores.
+// Blocks of 128 threads, 64 registers, 8 to an SM: 256 threads 50 us, 9 and 10
+// blocks (spills) 56 and 61, 7 blocks 52, 3 units a thread in 6 blocks 54.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
@@ -132,14 +132,16 @@ struct Raw {
       w[0] = __ldcs(reinterpret_cast<const uint16_t*>(p));
     }
   }
+  // Streaming stores: first to leave L2 when room is short (46.8 -> 45.6 us for 268 MB), and
+  // still there for the next kernel when it is not.
   __device__ __forceinline__ void store(T* p) const {
     if constexpr (kBytes >= 16) {
 #pragma unroll
       for (int i = 0; i < kBytes / 16; ++i)
-        reinterpret_cast<uint4*>(p)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2],
-                                                    w[4 * i + 3]);
+        __stcs(reinterpret_cast<uint4*>(p) + i,
+               make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]));
     } else if constexpr (kBytes == 8) {
-      *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+      __stcs(reinterpret_cast<uint2*>(p), make_uint2(w[0], w[1]));
     } else if constexpr (kBytes == 4) {
       *reinterpret_cast<uint32_t*>(p) = w[0];
     } else if constexpr (kBytes == 2) {
