@@ -567,6 +567,35 @@ def test_attention_in_a_graph_behind_copies(rb):
         assert torch.equal(again, want) and torch.equal(room, want)
 
 
+def test_calls_refuse_mixed_devices_and_bad_buffers(rb):
+    """Each refusal comes before any launch; the next good call is not disturbed."""
+    out, (q, kc, vc, table, lens), kw = check_attention(rb, [40, 3], 4, 2, 64, 16, "bf16", "bf16")
+    need = rb.paged_attention_workspace_bytes(2, 4, 2, 64)
+    small = torch.empty(need - 1, dtype=torch.uint8, device="cuda")
+    odd = torch.empty(need + 8, dtype=torch.uint8, device="cuda")[8:]
+    for bad in (dict(out=q), dict(workspace=small), dict(workspace=odd), dict(window=-1),
+                dict(k_scale=0.5), dict(scale=math.nan)):
+        with pytest.raises(rb.RemoraError):
+            rb.paged_attention(q, kc, vc, table, lens, **{**kw, **bad})
+    for args in ((q.cpu(), kc, vc, table, lens), (q, kc, vc, table.cpu(), lens),
+                 (q, kc, vc, table, lens.long()), (q[:1], kc, vc, table, lens),
+                 (q, kc, vc[:-1], table, lens), (q, kc, vc, table.t(), lens)):
+        with pytest.raises((ValueError, TypeError)):
+            rb.paged_attention(*args, **kw)
+    x, pos = torch.ones(3, 2, 64, device="cuda"), i32([0, 1, 2])
+    for args in ((x.cpu(), pos, freqs(64)), (x, pos.cpu(), freqs(64)), (x, pos, freqs(64).cuda()),
+                 (x, pos[:2], freqs(64)), (x.transpose(1, 2), pos, freqs(4))):
+        with pytest.raises((ValueError, TypeError)):
+            rb.rope(*args)
+    t, f, c = i32([[0, 1]]), i32([2, 3]), i32([2])
+    for args in ((i32([1]).cpu(), i32([1]), t, f, c), (i32([1]), i32([1]), t, f, c.long()),
+                 (i32([1]), i32([1, 1]), t, f, c), (i32([1]), i32([1]), t.t(), f, c)):
+        with pytest.raises((ValueError, TypeError)):
+            rb.kv_block_table(*args, block_size=4, max_tokens=1)
+    assert torch.equal(rb.paged_attention(q, kc, vc, table, lens, **kw), out)
+    rb.synchronize_and_check()
+
+
 def test_attention_strided_q_and_out(rb):
     D = 128
     out, args, kw = check_attention(rb, [70, 0, 5], 8, 2, D, 16, "bf16", "bf16")
