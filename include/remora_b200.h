@@ -207,8 +207,10 @@ int remora_b200_attention_fwd_bf16(const void* q, const void* k, const void* v, 
  *
  * A request whose blocks would not be free, counting those of the requests
  * before it, is refused whole (status 1), and so are later ones that need a
- * block; status 2 marks a bad length or count, tokens past max_blocks blocks
- * or past max_tokens.  A refused request keeps its length and blocks.
+ * block; status 2 marks a bad length or count, tokens past max_blocks blocks,
+ * or an append (of no tokens too) behind more than max_tokens of them.  A
+ * refused request keeps its length and blocks.  A release is refused for a
+ * bad length only.
  *
  * Written: lens_out[R] and free_count_out[1] (either may be its input),
  * cu_tokens[R+1] (first token of each request; refused ones keep their

@@ -61,7 +61,12 @@ __device__ __forceinline__ int32_t sat32(int64_t v) {
 // What one request asks for: tokens, blocks needed, blocks released.
 struct Ask {
   int64_t tokens, need, back;
-  bool bad;
+  bool bad, append;
+  // Refused where the tokens up to its own end are t?  A release has no tokens that could lie past
+  // the room for them, and its blocks are pushed whatever the requests in front of it ask for.
+  __device__ __forceinline__ bool refused(int64_t t, int32_t max_tokens) const {
+    return bad || (append && t > max_tokens);
+  }
 };
 
 // Blocks of n tokens, n in [0, 2^31).
@@ -70,7 +75,7 @@ __device__ __forceinline__ int32_t blocks_of(const TableArgs& a, int32_t n) {
 }
 
 __device__ __forceinline__ Ask ask_of(const TableArgs& a, int32_t len, int32_t n) {
-  Ask q{0, 0, 0, false};
+  Ask q{0, 0, 0, false, n >= 0};
   const int64_t room = (int64_t)a.max_blocks * a.bs;  // below 2^31
   const bool held = len >= 0 && len <= room;
   const int32_t own = held ? blocks_of(a, len) : 0;
@@ -162,7 +167,7 @@ __global__ void __launch_bounds__(1024) k_block_table(const TableArgs a) {
       need[r] = sat32(p1);
       back[r] = sat32(p2);
       t += q.tokens;
-      const bool bad = q.bad || t > a.max_tokens;
+      const bool bad = q.refused(t, a.max_tokens);
       if (t <= a.max_tokens) p1 += q.need;
       p2 += q.back;
       const bool dry = !bad && q.need > 0 && p1 > have;
