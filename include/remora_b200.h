@@ -192,8 +192,9 @@ int remora_b200_attention_fwd_bf16(const void* q, const void* k, const void* v, 
  * stores x / scale, rounded to nearest even and saturated at +-448 (scales
  * in [1e-30, 1e30]).
  * Values that only the device sees (block ids, slots, lengths) are checked
- * there: a bad one is skipped and reported by remora_b200_device_status()
- * as REMORA_B200_ERR_INVALID.
+ * there: a bad one is skipped (a length past a request's table is taken as
+ * the table's room) and reported by remora_b200_device_status() as
+ * REMORA_B200_ERR_INVALID.  The report names no request.
  * --------------------------------------------------------------------- */
 
 /* Block tables, slots and positions of one step, from the requests' lengths.
@@ -216,8 +217,11 @@ int remora_b200_attention_fwd_bf16(const void* q, const void* k, const void* v, 
  * cu_tokens[R+1] (first token of each request; refused ones keep their
  * place), the new entries of block_table, and for each token t < max_tokens
  * its slot, position and request: -1, 0, r for a token of a refused request
- * and -1, 0, -1 behind the last token.  Deterministic; the same call on the
- * same lens and free_count gives the same result again. */
+ * and -1, 0, -1 behind the last token.  An id outside [0, num_blocks), popped
+ * or released, is reported and goes into the table or onto the stack as -1;
+ * its request is not refused for it (its length grows, the tokens there have
+ * slot -1).  Deterministic; the same call on the same lens and free_count
+ * gives the same result again. */
 typedef struct remora_b200_kv_block_table_args {
   const int32_t* lens;
   const int32_t* new_tokens;

@@ -69,6 +69,14 @@ struct Ask {
   }
 };
 
+// A block id as it may enter the table or the stack: one outside the cache is reported and
+// becomes -1.
+__device__ __forceinline__ int32_t checked_id(const TableArgs& a, int32_t id) {
+  if (id >= 0 && id < a.num_blocks) return id;
+  atomicExch(&g_device_error, 3);
+  return -1;
+}
+
 // Blocks of n tokens, n in [0, 2^31).
 __device__ __forceinline__ int32_t blocks_of(const TableArgs& a, int32_t n) {
   return n > 0 ? a.by_bs.div(n - 1) + 1 : 0;
@@ -194,7 +202,7 @@ __global__ void __launch_bounds__(1024) k_block_table(const TableArgs a) {
     const int room = min(n_back, a.num_blocks - count0);
     for (int64_t i = me; i < room; i += step) {
       const int j = (int)i, r = find_le(back, a.R, j);
-      a.free_blocks[count0 + j] = a.table[(int64_t)r * a.ld_table + (j - back[r])];
+      a.free_blocks[count0 + j] = checked_id(a, a.table[(int64_t)r * a.ld_table + (j - back[r])]);
     }
     cluster_barrier();
   }
@@ -223,14 +231,10 @@ __global__ void __launch_bounds__(1024) k_block_table(const TableArgs a) {
       if (r != seen_r || page != seen_page) {
         const int32_t own = blocks_of(a, l);
         if (page < own) {
-          id = a.table[(int64_t)r * a.ld_table + page];
+          id = checked_id(a, a.table[(int64_t)r * a.ld_table + page]);
         } else {
-          id = __ldcg(a.free_blocks + (have - 1 - (need[r] + page - own)));
+          id = checked_id(a, __ldcg(a.free_blocks + (have - 1 - (need[r] + page - own))));
           if (off == 0) a.table[(int64_t)r * a.ld_table + page] = id;
-        }
-        if (id < 0 || id >= a.num_blocks) {
-          atomicExch(&g_device_error, 3);
-          id = -1;
         }
         seen_r = r;
         seen_page = page;

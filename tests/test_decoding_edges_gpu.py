@@ -34,3 +34,52 @@ def test_block_table_releases_behind_an_overflow(rb, lens, new, mb, bs, spare, m
         if n == -1:
             assert int(got.status[r]) == 0 and int(got.lens[r]) == 0
     assert blocks_disjoint(got.lens.tolist(), want["table"], want["free"], int(got.free_count), bs)
+
+
+def test_block_table_ids_out_of_range_enter_neither_table_nor_stack(rb):
+    """A bad id on the stack: the table takes -1 for it and its tokens have no slot.  A bad id in
+    a released row: the stack takes -1, and so does the next request.  Each step reports."""
+    free = i32([3, 77, 1, 2])
+    table = torch.full((2, 3), -9, dtype=torch.int32, device="cuda")
+    st = rb.kv_block_table(i32([0, 0]), i32([8, 11]), table, free, i32([4]), block_size=8,
+                           max_tokens=19)
+    assert table.tolist() == [[2, -9, -9], [1, -1, -9]]
+    assert st.slots.tolist() == [*range(16, 24), *range(8, 16), -1, -1, -1]
+    assert st.positions.tolist() == [*range(8), *range(11)]
+    assert st.lens.tolist() == [8, 11] and st.status.tolist() == [0, 0]
+    assert st.free_count.tolist() == [1] and free.tolist() == [3, 77, 1, 2]
+    with pytest.raises(rb.RemoraError, match="block id"):
+        rb.synchronize_and_check()
+    for bad in (-1, 4, -5, 2 ** 31 - 1, -2 ** 31):
+        table, free, count = i32([[2, bad], [-9, -9]]), i32([0, 1, -7, -7]), i32([2])
+        st = rb.kv_block_table(i32([16, 0]), i32([-1, 0]), table, free, count, block_size=8,
+                               max_tokens=4)
+        assert free.tolist() == [0, 1, 2, -1] and st.free_count.tolist() == [4]
+        assert st.lens.tolist() == [0, 0] and st.status.tolist() == [0, 0]
+        with pytest.raises(rb.RemoraError, match="block id"):
+            rb.synchronize_and_check()
+        st = rb.kv_block_table(st.lens, i32([0, 12]), table, free, st.free_count, block_size=8,
+                               max_tokens=12)
+        assert table[1].tolist() == [-1, 2] and st.free_count.tolist() == [2]
+        assert st.slots.tolist() == [-1] * 8 + [16, 17, 18, 19]
+        with pytest.raises(rb.RemoraError, match="block id"):
+            rb.synchronize_and_check()
+    rb.synchronize_and_check()
+
+
+def test_attention_over_a_block_that_was_missing(rb):
+    """The keys of a block that a step could not give are left out, and reported."""
+    D, bs = 64, 8
+    kc = torch.randn(4, bs, 1, D, generator=gen(1)).to(torch.bfloat16).cuda()
+    vc = torch.randn(4, bs, 1, D, generator=gen(2)).to(torch.bfloat16).cuda()
+    q = torch.randn(1, 2, D, generator=gen(3)).to(torch.bfloat16).cuda()
+    table = i32([[-9, -9]])
+    st = rb.kv_block_table(i32([0]), i32([12]), table, i32([4, 3, -7, -7]), i32([2]),
+                           block_size=bs, max_tokens=12)
+    assert table.tolist() == [[3, -1]]
+    got = rb.paged_attention(q, kc, vc, table, st.lens)
+    with pytest.raises(rb.RemoraError, match="block id"):
+        rb.synchronize_and_check()
+    o, l, mag, size = ref.attention(q[0].cpu(), kc[3].cpu(), vc[3].cpu(), D ** -0.5)
+    close(got[0], o, ref.attention_bound(o, l, mag, size, bs, D, torch.bfloat16,
+                                         float(vc.abs().max()))[0])
