@@ -249,8 +249,8 @@ int remora_b200_kv_block_table(const remora_b200_kv_block_table_args* args, void
  * device.  freq (rot / 2 doubles) and axis_of (rot / 2 ints, NULL = all 0)
  * are HOST arrays, read before the call returns.  rot even, <= min(D, 256);
  * D <= 512 (above 256, sizes, strides and bases in whole 4 elements); n_axes
- * <= 8.  Angles are exact to 2^-25 of a quarter turn at
- * every 32-bit position.  Any strides (of tokens and heads below 2^31
+ * <= 8.  Frequencies below 2^64 radians per position; angles are exact to
+ * 2^-25 of a quarter turn at every one of them and every 32-bit position.  Any strides (of tokens and heads below 2^31
  * elements), at most 2^30 tokens; sizes, strides and bases that are multiples
  * of 8 elements (and 16 bytes) move 8 pairs at a time. */
 typedef struct remora_b200_rope_args {

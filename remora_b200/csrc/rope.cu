@@ -14,7 +14,8 @@
 // turns with the whole turns already gone: integer arithmetic, exact for every
 // 32-bit position up to the 2^-64 rounding of F.  The nearest quarter turn
 // comes off as an integer too, which leaves at most pi/4 for sincospif and an
-// error of 2^-25 of that, however far the position.
+// error of 2^-25 of that, however far the position (and whatever the frequency:
+// below a turn per position it is a long double product, above by words).
 //
 // Bound: HBM (each element read once and written once).  A block takes a few
 // tokens at a time, puts their cosines and sines into shared memory (one
@@ -420,6 +421,27 @@ int launch(Args& a, int v, int interleaved, cudaStream_t st) {
   return REMORA_B200_OK;
 }
 
+// freq / (2 pi) modulo one turn, in 2^-64 of a turn, for 1 <= |freq| < 2^64: the mantissa times
+// floor(2^192 / (2 pi)) by words, of which the 64 bits behind the point are taken.  What the
+// constant lacks is below 2^-128 turns; a product in long double would lose the bits behind the
+// point to those in front of it.
+inline uint64_t turns_of(double freq) {
+  constexpr uint64_t c[3] = {0x36d8a5664f10e410ull, 0x7f09d5f47d4d3770ull, 0x28be60db9391054aull};
+  int e;
+  const uint64_t m = (uint64_t)std::ldexp(std::frexp(std::fabs(freq), &e), 53);
+  uint64_t p[4];  // m * 2^192 / (2 pi)
+  unsigned __int128 carry = 0;
+  for (int i = 0; i < 3; ++i) {
+    carry += (unsigned __int128)m * c[i];
+    p[i] = (uint64_t)carry;
+    carry >>= 64;
+  }
+  p[3] = (uint64_t)carry;
+  const int down = 128 - (e - 53), word = down / 64, bit = down % 64;  // down in [117, 180]
+  const uint64_t f = p[word] >> bit | (bit ? p[word + 1] << (64 - bit) : 0);
+  return freq < 0 ? 0 - f : f;
+}
+
 // Checks and converts what both entry points share.
 inline int angles(const char* who, Args& a, const int32_t* positions, int64_t ld_pos, int n_axes,
                   const double* freq, const int32_t* axis_of, int64_t rot, int64_t D,
@@ -442,14 +464,17 @@ inline int angles(const char* who, Args& a, const int32_t* positions, int64_t ld
   a.ld_pos = ld_pos;
   a.tokens = (int32_t)tokens;
   for (int i = 0; i < a.half; ++i) {
-    RB_CHECK_ARG(std::isfinite(freq[i]), "%s: freq[%d] is not finite", who, i);
+    RB_CHECK_ARG(std::fabs(freq[i]) < 18446744073709551616.0,
+                 "%s: freq[%d] is not finite or not below 2^64", who, i);
     const int ax = axis_of ? axis_of[i] : 0;
     RB_CHECK_ARG(ax >= 0 && ax < n_axes, "%s: axis_of[%d] = %d is not in [0, %d)", who, i, ax,
                  n_axes);
     long double t = (long double)freq[i] * 0.159154943091895335768883763373L;  // / (2 pi)
-    if (!(t >= 0 && t < 1)) t -= floorl(t);
+    if (t > -1 && t < 0) t += 1;
     const long double f = t * 18446744073709551616.0L;
-    a.turns.f[i] = f >= 18446744073709551615.0L ? 0 : (uint64_t)f;
+    a.turns.f[i] = !(t > -1 && t < 1)              ? turns_of(freq[i])
+                   : f >= 18446744073709551615.0L ? 0
+                                                  : (uint64_t)f;
     a.turns.axis[i] = (uint8_t)ax;
   }
   return REMORA_B200_OK;

@@ -83,3 +83,43 @@ def test_attention_over_a_block_that_was_missing(rb):
     o, l, mag, size = ref.attention(q[0].cpu(), kc[3].cpu(), vc[3].cpu(), D ** -0.5)
     close(got[0], o, ref.attention_bound(o, l, mag, size, bs, D, torch.bfloat16,
                                          float(vc.abs().max()))[0])
+
+
+# ------------------------------------------------------------------- rotary
+def two_pi(bits):
+    """floor(2 pi * 2^bits), by arctan(1/5) and arctan(1/239)."""
+    def arctan_inverse(n):
+        term = (1 << bits + 32) // n
+        total, k, sign = term, 1, -1
+        while term:
+            term //= n * n
+            k += 2
+            total += sign * (term // k)
+            sign = -sign
+        return total >> 32
+    return 8 * (4 * arctan_inverse(5) - arctan_inverse(239))
+
+
+def angle_of(position, freq, turn=two_pi(400)):
+    """position * freq modulo 2 pi, exactly and then rounded."""
+    f = Fraction(float(freq)) * position * 2 ** 400
+    return float(Fraction(f.numerator % (turn * f.denominator), f.denominator * 2 ** 400))
+
+
+@pytest.mark.parametrize("inverse", [False, True])
+def test_rope_frequencies_of_many_turns(rb, inverse):
+    """The angle keeps its precision whatever the frequency: here to just below 2^64."""
+    below = math.nextafter(2.0 ** 64, 0)
+    f = [1.0, 6.28, 2 * math.pi, math.nextafter(2 * math.pi, 7), 7.5, 1e3, 1e4, 31415.9, 1e6, 1e9,
+         1e12 + 0.5, 2.0 ** 53 - 1, 1e18, below, 2.0 ** 63, 1e-9]
+    f = torch.tensor(f + [-x for x in f], dtype=torch.float64)
+    pos = [0, 1, -1, 5, 2 ** 24 + 1, 2 ** 31 - 1, -2 ** 31, 123456789]
+    x = torch.randn(len(pos), 2, 64, generator=gen(4))
+    got = rb.rope(x.cuda(), i32(pos), f, inverse=inverse)
+    a = torch.tensor([[angle_of(p, v) for v in f.tolist()] for p in pos], dtype=torch.float64)
+    c, s = a.cos()[:, None], a.sin()[:, None] * (-1 if inverse else 1)
+    lo, hi = x[..., :32].double(), x[..., 32:].double()
+    want = torch.cat([lo * c - hi * s, lo * s + hi * c], -1)
+    # the errors that rope_bound counts, without its reference's own rounded angle
+    b = ((lo.abs() + hi.abs()) * 2.0 ** -21).repeat(1, 1, 2)
+    close(got, want, ref.half_step(torch.float32) * (want.abs() + b) + b)
