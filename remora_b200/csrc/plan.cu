@@ -100,8 +100,9 @@ void decode_plan(Text& t, int64_t R, int64_t Hq, int64_t Hkv, int64_t S) {
         l.smem);
   t.add("remora_b200_rope_kv_append(q bf16[%lld,%lld,128], k/v bf16[%lld,%lld,128], cache blocks of "
         "%lld tokens)\n", (long long)R, (long long)Hq, (long long)R, (long long)Hkv, (long long)bs);
-  t.add("  rb::rope::k_rope  grid %lld x block %d (whole heads in units of 8 pairs)\n",
-        (long long)std::min<int64_t>(R, (int64_t)num_sms() * 16), rope::kThreads);
+  const rope::Tiling rt = rope::tiling((int)D, (int)D / 2, 8, (int)(Hq + 2 * Hkv), R);
+  t.add("  rb::rope::k_rope  grid %d x block %d (tiles of %d tokens, heads in units of 8 pairs)\n",
+        rt.grid, rope::kThreads, rt.tile);
   t.add("remora_b200_paged_attention(q bf16[%lld,%lld,128], %lld kv heads, up to %lld keys)\n",
         (long long)R, (long long)Hq, (long long)Hkv, (long long)S + 1);
   t.add("  rb::paged::k_paged_split  grid %d x block %d, smem %d B (tiles of %d keys, %d in a "

@@ -386,24 +386,38 @@ struct Fit {
   }
 };
 
-template <typename T, typename C, bool kAppend>
-int launch(Args& a, int v, int interleaved, cudaStream_t st) {
-  a.rot_units = a.half / v;
-  a.units = (a.D / v + 1) / 2;  // = rot_units + ceil of half the rest
-  RB_CHECK_ARG(a.units <= kThreads,
-               "rope: head_dim above %d needs sizes, strides and bases of whole 4 elements",
-               2 * kThreads);
-  a.pass = kThreads / a.units;
-  const int heads = a.q.H + (kAppend ? a.k.H + a.v.H : 0);
-  a.heads = Divisor((uint32_t)heads);
+// How a launch is cut, for heads of D elements of which 2 * half turn, v pairs at a time: units of
+// a head (at most kThreads, which the caller checks), heads side by side, tokens of a tile, blocks.
+struct Tiling {
+  int units, pass, tile, grid;
+};
+inline Tiling tiling(int D, int half, int v, int heads, int64_t tokens) {
+  Tiling t;
+  t.units = (D / v + 1) / 2;  // half / v, and ceil of half the rest
+  t.pass = std::max(kThreads / t.units, 1);
   // The tokens whose heads fill a block's units once, within the angles' room, and no more than
   // leave every SM a tile.  (Several rounds of units per tile measured slower: 8 tokens of 32 heads
   // 55 us against 47, 8 of 48 into e4m3 39.4 against 37.5; one token of 12 heads 5.9 against 5.6.)
-  const int64_t room = std::min<int64_t>(kTileAngles / std::max(a.half, 1), kTileTokens);
-  const int64_t most = std::min<int64_t>(room, a.tokens / num_sms());
-  a.tile = (int)std::max<int64_t>(std::min<int64_t>(most, kUnits * a.pass / heads), 1);
-  const int64_t tiles = ((int64_t)a.tokens + a.tile - 1) / a.tile;
-  const int grid = (int)std::min<int64_t>(tiles, (int64_t)num_sms() * 16);
+  const int64_t room = std::min<int64_t>(kTileAngles / std::max(half, 1), kTileTokens);
+  const int64_t most = std::min<int64_t>(room, tokens / num_sms());
+  t.tile = (int)std::max<int64_t>(std::min<int64_t>(most, kUnits * t.pass / heads), 1);
+  t.grid = (int)std::min<int64_t>((tokens + t.tile - 1) / t.tile, (int64_t)num_sms() * 16);
+  return t;
+}
+
+template <typename T, typename C, bool kAppend>
+int launch(Args& a, int v, int interleaved, cudaStream_t st) {
+  const int heads = a.q.H + (kAppend ? a.k.H + a.v.H : 0);
+  const Tiling t = tiling(a.D, a.half, v, heads, a.tokens);
+  RB_CHECK_ARG(t.units <= kThreads,
+               "rope: head_dim above %d needs sizes, strides and bases of whole 4 elements",
+               2 * kThreads);
+  a.rot_units = a.half / v;
+  a.units = t.units;
+  a.pass = t.pass;
+  a.tile = t.tile;
+  a.heads = Divisor((uint32_t)heads);
+  const int grid = t.grid;
 #define RB_ROPE(VV, I) k_rope<T, C, VV, I, kAppend><<<grid, kThreads, 0, st>>>(a)
 #define RB_ROPE_V(I)                          \
   do {                                        \

@@ -13,3 +13,14 @@ def test_rope_refuses_frequencies_it_cannot_hold(L, bad):  # noqa: F811
     freq = (ctypes.c_double * 64)(*[0.5] * 63, bad)
     for call in (rope, append):
         assert call(L, freq=ctypes.addressof(freq)) == rb.ERR_INVALID and "freq[63]" in rb.last_error()
+
+
+@pytest.mark.parametrize("config,tile,grid", [
+    ("64x32x8x4096", 1, 64),     # fewer tokens than SMs
+    ("4000x4x4x100", 2, 2000),   # 12 heads of 8 units: 32 of them fill a block's units
+    ("4096x4x1x16", 5, 820),     # 6 heads
+    ("8192x32x8x100", 1, 2368),  # 48 heads: one token, 16 blocks to each of 148 SMs
+])
+def test_decode_plan_cuts_the_append_as_the_launch_does(L, config, tile, grid):  # noqa: F811
+    line = next(x for x in rb.launch_plan("decode", config).splitlines() if "k_rope" in x)
+    assert f"grid {grid} x block 128" in line and f"tiles of {tile} tokens" in line
