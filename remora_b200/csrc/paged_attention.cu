@@ -622,8 +622,9 @@ __global__ void __launch_bounds__(Shape<C, D, NT>::W * 32, 1)
       for (int n = 0; n < NT; ++n) {
         float fac = 1.0f;
         if constexpr (F8 && !std::is_same<T, __half>::value) {
-          // bf16 queries against keys widened to f16: the row is brought to [1, 2) by a
-          // power of two (put back on the scores), so that f16 holds all of a bf16's 8 bits
+          // bf16 queries against keys widened to f16: the row is brought to [2^14, 2^15), the top
+          // of f16, by a power of two (put back on the scores), so that elements down to 2^-31 of
+          // the largest keep all of a bf16's 8 bits
           uint32_t top = 0;
 #pragma unroll
           for (int j = 0; j < D / 16; ++j)
@@ -634,9 +635,9 @@ __global__ void __launch_bounds__(Shape<C, D, NT>::W * 32, 1)
             }
           top = max(top, __shfl_xor_sync(~0u, top, 1));
           top = max(top, __shfl_xor_sync(~0u, top, 2));
-          const uint32_t ex = min(max(top << 16 & 0x7f800000u, 0x00800000u), 0x7e800000u);
-          fac = __uint_as_float(ex);
-          const float inv = __uint_as_float(0x7f000000u - ex);
+          const uint32_t ex = min(max(top << 16 & 0x7f800000u, 0x07800000u), 0x7f000000u);
+          fac = __uint_as_float(ex - 0x07000000u);             // 2^-14 of it
+          const float inv = __uint_as_float(0x86000000u - ex);  // 1 / fac
 #pragma unroll
           for (int j = 0; j < D / 16; ++j)
 #pragma unroll

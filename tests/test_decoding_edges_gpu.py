@@ -123,3 +123,27 @@ def test_rope_frequencies_of_many_turns(rb, inverse):
     # the errors that rope_bound counts, without its reference's own rounded angle
     b = ((lo.abs() + hi.abs()) * 2.0 ** -21).repeat(1, 1, 2)
     close(got, want, ref.half_step(torch.float32) * (want.abs() + b) + b)
+
+
+# ---------------------------------------------------------------- attention
+@pytest.mark.parametrize("below", [14, 20, 27, 30])
+def test_attention_small_queries_beside_large_ones(rb, below):
+    """bf16 queries over 8-bit keys: one element is 2^below times the others and meets zeros, so
+    the others decide.  All of a bf16's bits of theirs count."""
+    D, n, bs = 128, 100, 16
+    g = gen(below)
+    k = torch.randint(-448, 449, (7 * bs, 1, D), generator=g).float().to(torch.float8_e4m3fn)
+    k.view(torch.uint8)[..., 5] = 0
+    v = torch.randn(7 * bs, 1, D, generator=g).to(torch.float8_e4m3fn)
+    q = torch.randn(1, 2, D, generator=g).sign() * (1 + torch.randint(0, 128, (1, 2, D), generator=g) / 128)
+    q[..., 5] = 2.0 ** below
+    scale = 1.0 / 2000
+    lse = torch.empty(1, 2, device="cuda")
+    out = rb.paged_attention(q.to(torch.bfloat16).cuda(), k.view(7, bs, 1, D).cuda(),
+                             v.view(7, bs, 1, D).cuda(), i32([range(7)]), i32([n]), scale=scale,
+                             lse=lse)
+    o, l, mag, size = ref.attention(q[0], k[:n].float(), v[:n].float(), scale)
+    b, bl = ref.attention_bound(o, l, mag, size, n, D, torch.bfloat16, float(v.float().abs().max()),
+                                torch.float8_e4m3fn)
+    close(out[0], o, b)
+    close(lse[0], l, bl)
