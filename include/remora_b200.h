@@ -311,7 +311,7 @@ size_t remora_b200_paged_attention_workspace_bytes(int64_t R, int64_t Hq, int64_
  * column NaN.  q and out: dtype BF16 or F16, [R][Hq][D] by strides (out must
  * not be q); caches: dtype, or E4M3 with scales.  D in {64, 128, 256},
  * Hq % Hkv == 0, R <= 8192; 16-byte aligned bases, strides of whole 16
- * bytes.  The call is two launches: the split over the keys, then the join
+ * bytes; |scale| and |scale * k_scale| below 2.3e38.  The call is two launches: the split over the keys, then the join
  * of what was split. */
 typedef struct remora_b200_paged_attention_args {
   const void* q;

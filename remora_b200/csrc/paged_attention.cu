@@ -648,8 +648,9 @@ __global__ void __launch_bounds__(Shape<C, D, NT>::W * 32, 1)
             }
         }
         // the scale's sign goes to the queries, so that the maximum is found before scaling; a
-        // scale of zero is queries of zero (a masked score stays -inf)
-        const float f = fmaxf(fabsf(a.scale2) * fac, 1.2e-38f);  // of this lane's row, head g
+        // scale of zero is queries of zero.  The factor of this lane's row, head g, is neither zero
+        // nor infinite: a masked score stays -inf, and a product of zero a score of zero
+        const float f = fminf(fmaxf(fabsf(a.scale2) * fac, 1.4e-45f), 3.4e38f);
         sc[n][0] = __shfl_sync(~0u, f, 8 * t4);
         sc[n][1] = __shfl_sync(~0u, f, 8 * t4 + 4);
         if (a.scale2 <= 0.0f) {
@@ -1114,6 +1115,8 @@ extern "C" int remora_b200_paged_attention(const remora_b200_paged_attention_arg
                "paged_attention: max_blocks * block_size must be in [1, 2^31) and ld_table at "
                "least max_blocks");
   RB_CHECK_ARG(std::isfinite(p.scale), "paged_attention: scale is not finite");
+  RB_CHECK_ARG(std::isfinite(p.scale * 1.4426950408889634f * p.k_scale),
+               "paged_attention: scale, and scale times k_scale, must be below 2.3e38");
   RB_CHECK_ARG(p.window >= 0, "paged_attention: window must not be negative");
   RB_CHECK_ARG(rope::scale_ok(p.k_scale) && rope::scale_ok(p.v_scale),
                "paged_attention: the cache scales must lie in [1e-30, 1e30]");

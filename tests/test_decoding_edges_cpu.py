@@ -24,3 +24,10 @@ def test_rope_refuses_frequencies_it_cannot_hold(L, bad):  # noqa: F811
 def test_decode_plan_cuts_the_append_as_the_launch_does(L, config, tile, grid):  # noqa: F811
     line = next(x for x in rb.launch_plan("decode", config).splitlines() if "k_rope" in x)
     assert f"grid {grid} x block 128" in line and f"tiles of {tile} tokens" in line
+
+
+@pytest.mark.parametrize("bad", [dict(scale=3e38), dict(scale=-3e38),
+                                 dict(cdt=rb.E4M3, scale=1e10, ks=1e30),
+                                 dict(cdt=rb.E4M3, scale=3e9, ks=1e29, R=0)])
+def test_attention_refuses_scales_whose_product_is_infinite(L, bad):  # noqa: F811
+    assert attention(L, **bad) == rb.ERR_INVALID and "k_scale" in rb.last_error()

@@ -147,3 +147,34 @@ def test_attention_small_queries_beside_large_ones(rb, below):
                                 torch.float8_e4m3fn)
     close(out[0], o, b)
     close(lse[0], l, bl)
+
+
+@pytest.mark.parametrize("dtype,cache,q,key,scale,k_scale", [
+    ("bf16", "e4m3", 1e38, 0.0, 0.125, 1e6),      # a factor past 32 bits, of products of zero
+    ("bf16", "e4m3", 1e38, 0.0, -1e7, 1.0),
+    ("bf16", "bf16", 1e18, 1e18, 1e-40, 1.0),     # a scale below the normal range
+    ("f16", "e4m3", 3e4, 448.0, 1e-30, 1e-12),
+    ("bf16", "e4m3", 1e-38, 448.0, 1e-8, 1e-30),  # a factor that is zero in 32 bits
+])
+def test_attention_factors_out_of_range(rb, dtype, cache, q, key, scale, k_scale):
+    """Scores that are ordinary numbers (here equal, so the output is the mean of the values and
+    lse = score + log n), though the factor of their products is none."""
+    from tests.test_paged_gpu import DT
+    D, n = 64, 20
+    kc = torch.full((2, 16, 1, D), key).to(DT[cache]).cuda()
+    vc = torch.randn(2, 16, 1, D, generator=gen(2)).to(DT[cache]).cuda()
+    lse = torch.empty(1, 2, device="cuda")
+    x = torch.full((1, 2, D), q).to(DT[dtype])
+    out = rb.paged_attention(x.cuda(), kc, vc, i32([[0, 1]]), i32([n]), scale=scale, k_scale=k_scale,
+                             lse=lse)
+    v = vc.float().cpu().view(32, D)[:n].double()
+    score = float(x[0, 0, 0].double() * kc[0, 0, 0, 0].cpu().double()) * D * scale * k_scale
+    mean, mag = v.mean(0), v.abs().mean(0)
+    # the mean's sums and weights (2^-11 of one f16 piece), then the output's rounding
+    b = mag * (2.0 ** -11 + (n + 8) * 2.0 ** -23) + 2.0 ** -24
+    assert bool(((out[0].double().cpu() - mean).abs() <= b + ref.half_step(DT[dtype]) *
+                 (mean.abs() + b)).all())
+    # 1e-40 holds 17 bits: 2^-17 of the score, and the logarithm's sum 2^-20
+    want = score + math.log(n)
+    assert bool(((lse.cpu().double() - want).abs() <= 2.0 ** -16 * abs(score) + 2.0 ** -20).all())
+    rb.synchronize_and_check()
