@@ -691,9 +691,10 @@ extern "C" int remora_b200_device_status(void) {
 
 extern "C" int remora_b200_recognise(const char* test) {
   if (!test) return 0;
-  std::string t = test;
-  return t == "elementwise" || t == "projection" || t == "elementwise_chain" || t == "gemm" ||
-         t == "attention" || t == "decode" || t == "moe";
+  for (const char* kind : {"elementwise", "projection", "elementwise_chain", "gemm", "attention",
+                           "decode", "moe"})
+    if (strcmp(test, kind) == 0) return 1;
+  return 0;
 }
 
 extern "C" int remora_b200_run_test(const char* test, const remora_b200_opts* o,
@@ -705,24 +706,17 @@ extern "C" int remora_b200_run_test(const char* test, const remora_b200_opts* o,
   RB_CUDA(cudaSetDevice(o ? o->device : 0));
   cudaStream_t st;
   RB_CUDA(cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking));
-  std::string t = test;
-  int rc;
-  if (t == "elementwise")
-    rc = run_elementwise(o, r, st);
-  else if (t == "projection")
-    rc = run_projection(o, r, st);
-  else if (t == "elementwise_chain")
-    rc = run_chain(o, r, st);
-  else if (t == "gemm")
-    rc = run_gemm(o, r, st);
-  else if (t == "attention")
-    rc = run_attention(o, r, st);
-  else if (t == "decode")
-    rc = run_decode(o, r, st);
-  else if (t == "moe")
-    rc = run_moe(o, r, st);
-  else
-    rc = fail(REMORA_B200_ERR_UNSUPPORTED, "--run-gpu for test '%s' not recognised", test);
+  int rc = guarded("run_test", [&] {
+    const std::string t = test;
+    if (t == "elementwise") return run_elementwise(o, r, st);
+    if (t == "projection") return run_projection(o, r, st);
+    if (t == "elementwise_chain") return run_chain(o, r, st);
+    if (t == "gemm") return run_gemm(o, r, st);
+    if (t == "attention") return run_attention(o, r, st);
+    if (t == "decode") return run_decode(o, r, st);
+    if (t == "moe") return run_moe(o, r, st);
+    return fail(REMORA_B200_ERR_UNSUPPORTED, "--run-gpu for test '%s' not recognised", test);
+  });
   cudaStreamDestroy(st);
   if (rc == REMORA_B200_OK && !r->passed)
     rc = fail(REMORA_B200_ERR_PARITY, "%s", r->detail);

@@ -114,15 +114,7 @@ void decode_plan(Text& t, int64_t R, int64_t Hq, int64_t Hkv, int64_t S) {
           paged::kJoinWarps * 32);
 }
 
-}  // namespace plan
-}  // namespace rb
-
-extern "C" int remora_b200_launch_plan(const char* test, const char* config, char* out,
-                                       size_t out_bytes) {
-  using namespace rb;
-  using namespace rb::plan;
-  clear_error();
-  RB_CHECK_ARG(test && out && out_bytes > 0, "launch_plan: null argument");
+int program_plan(const char* test, const char* config, char* out, size_t out_bytes) {
   const std::string kind = test, c = config ? config : "";
   Text t;
   if (kind == "elementwise") {
@@ -189,4 +181,15 @@ extern "C" int remora_b200_launch_plan(const char* test, const char* config, cha
   out[m] = '\0';
   return t.s.size() < out_bytes ? REMORA_B200_OK
                                  : fail(REMORA_B200_ERR_INVALID, "launch_plan: buffer too small");
+}
+
+}  // namespace plan
+}  // namespace rb
+
+extern "C" int remora_b200_launch_plan(const char* test, const char* config, char* out,
+                                       size_t out_bytes) {
+  using namespace rb;
+  clear_error();
+  RB_CHECK_ARG(test && out && out_bytes > 0, "launch_plan: null argument");
+  return guarded("launch_plan", [&] { return plan::program_plan(test, config, out, out_bytes); });
 }

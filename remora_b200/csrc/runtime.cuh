@@ -11,6 +11,7 @@
 #include <cstdint>
 #include <cstdio>
 #include <cstring>
+#include <exception>
 #include <mutex>
 
 #include "../../include/remora_b200.h"
@@ -50,6 +51,17 @@ inline void clear_error() { t_last_error[0] = '\0'; }
       return ::rb::fail(REMORA_B200_ERR_CUDA, "launch failed: %s (%s:%d)",              \
                         cudaGetErrorString(_e), __FILE__, __LINE__);                    \
   } while (0)
+
+// What a C entry point does with host containers: an exception (no memory, above all) becomes a
+// status, since none may leave an extern "C" function.
+template <typename F>
+int guarded(const char* who, F&& body) {
+  try {
+    return body();
+  } catch (const std::exception& e) {
+    return fail(REMORA_B200_ERR_INVALID, "%s: on the host: %s", who, e.what());
+  }
+}
 
 inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s); }
 

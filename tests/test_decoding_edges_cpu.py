@@ -31,3 +31,27 @@ def test_decode_plan_cuts_the_append_as_the_launch_does(L, config, tile, grid): 
                                  dict(cdt=rb.E4M3, scale=3e9, ks=1e29, R=0)])
 def test_attention_refuses_scales_whose_product_is_infinite(L, bad):  # noqa: F811
     assert attention(L, **bad) == rb.ERR_INVALID and "k_scale" in rb.last_error()
+
+
+_SCARCE = """
+import ctypes, resource, sys
+import remora_b200 as rb
+L, big = rb.lib(), b"x" * (64 << 20)
+buf = ctypes.create_string_buffer(64)
+held = int(next(x for x in open("/proc/self/status") if x.startswith("VmSize")).split()[1]) * 1024
+resource.setrlimit(resource.RLIMIT_AS, (held + (16 << 20), resource.RLIM_INFINITY))
+print(L.remora_b200_recognise(big), L.remora_b200_launch_plan(b"decode", big, buf, 64))
+print(L.remora_b200_last_error().decode())
+print(L.remora_b200_launch_plan(big, None, buf, 64), L.remora_b200_recognise(b"decode"))
+"""
+
+
+def test_no_exception_leaves_the_c_entry_points(L):  # noqa: F811
+    """Host memory that cannot be had is a status, not the end of the process."""
+    import subprocess
+    import sys
+
+    r = subprocess.run([sys.executable, "-c", _SCARCE], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stderr
+    first, text, last = r.stdout.splitlines()
+    assert first == f"0 {rb.ERR_INVALID}" and "launch_plan" in text and last == f"{rb.ERR_INVALID} 1"
