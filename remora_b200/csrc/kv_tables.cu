@@ -313,6 +313,10 @@ extern "C" int remora_b200_kv_block_table(const remora_b200_kv_block_table_args*
                "kv_block_table: null pointer");
   RB_CHECK_ARG(x.max_tokens == 0 || (x.slots && x.positions && x.requests),
                "kv_block_table: null pointer");
+  RB_CHECK_ARG(aligned4(x.lens, x.new_tokens, x.block_table, x.free_blocks, x.free_count,
+                        x.lens_out, x.free_count_out, x.cu_tokens, x.slots, x.positions,
+                        x.requests, x.status),
+               "kv_block_table: a pointer is not aligned to its elements");
   TableArgs a{x.lens, x.new_tokens, x.block_table, x.ld_table, x.free_blocks, x.lens_out,
               x.free_count_out, x.cu_tokens, x.slots, x.positions, x.requests, x.status,
               x.free_count, (int32_t)x.R, (int32_t)x.max_blocks, (int32_t)x.num_blocks,

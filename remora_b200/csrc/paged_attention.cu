@@ -1128,6 +1128,8 @@ extern "C" int remora_b200_paged_attention(const remora_b200_paged_attention_arg
   RB_CHECK_ARG(p.q != p.out, "paged_attention: out must not be q");
   RB_CHECK_ARG(aligned16(p.q) && aligned16(p.k_cache) && aligned16(p.v_cache) && aligned16(p.out),
                "paged_attention: q, the caches and out must be 16-byte aligned");
+  RB_CHECK_ARG(aligned4(p.block_table, p.lens, p.lse),
+               "paged_attention: a pointer is not aligned to its elements");
   const int64_t ce = p.cache_dtype == REMORA_B200_E4M3 ? 16 : 8;
   RB_CHECK_ARG(p.q_t % 8 == 0 && p.q_h % 8 == 0 && p.out_t % 8 == 0 && p.out_h % 8 == 0 &&
                    p.kc_block % ce == 0 && p.kc_token % ce == 0 && p.kc_head % ce == 0 &&

@@ -526,7 +526,7 @@ extern "C" int remora_b200_rope(const remora_b200_rope_args* args, void* stream)
   f.elems(D);
   f.rows(p.x, e, B > 1 ? p.x_b : 0, p.x_s, p.x_h);
   f.rows(p.out, e, B > 1 ? p.out_b : 0, p.out_s, p.out_h);
-  RB_CHECK_ARG(f.whole, "rope: a pointer is not aligned to its elements");
+  RB_CHECK_ARG(f.whole && aligned4(p.positions), "rope: a pointer is not aligned to its elements");
   cudaStream_t st = as_stream(stream);
   if (p.dtype == REMORA_B200_BF16)
     return launch<__nv_bfloat16, __nv_bfloat16, false>(a, f.v, p.interleaved, st);
@@ -595,7 +595,8 @@ extern "C" int remora_b200_rope_kv_append(const remora_b200_rope_kv_append_args*
   f.rows(p.v, 2, p.v_t, p.v_h, 0);
   f.rows(p.k_cache, c, p.kc_block, p.kc_token, p.kc_head);
   f.rows(p.v_cache, c, p.vc_block, p.vc_token, p.vc_head);
-  RB_CHECK_ARG(f.whole, "rope_kv_append: a pointer is not aligned to its elements");
+  RB_CHECK_ARG(f.whole && aligned4(p.positions, p.slots),
+               "rope_kv_append: a pointer is not aligned to its elements");
   cudaStream_t st = as_stream(stream);
   if (p.dtype == REMORA_B200_BF16)
     return p.cache_dtype == REMORA_B200_E4M3

@@ -67,6 +67,12 @@ inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// Whether all of these arrays of 32-bit elements lie where the device can read one.
+template <typename... P>
+inline bool aligned4(const P*... p) {
+  return ((reinterpret_cast<uintptr_t>(p) | ... | uintptr_t(0)) & 3u) == 0;
+}
+
 // Division of n < 2^31 by d, as a multiplication: m = floor(2^(31 + s) / d) + 1 with 2^s >= d
 // is off by at most 2^s / d < 1 per n / 2^31, which never carries into the quotient.
 struct Divisor {

@@ -55,3 +55,13 @@ def test_no_exception_leaves_the_c_entry_points(L):  # noqa: F811
     assert r.returncode == 0, r.stderr
     first, text, last = r.stdout.splitlines()
     assert first == f"0 {rb.ERR_INVALID}" and "launch_plan" in text and last == f"{rb.ERR_INVALID} 1"
+
+
+@pytest.mark.parametrize("off", [1, 2, 3])
+@pytest.mark.parametrize("call,fields", [
+    (tables, "lens new table free count lo co cu slots pos req status"), (rope, "pos"),
+    (append, "pos slots"), (attention, "table lens lse")])
+def test_arrays_between_elements_are_refused(L, call, fields, off):  # noqa: F811
+    """A 32-bit array at an address that no 32-bit load can take."""
+    for name in fields.split():
+        assert call(L, **{name: A + off}) == rb.ERR_INVALID and "aligned" in rb.last_error(), name
