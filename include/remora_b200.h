@@ -245,8 +245,8 @@ int remora_b200_kv_block_table(const remora_b200_kv_block_table_args* args, void
  * which is also the gradient of the forward form.  Pairs are (i, i + rot/2),
  * or (2i, 2i + 1) if interleaved != 0; elements from rot on are copied.
  * x and out: dtype BF16, F16 or F32, [B][S][H][D] by the strides x_b, x_s,
- * x_h (elements; out may be x).  positions: n_axes rows of B * S int32 on the
- * device.  freq (rot / 2 doubles) and axis_of (rot / 2 ints, NULL = all 0)
+ * x_h (elements; out may be x, with its strides; the rows of out must not
+ * overlap).  positions: n_axes rows of B * S int32 on the device.  freq (rot / 2 doubles) and axis_of (rot / 2 ints, NULL = all 0)
  * are HOST arrays, read before the call returns.  rot even, <= min(D, 256);
  * D <= 512 (above 256, sizes, strides and bases in whole 4 elements); n_axes
  * <= 8.  Frequencies below 2^64 radians per position; angles are exact to
@@ -268,8 +268,8 @@ int remora_b200_rope(const remora_b200_rope_args* args, void* stream);
 /* The same rotation of q and k, and the append of k and v to the cache, in
  * one pass: q_out[t] = rope(q[t]), cache row of slots[t] = rope(k[t]) and
  * v[t].  q [T][Hq][D], k and v [T][Hkv][D] by token and head strides (slices
- * of one projection are taken as they lie; q_out may be q); dtype BF16 or
- * F16; cache_dtype is dtype or E4M3 (then with the scales k_scale and
+ * of one projection are taken as they lie; q_out may be q, with its strides;
+ * the rows of q_out and of the caches must not overlap); dtype BF16 or F16; cache_dtype is dtype or E4M3 (then with the scales k_scale and
  * v_scale, else both must be 1).  A token whose slot is -1 writes no cache
  * row.  Two tokens of one slot leave one row or the other in each element.
  * kc_* and vc_*: the caches' strides of block, token and head.  The rest as
@@ -309,7 +309,7 @@ size_t remora_b200_paged_attention_workspace_bytes(int64_t R, int64_t Hq, int64_
  * lse = -infinity.  Cache rows past a request's length are never used,
  * whatever they hold; an infinity or NaN in a used row of values makes its
  * column NaN.  q and out: dtype BF16 or F16, [R][Hq][D] by strides (out must
- * not be q); caches: dtype, or E4M3 with scales.  D in {64, 128, 256},
+ * not be q, nor its rows overlap); caches: dtype, or E4M3 with scales.  D in {64, 128, 256},
  * Hq % Hkv == 0, R <= 8192; 16-byte aligned bases, strides of whole 16
  * bytes; |scale| and |scale * k_scale| below 2.3e38.  The call is two launches: the split over the keys, then the join
  * of what was split. */

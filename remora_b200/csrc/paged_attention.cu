@@ -1135,6 +1135,8 @@ extern "C" int remora_b200_paged_attention(const remora_b200_paged_attention_arg
                    p.kc_block % ce == 0 && p.kc_token % ce == 0 && p.kc_head % ce == 0 &&
                    p.vc_block % ce == 0 && p.vc_token % ce == 0 && p.vc_head % ce == 0,
                "paged_attention: strides must be multiples of 16 bytes");
+  RB_CHECK_ARG(!rows_overlap(R, p.out_t, D) && !rows_overlap(Hq, p.out_h, D),
+               "paged_attention: the rows of out overlap");
   const size_t need = remora_b200_paged_attention_workspace_bytes(R, Hq, Hkv, D);
   RB_CHECK_ARG(p.workspace && p.workspace_bytes >= need && aligned16(p.workspace),
                "paged_attention: workspace of %zu bytes, 16-byte aligned, is needed", need);

@@ -515,6 +515,9 @@ extern "C" int remora_b200_rope(const remora_b200_rope_args* args, void* stream)
   RB_CHECK_ARG(p.x && p.out, "rope: null pointer");
   RB_CHECK_ARG(fits32(p.x_s) && fits32(p.x_h) && fits32(p.out_s) && fits32(p.out_h),
                "rope: strides of tokens and heads must be below 2^31 elements");
+  RB_CHECK_ARG(!rows_overlap(B, p.out_b, D) && !rows_overlap(S, p.out_s, D) &&
+                   !rows_overlap(H, p.out_h, D),
+               "rope: the rows of out overlap");
   a.S = (int32_t)S;
   a.batch = Divisor((uint32_t)S);
   a.q = Heads{p.x, p.out, p.x_b, p.out_b, (int32_t)p.x_s, (int32_t)p.x_h, (int32_t)p.out_s,
@@ -564,6 +567,13 @@ extern "C" int remora_b200_rope_kv_append(const remora_b200_rope_kv_append_args*
   RB_CHECK_ARG(fits32(p.q_t) && fits32(p.q_h) && fits32(p.k_t) && fits32(p.k_h) &&
                    fits32(p.v_t) && fits32(p.v_h) && fits32(p.q_out_t) && fits32(p.q_out_h),
                "rope_kv_append: strides of tokens and heads must be below 2^31 elements");
+  RB_CHECK_ARG(Hq == 0 || (!rows_overlap(T, p.q_out_t, D) && !rows_overlap(Hq, p.q_out_h, D)),
+               "rope_kv_append: the rows of q_out overlap");
+  RB_CHECK_ARG(!rows_overlap(p.num_blocks, p.kc_block, D) &&
+                   !rows_overlap(p.block_size, p.kc_token, D) &&
+                   !rows_overlap(Hkv, p.kc_head, D) && !rows_overlap(p.num_blocks, p.vc_block, D) &&
+                   !rows_overlap(p.block_size, p.vc_token, D) && !rows_overlap(Hkv, p.vc_head, D),
+               "rope_kv_append: the rows of a cache overlap");
   a.S = (int32_t)T;
   a.q = Heads{p.q, p.q_out, 0, 0, (int32_t)p.q_t, (int32_t)p.q_h, (int32_t)p.q_out_t,
               (int32_t)p.q_out_h, (int32_t)Hq};

@@ -67,6 +67,12 @@ inline cudaStream_t as_stream(void* s) { return reinterpret_cast<cudaStream_t>(s
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// Whether neighbouring rows of `width` adjacent elements, `stride` apart, share elements: what is
+// written there would depend on the order of the writes.
+inline bool rows_overlap(int64_t size, int64_t stride, int64_t width) {
+  return size > 1 && stride < width && stride > -width;
+}
+
 // Whether all of these arrays of 32-bit elements lie where the device can read one.
 template <typename... P>
 inline bool aligned4(const P*... p) {

@@ -65,3 +65,16 @@ def test_arrays_between_elements_are_refused(L, call, fields, off):  # noqa: F81
     """A 32-bit array at an address that no 32-bit load can take."""
     for name in fields.split():
         assert call(L, **{name: A + off}) == rb.ERR_INVALID and "aligned" in rb.last_error(), name
+
+
+@pytest.mark.parametrize("call,bad", [
+    (rope, dict(oh=0)), (rope, dict(os=0)), (rope, dict(os=127)), (rope, dict(oh=-64)),
+    (rope, dict(B=2, ob=0, ld=8)), (rope, dict(x=2 * A, os=-127)),
+    (append, dict(ot=0)), (append, dict(oh=64)), (append, dict(ot=-1)),
+    (append, dict(kb=0)), (append, dict(ktok=0)), (append, dict(khd=120)), (append, dict(vb=0)),
+    (append, dict(vtok=-8)), (append, dict(vhd=0)),
+    (attention, dict(ot=0)), (attention, dict(oh=0)), (attention, dict(oh=-120))])
+def test_outputs_whose_rows_overlap_are_refused(L, call, bad):  # noqa: F811
+    """Rows that share elements (an expanded tensor, say) would hold whichever came last; in
+    place, values turned once or twice."""
+    assert call(L, **bad) == rb.ERR_INVALID and "overlap" in rb.last_error()
