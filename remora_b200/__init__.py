@@ -434,7 +434,33 @@ def rope(x: torch.Tensor, positions: torch.Tensor, freq: torch.Tensor,
     [rot / 2], rot <= D; axis_of: host int32 [rot / 2], the axis that each
     frequency follows.  Pairs are (i, i + rot / 2), or neighbours if
     interleaved.  inverse=True turns the other way: the gradient with respect
-    to x of the forward form.  out may be x; by default it has x's layout."""
+    to x of the forward form, which is also what backward() runs where x
+    requires a gradient (positions must then stay as they are until it has).
+    out may be x, and no gradient is recorded through it; by default it has
+    x's layout."""
+    if out is None and x.requires_grad and torch.is_grad_enabled():
+        return _Rope.apply(x, positions, freq, axis_of, interleaved, inverse)
+    return _rotate(x, positions, freq, axis_of, interleaved, inverse, out)
+
+
+class _Rope(torch.autograd.Function):
+    """rope() under autograd: a rotation, so its gradient is the rotation back."""
+
+    @staticmethod
+    def forward(ctx, x, positions, freq, axis_of, interleaved, inverse):
+        ctx.save_for_backward(positions, freq, axis_of)
+        ctx.how = interleaved, inverse
+        return _rotate(x, positions, freq, axis_of, interleaved, inverse, None)
+
+    @staticmethod
+    def backward(ctx, grad):
+        interleaved, inverse = ctx.how
+        if grad.stride(-1) != 1:  # a sum's gradient is expanded
+            grad = grad.contiguous()
+        return rope(grad, *ctx.saved_tensors, interleaved, not inverse), None, None, None, None, None
+
+
+def _rotate(x, positions, freq, axis_of, interleaved, inverse, out):
     if x.dim() not in (3, 4):
         raise ValueError("rope takes x as [B, S, H, D] or [T, H, D]")
     if x.dtype not in (torch.bfloat16, torch.float16, torch.float32):
@@ -487,7 +513,7 @@ def rope_kv_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions:
     k_cache and v_cache [num_blocks, block_size, Hkv, D] of q's type or
     float8_e4m3fn (x / scale is stored), any strides but adjacent row
     elements; row slots[t] of each is written, slot -1 writes none.  Returns
-    the rotated q (q_out may be q)."""
+    the rotated q (q_out may be q).  For serving: no gradient is recorded."""
     if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[0] != k.shape[0] or \
             q.shape[2] != k.shape[2]:
         raise ValueError("rope_kv_append takes q [T, Hq, D] and k, v [T, Hkv, D]")
@@ -537,7 +563,8 @@ def paged_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     each request (0: its rows of out are zero).  window > 0: the last `window`
     keys only.  lse f32 [R, Hq], if given, takes the natural logarithm of each
     softmax's sum (-inf without keys).  Calls that may run at the same time
-    need a workspace each (by default every call has its own)."""
+    need a workspace each (by default every call has its own).  For serving:
+    no gradient is recorded."""
     if q.dim() != 3 or block_table.dim() != 2:
         raise ValueError("paged_attention takes q [R, Hq, D] and block_table [R, max_blocks]")
     if q.dtype not in (torch.bfloat16, torch.float16):

@@ -178,3 +178,100 @@ def test_attention_factors_out_of_range(rb, dtype, cache, q, key, scale, k_scale
     want = score + math.log(n)
     assert bool(((lse.cpu().double() - want).abs() <= 2.0 ** -16 * abs(score) + 2.0 ** -20).all())
     rb.synchronize_and_check()
+
+
+# ---------------------------------------------------------------- gradients
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("inter,inverse", [(False, False), (True, False), (False, True)])
+def test_rope_records_its_gradient(rb, dtype, inter, inverse):
+    """backward() through rope: against the formula's transpose in 64 bits, of strided inputs and
+    of gradients of several layouts, added to what else the leaf is used for."""
+    B, S, H, D, rot = 2, 7, 3, 40, 24
+    g = gen(5)
+    pos = torch.randint(0, 4000, (2, B, S), generator=g, dtype=torch.int32)
+    f, ax = freqs(rot), (torch.arange(rot // 2) % 2).to(torch.int32)
+    x = torch.randn(B, H, S, D, generator=g).to(dtype)
+    leaf = x.cuda().requires_grad_(True)
+    y = rb.rope(leaf.transpose(1, 2), pos.cuda(), f, axis_of=ax, interleaved=inter, inverse=inverse)
+    with torch.no_grad():
+        plain = rb.rope(leaf.transpose(1, 2), pos.cuda(), f, axis_of=ax, interleaved=inter,
+                        inverse=inverse)
+    assert plain.grad_fn is None and torch.equal(plain, y) and y.stride() == plain.stride()
+    dy = torch.randn(B, S, H, D, generator=g).to(dtype)
+    for grad in (dy, dy.transpose(0, 2).contiguous().transpose(0, 2), dy[:, :, :, :1].expand_as(dy)):
+        got, = torch.autograd.grad(y, leaf, grad.cuda(), retain_graph=True)
+        want = ref.rope(grad, pos, f, ax, inter, not inverse)
+        bound = ref.rope_bound(grad, want, f, pos, dtype, inter)
+        close(got.transpose(1, 2), want, bound)
+    (y.float().sum() + leaf.float().sum()).backward()
+    want = ref.rope(torch.ones_like(dy), pos, f, ax, inter, not inverse)
+    bound = ref.rope_bound(torch.ones_like(dy), want, f, pos, dtype, inter)
+    # the sum's two gradients are added in dtype: a rounding more
+    close(leaf.grad.transpose(1, 2), want + 1, bound + ref.half_step(dtype) * ((want + 1).abs() + bound))
+
+
+def test_rope_gradient_against_differences_and_its_own(rb):
+    """Differences of a loss (linear in x but for its square, so a step of 1/8 is exact enough),
+    and the gradient of the gradient."""
+    g = gen(6)
+    x = torch.randn(4, 2, 16, generator=g)
+    pos, f = i32([0, 3, 50, 900]), freqs(16)
+    w = torch.randn(4, 2, 16, generator=g).cuda()
+
+    def loss(t):
+        y = rb.rope(t, pos, f)
+        return (w * y + y * y * 0.25).double().sum()
+
+    leaf = x.cuda().requires_grad_(True)
+    grad, = torch.autograd.grad(loss(leaf), leaf, create_graph=True)
+    h = 0.125
+    for at in ((0, 0, 0), (1, 1, 3), (2, 0, 9), (3, 1, 15)):
+        e = torch.zeros_like(x)
+        e[at] = h
+        with torch.no_grad():
+            diff = (loss((x + e).cuda()) - loss((x - e).cuda())) / (2 * h)
+        # 128 elements of at most 16, each rounded a few times in 32 bits, over the step
+        assert abs(float(diff - grad[at].detach())) <= 128 * 16 * 2.0 ** -21 / h
+    # the loss is w y + y^2 / 4 and |y| = |x|: grad = rope back of w, + x / 2
+    second, = torch.autograd.grad(grad.sum(), leaf)
+    assert float((second - 0.5).abs().max()) <= 2.0 ** -20
+
+
+def test_rope_gradient_keeps_to_its_positions(rb):
+    """Positions changed between the two passes are an error, not another angle; a call with out
+    records nothing; nor do the serving calls."""
+    x, pos, f = torch.ones(3, 1, 8, device="cuda", requires_grad=True), i32([1, 2, 3]), freqs(8)
+    y = rb.rope(x, pos, f)
+    pos.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    y = rb.rope(x, pos, f, out=torch.empty(3, 1, 8, device="cuda"))
+    assert y.grad_fn is None
+    kc = torch.zeros(1, 4, 1, 8, device="cuda", dtype=torch.bfloat16)
+    q = torch.ones(3, 1, 8, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    assert rb.rope_kv_append(q, q, q, pos, i32([0, 1, 2]), f, kc, kc.clone()).grad_fn is None
+
+
+def test_rope_gradient_in_a_graph(rb):
+    """Forward and backward captured together: each replay takes the inputs of its time."""
+    g = gen(7)
+    f, pos = freqs(64), torch.arange(12, dtype=torch.int32, device="cuda")
+    x, dy = (torch.randn(12, 2, 64, generator=g).cuda() for _ in range(2))
+    leaf = x.clone().requires_grad_(True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.autograd.grad(rb.rope(leaf, pos, f), leaf, dy)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = rb.rope(leaf, pos, f)
+        grad, = torch.autograd.grad(y, leaf, dy)
+    for _ in range(2):
+        with torch.no_grad():
+            leaf.copy_(torch.randn(12, 2, 64, generator=g))
+        dy.copy_(torch.randn(12, 2, 64, generator=g))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, rb.rope(leaf.detach(), pos, f))
+        assert torch.equal(grad, rb.rope(dy, pos, f, inverse=True))
