@@ -78,3 +78,28 @@ def test_outputs_whose_rows_overlap_are_refused(L, call, bad):  # noqa: F811
     """Rows that share elements (an expanded tensor, say) would hold whichever came last; in
     place, values turned once or twice."""
     assert call(L, **bad) == rb.ERR_INVALID and "overlap" in rb.last_error()
+
+
+_RENAMED = """
+import types
+import torch
+for name in ("_cuda_getDevice", "_cuda_getCurrentRawStream"):
+    if hasattr(torch._C, name):
+        delattr(torch._C, name)
+import remora_b200 as rb
+torch.cuda.current_device = rb._current_device = lambda: 0
+torch.cuda.current_stream = lambda index: types.SimpleNamespace(cuda_stream=70 + index)
+seen = []
+rb._launch(lambda args, stream: seen.append((args, stream)) or rb.OK, b"x", 0)
+print(seen)
+"""
+
+
+def test_calls_without_torchs_private_functions():
+    """A torch that has renamed them: streams and devices come from its public interface."""
+    import subprocess
+    import sys
+
+    r = subprocess.run([sys.executable, "-c", _RENAMED], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stderr
+    assert r.stdout.strip() == "[(b'x', 70)]"
