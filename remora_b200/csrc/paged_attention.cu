@@ -465,7 +465,7 @@ __global__ void __launch_bounds__(Shape<C, D, NT>::W * 32, 1)
   using X = Shape<C, D, NT>;
   using M = typename std::conditional<sizeof(C) == 1, __half, T>::type;  // the product's type
   constexpr int W = X::W, S = X::S, KT = X::KT, PF = kPartFloats<D, NT>;
-  constexpr bool F8 = sizeof(C) == 1, kTwo = !F8 || std::is_same<T, __half>::value;
+  constexpr bool F8 = sizeof(C) == 1;
   extern __shared__ __align__(128) char ring_all[];
   __shared__ int64_t before[kMaxRequests / 32 + 1];
   __shared__ Stage stages[W][S];
@@ -764,11 +764,12 @@ __global__ void __launch_bounds__(Shape<C, D, NT>::W * 32, 1)
           }
         }
       }
-      // The weights enter the second product as two pieces of the 16-bit type where one would be
-      // off by as much as the output's own rounding.  f16 weights of a bf16 output are one piece:
-      // off by 2^-11 of a weight at most, an eighth of the output's half step (the second piece
-      // costs a third of the tensor work: 127 us instead of 118 for 3 long requests at the clocks
-      // of a lasting load).
+      // The weights enter the second product as two pieces of the 16-bit type: off by 2^-17 of a
+      // weight (bf16) or 2^-22 (f16).  One f16 piece, off by 2^-12, is hidden by a bf16 output's
+      // rounding only where the values do not cancel: of 3 long requests over e4m3 it let 4.9 % of
+      // the outputs round the other way (two: 0.2 %, torch in 32 bits: 0.2 %).  The second costs 1 %
+      // there (119 us; 5 % at the clocks of a lasting load), 5 % for e4m3 rows of 64 and 12 % for 16
+      // heads per kv head.
       uint32_t ph[NT][KT / 8], pl[NT][KT / 8];
 #pragma unroll
       for (int k = 0; k < KT / 8; ++k)
@@ -783,10 +784,8 @@ __global__ void __launch_bounds__(Shape<C, D, NT>::W * 32, 1)
           l[n][1] += y;
           const uint32_t w = pack2<M>(x, y);
           ph[n][k] = transpose8x8(w);  // keys x heads -> a B operand's heads x keys
-          if constexpr (kTwo) {
-            const float2 r = unpack2<M>(w);
-            pl[n][k] = transpose8x8(pack2<M>(x - r.x, y - r.y));
-          }
+          const float2 r = unpack2<M>(w);
+          pl[n][k] = transpose8x8(pack2<M>(x - r.x, y - r.y));
         }
 
       // values: rows = d's, columns = heads
@@ -806,8 +805,7 @@ __global__ void __launch_bounds__(Shape<C, D, NT>::W * 32, 1)
 #pragma unroll
               for (int n = 0; n < NT; ++n) {
                 mma16816<M>(o[n][j + u], a0, a1, a2, a3, ph[n][2 * k2], ph[n][2 * k2 + 1]);
-                if constexpr (kTwo)
-                  mma16816<M>(o[n][j + u], a0, a1, a2, a3, pl[n][2 * k2], pl[n][2 * k2 + 1]);
+                mma16816<M>(o[n][j + u], a0, a1, a2, a3, pl[n][2 * k2], pl[n][2 * k2 + 1]);
               }
             }
           } else {

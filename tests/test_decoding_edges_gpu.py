@@ -275,3 +275,26 @@ def test_rope_gradient_in_a_graph(rb):
         torch.cuda.synchronize()
         assert torch.equal(y, rb.rope(leaf.detach(), pos, f))
         assert torch.equal(grad, rb.rope(dy, pos, f, inverse=True))
+
+
+# ------------------------------------------------- attention whose values cancel
+@pytest.mark.parametrize("dtype,cache", [("bf16", "e4m3"), ("f16", "e4m3"), ("bf16", "bf16")])
+@pytest.mark.parametrize("Hq,D", [(4, 64), (8, 128), (12, 128), (4, 256)])
+def test_attention_values_that_cancel(rb, dtype, cache, Hq, D):
+    """Pairs of keys of nearly the same score hold opposite values, so that the output is small
+    beside what it is summed from, and the weights' own rounding shows: 2^-17 whatever the types."""
+    from tests.test_paged_gpu import DT
+    n, bs = 32, 16
+    g = gen(D + Hq)
+    k = torch.randn(n // 2, 1, D, generator=g).repeat_interleave(2, 0)
+    k[1::2, 0, :2] += 0.25
+    v = torch.randn(n // 2, 1, D, generator=g).sign() * 240
+    v = torch.stack([v, -v], 1).flatten(0, 1)
+    q = torch.randn(1, Hq, D, generator=g).to(DT[dtype])
+    kc, vc = k.to(DT[cache]), v.to(DT[cache])
+    scale = 2.0 ** -5 / D  # small scores: their own rounding does not hide the weights'
+    out = rb.paged_attention(q.cuda(), kc.view(2, bs, 1, D).cuda(), vc.view(2, bs, 1, D).cuda(),
+                             i32([[0, 1]]), i32([n]), scale=scale)
+    o, l, mag, size = ref.attention(q[0], kc.float(), vc.float(), scale)
+    assert float(o.abs().max()) < 2.0 ** -6 * float(mag.min())
+    close(out[0], o, ref.attention_bound(o, l, mag, size, n, D, DT[dtype], 240.0)[0])
