@@ -69,12 +69,12 @@ struct Ask {
   }
 };
 
-// A block id as it may enter the table or the stack: one outside the cache is reported and
-// becomes -1.
-__device__ __forceinline__ int32_t checked_id(const TableArgs& a, int32_t id) {
-  if (id >= 0 && id < a.num_blocks) return id;
-  atomicExch(&g_device_error, 3);
-  return -1;
+// A block id as it may enter the table or the stack: one outside the cache becomes -1 (`bad`: it
+// is to be reported).
+__device__ __forceinline__ int32_t checked_id(const TableArgs& a, int32_t id, bool& bad) {
+  const bool in = (uint32_t)id < (uint32_t)a.num_blocks;
+  bad |= !in;
+  return in ? id : -1;
 }
 
 // Blocks of n tokens, n in [0, 2^31).
@@ -193,8 +193,7 @@ __global__ void __launch_bounds__(1024) k_block_table(const TableArgs a) {
   const int me = rank * nt + tid, step = ctas * nt;
   cluster_barrier();  // every CTA has read the lengths and the count: they may be overwritten
 
-  if (me == 0 && (count_in != count0 || (int64_t)count0 + all2 > a.num_blocks))
-    atomicExch(&g_device_error, 3);
+  bool bad = count_in != count0 || (int64_t)count0 + all2 > a.num_blocks;
 
   // push the released blocks
   const int32_t n_back = back[a.R];
@@ -202,7 +201,7 @@ __global__ void __launch_bounds__(1024) k_block_table(const TableArgs a) {
     const int room = min(n_back, a.num_blocks - count0);
     for (int64_t i = me; i < room; i += step) {
       const int j = (int)i, r = find_le(back, a.R, j);
-      a.free_blocks[count0 + j] = checked_id(a, a.table[(int64_t)r * a.ld_table + (j - back[r])]);
+      a.free_blocks[count0 + j] = checked_id(a, a.table[(int64_t)r * a.ld_table + (j - back[r])], bad);
     }
     cluster_barrier();
   }
@@ -231,9 +230,9 @@ __global__ void __launch_bounds__(1024) k_block_table(const TableArgs a) {
       if (r != seen_r || page != seen_page) {
         const int32_t own = blocks_of(a, l);
         if (page < own) {
-          id = checked_id(a, a.table[(int64_t)r * a.ld_table + page]);
+          id = checked_id(a, a.table[(int64_t)r * a.ld_table + page], bad);
         } else {
-          id = checked_id(a, __ldcg(a.free_blocks + (have - 1 - (need[r] + page - own))));
+          id = checked_id(a, __ldcg(a.free_blocks + (have - 1 - (need[r] + page - own))), bad);
           if (off == 0) a.table[(int64_t)r * a.ld_table + page] = id;
         }
         seen_r = r;
@@ -255,6 +254,8 @@ __global__ void __launch_bounds__(1024) k_block_table(const TableArgs a) {
         }
     }
   }
+
+  if (bad) atomicExch(&g_device_error, 3);
 
   for (int r = me; r < a.R; r += step) {
     const int32_t n = a.fresh[r], l = len0[r];
