@@ -12,7 +12,7 @@
 // handed out by an atomic whose order could change the result.
 //
 // The call is latency bound (a few KB per thousand tokens): 4.9 us on the
-// device for 8 requests, 8.9 for 256, 14.5 for 128544 tokens.  It is therefore
+// device for 8 requests, 9.0 for 256, 14.8 for 128544 tokens.  It is therefore
 // one launch of one cluster: every CTA scans the requests by itself (at most
 // 8192 lengths), the CTAs meet at a cluster barrier before anything is written,
 // and tokens are then spread over all threads, four to each, which find their

@@ -13,27 +13,28 @@
 //   - The lengths are on the device, so the split is made there.  All requests'
 //     tiles (16 or 32 keys of one kv head) form one line; every warp takes the
 //     same length of it, counting kItemCost tiles for each item that it starts
-//     (128 requests of 8 to 16001 keys: 69.6 us without that cost, 56.2 with).
+//     (128 requests of 8 to 16001 keys: 62.7 us without that cost, 51.0 with).
 //     A warp walks its tiles alone, through items and requests, with no barrier
 //     to the others.
-//   - Tiles come by cp.async into a ring per warp, 128 KB in flight per SM: the
-//     rows of a page are short (64 to 512 bytes) and lie where the block table
-//     says, so a copy is 16 bytes per lane with one address per 16 keys, the
-//     table entry fetched a tile ahead.
+//   - Tiles come by cp.async into a ring per warp, 128 KB in flight per SM (12
+//     warps: 96, or 144 in tiles of 4 KB): the rows of a page are short (64 to
+//     512 bytes) and lie where the block table says, so a copy is 16 bytes per
+//     lane with one address per 16 keys, the table entry fetched a tile ahead.
 //   - Products by mma.sync: one new token is 1 to 16 rows, far too few for a
-//     128-row tile in tensor memory, and 18 % of this pipe is enough.  Scores
-//     have the keys as rows and the heads as columns, so that no half of the
-//     instruction idles; the weights turn by movmatrix into the second
-//     product's operand.  8-bit values become f16 in registers, exactly.
+//     128-row tile in tensor memory, and for up to 8 heads per kv head 15 to
+//     27 % of this pipe is enough.  Scores have the keys as rows and the heads
+//     as columns, so that no half of the instruction idles; the weights turn by
+//     movmatrix into the second product's operand.  8-bit values become f16 in
+//     registers, exactly.
 //   - What crosses a warp's end joins in shared memory when the CTA is done,
 //     what crosses a CTA's end in the second launch, at most two parts a CTA.
 //     No atomics: the same inputs give the same bits.
 //
 // B200 (device time; the copy rate is 6462 GB/s): 64 requests of 7900 to 8190
 // keys, 8 kv heads of 128 bf16 elements, 2.11 GB: 321 to 338 us, 6.2 to 6.6
-// TB/s.  3 requests of 90 to 131 thousand keys over e4m3, 675 MB: 119 to 124 us
+// TB/s.  3 requests of 90 to 131 thousand keys over e4m3, 675 MB: 119 to 130 us
 // (the SM clock under power decides).  128 ragged requests, 272 MB: 51 us, of
-// which 7 are before the first and after the last tile.  700 keys: 9.1 us, two
+// which 7 are before the first and after the last tile.  700 keys: 9.2 us, two
 // launches of cold code.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -50,8 +51,8 @@ namespace paged {
 
 constexpr int kMaxRequests = 8192;
 constexpr int kRingBytes = 196608;  // shared memory of a CTA's rings
-// What starting and ending an item costs a warp, in tiles.  128 ragged requests: 69.6 us at 0,
-// 56.2 at 2, 56.1 at 4.  A warp's share has no lower bound: 700 keys take 9.0 us at one share and
+// What starting and ending an item costs a warp, in tiles.  128 ragged requests: 62.7 us at 0,
+// 51.0 at 2, 51.4 at 4.  A warp's share has no lower bound: 700 keys take 9.0 us at one share and
 // 10.1, 12.3 and 14.7 us where a warp takes at least 2, 4 and 6.
 constexpr int kItemCost = 2;
 constexpr int kMostWarps = 12;
@@ -147,10 +148,10 @@ __device__ __forceinline__ float2 unpack2(uint32_t x) {
 // tile's keys and values in bytes, the warps of a CTA and the tiles of a warp's ring.  8 KB tiles
 // and rings of 3 for 8 warps keep 16 KB in flight per warp while it computes.  8-bit rows take the
 // most instructions per byte (every element is widened), and 8 warps do not hide their latencies:
-// 12 with shorter rings take 121 us where 8 take 129 (3 requests of 90 to 131 thousand keys, 128
-// elements) and 73 where 8 take 95 (32 x 8k, 64 elements), but 78 where 8 take 74.5 if two groups
-// of heads fill the registers (16 heads per kv head).  For 16-bit rows of 128 bytes 12 warps
-// measure alike (53.2 and 52.6 us, 128 ragged requests), and 12 or 16 warps of half the keys
+// 12 with shorter rings take 65 us where 8 take 94 (32 x 8k, 64 elements) and 124 where 8 take 124
+// too (3 requests of 90 to 131 thousand keys, 128 elements), but 102 where 8 take 75 if two groups
+// of heads fill the registers (16 heads per kv head: they spill).  For 16-bit rows of 128 bytes 12
+// warps measured alike (53.2 and 52.6 us, 128 ragged requests), and 12 or 16 warps of half the keys
 // slower (60 and 67 us against 56: more instructions per key).
 __host__ __device__ constexpr int tile_keys(int rb) { return rb <= 128 ? 32 : 16; }
 __host__ __device__ constexpr int tile_bytes(int rb) { return 2 * tile_keys(rb) * rb; }
@@ -345,8 +346,8 @@ struct Walk {
           }
         }
       };
-      // (blocks of whole 16 keys; by one address per key, below, the batch of 64 takes 360 us
-      // instead of 324)
+      // (blocks of whole 16 keys; by one address per key, below, the batch of 64 takes 357 us
+      // instead of 330)
       if (a.whole16 && mask == kAll) {
         rows(std::true_type());
       } else if (a.whole16) {
@@ -1012,7 +1013,7 @@ __global__ void __launch_bounds__(kJoinWarps * 32)
 }
 
 // Groups of eight query heads that a warp takes at once: two where a kv head has more than eight
-// and registers allow (16 heads per kv head, 16 x 4k: 59 us against 93 in two items of eight, each
+// and registers allow (16 heads per kv head, 16 x 4k: 59 us against 91 in two items of eight, each
 // reading the keys).
 inline int head_tiles(int64_t Hq, int64_t Hkv, int64_t D) { return Hq / Hkv > 8 && D <= 128 ? 2 : 1; }
 

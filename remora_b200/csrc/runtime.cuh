@@ -79,8 +79,10 @@ inline bool aligned4(const P*... p) {
   return ((reinterpret_cast<uintptr_t>(p) | ... | uintptr_t(0)) & 3u) == 0;
 }
 
-// Division of n < 2^31 by d, as a multiplication: m = floor(2^(31 + s) / d) + 1 with 2^s >= d
-// is off by at most 2^s / d < 1 per n / 2^31, which never carries into the quotient.
+// Division of n < 2^31 by d, as a multiplication (Granlund and Montgomery, "Division by invariant
+// integers using multiplication", 1994).  m = floor(2^(31 + s) / d) + 1 with 2^s >= d is above
+// 2^(31 + s) / d by e / d, 0 < e <= d <= 2^s, so that n m / 2^(31 + s) is above n / d by
+// n e / (d 2^(31 + s)) < 1 / d, which never carries into the quotient.
 struct Divisor {
   uint32_t d, m, s;
   Divisor() = default;
