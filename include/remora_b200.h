@@ -200,8 +200,8 @@ int remora_b200_attention_fwd_bf16(const void* q, const void* k, const void* v, 
 /* Block tables, slots and positions of one step, from the requests' lengths.
  * Request r (r < R <= 8192) holds lens[r] tokens in the first
  * ceil(lens[r] / block_size) blocks of block_table[r * ld_table ...]
- * (max_blocks entries; a block belongs to one request); free_blocks (num_blocks entries) is a stack of the
- * *free_count free block ids.  new_tokens[r] >= 0 appends that many tokens,
+ * (max_blocks entries; a block belongs to one request); free_blocks
+ * (num_blocks entries) is a stack of the *free_count free block ids.  new_tokens[r] >= 0 appends that many tokens,
  * REMORA_B200_KV_RELEASE gives the request's blocks back (its table row is
  * left as it is, its length becomes 0).  Released blocks are pushed first, in
  * (request, page) order; then blocks are popped in the same order.
@@ -246,13 +246,15 @@ int remora_b200_kv_block_table(const remora_b200_kv_block_table_args* args, void
  * or (2i, 2i + 1) if interleaved != 0; elements from rot on are copied.
  * x and out: dtype BF16, F16 or F32, [B][S][H][D] by the strides x_b, x_s,
  * x_h (elements; out may be x, with its strides; the rows of out must not
- * overlap).  positions: n_axes rows of B * S int32 on the device.  freq (rot / 2 doubles) and axis_of (rot / 2 ints, NULL = all 0)
- * are HOST arrays, read before the call returns.  rot even, <= min(D, 256);
- * D <= 512 (above 256, sizes, strides and bases in whole 4 elements); n_axes
- * <= 8.  Frequencies below 2^64 radians per position; angles are exact to
- * 2^-25 of a quarter turn at every one of them and every 32-bit position.  Any strides (of tokens and heads below 2^31
- * elements), at most 2^30 tokens; sizes, strides and bases that are multiples
- * of 8 elements (and 16 bytes) move 8 pairs at a time. */
+ * overlap).  positions: n_axes rows of B * S int32 on the device.  freq
+ * (rot / 2 doubles) and axis_of (rot / 2 ints, NULL = all 0) are HOST arrays,
+ * read before the call returns.  rot even, <= min(D, 256); D <= 512 (above
+ * 256, sizes, strides and bases in whole 4 elements); n_axes <= 8.
+ * Frequencies below 2^64 radians per position; angles are exact to 2^-25 of a
+ * quarter turn at every one of them and every 32-bit position.  Any strides
+ * (of tokens and heads below 2^31 elements), at most 2^30 tokens; sizes,
+ * strides and bases that are multiples of 8 elements (and 16 bytes) move 8
+ * pairs at a time. */
 typedef struct remora_b200_rope_args {
   const void* x;
   void* out;
@@ -269,8 +271,9 @@ int remora_b200_rope(const remora_b200_rope_args* args, void* stream);
  * one pass: q_out[t] = rope(q[t]), cache row of slots[t] = rope(k[t]) and
  * v[t].  q [T][Hq][D], k and v [T][Hkv][D] by token and head strides (slices
  * of one projection are taken as they lie; q_out may be q, with its strides;
- * the rows of q_out and of the caches must not overlap); dtype BF16 or F16; cache_dtype is dtype or E4M3 (then with the scales k_scale and
- * v_scale, else both must be 1).  A token whose slot is -1 writes no cache
+ * the rows of q_out and of the caches must not overlap); dtype BF16 or F16;
+ * cache_dtype is dtype or E4M3 (then with the scales k_scale and v_scale,
+ * else both must be 1).  A token whose slot is -1 writes no cache
  * row.  Two tokens of one slot leave one row or the other in each element.
  * kc_* and vc_*: the caches' strides of block, token and head.  The rest as
  * remora_b200_rope. */
@@ -309,10 +312,11 @@ size_t remora_b200_paged_attention_workspace_bytes(int64_t R, int64_t Hq, int64_
  * lse = -infinity.  Cache rows past a request's length are never used,
  * whatever they hold; an infinity or NaN in a used row of values makes its
  * column NaN.  q and out: dtype BF16 or F16, [R][Hq][D] by strides (out must
- * not be q, nor its rows overlap); caches: dtype, or E4M3 with scales.  D in {64, 128, 256},
- * Hq % Hkv == 0, R <= 8192; 16-byte aligned bases, strides of whole 16
- * bytes; |scale| and |scale * k_scale| below 2.3e38.  The call is two launches: the split over the keys, then the join
- * of what was split. */
+ * not be q, nor its rows overlap); caches: dtype, or E4M3 with scales.  D in
+ * {64, 128, 256}, Hq % Hkv == 0, R <= 8192; 16-byte aligned bases, strides of
+ * whole 16 bytes; |scale| and |scale * k_scale| below 2.3e38.  Scores are f32;
+ * the weights meet the values with 16 bits or more of each.  The call is two
+ * launches: the split over the keys, then the join of what was split. */
 typedef struct remora_b200_paged_attention_args {
   const void* q;
   const void* k_cache;

@@ -444,9 +444,9 @@ def rope(x: torch.Tensor, positions: torch.Tensor, freq: torch.Tensor,
     frequency follows.  Pairs are (i, i + rot / 2), or neighbours if
     interleaved.  inverse=True turns the other way: the gradient with respect
     to x of the forward form, which is also what backward() runs where x
-    requires a gradient (positions must then stay as they are until it has).
-    out may be x, and no gradient is recorded through it; by default it has
-    x's layout."""
+    requires a gradient (positions must then stay as they are until it has;
+    freq gets none).  out may be x, and no gradient is recorded through it;
+    by default it has x's layout."""
     if out is None and x.requires_grad and torch.is_grad_enabled():
         return _Rope.apply(x, positions, freq, axis_of, interleaved, inverse)
     return _rotate(x, positions, freq, axis_of, interleaved, inverse, out)

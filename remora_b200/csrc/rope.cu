@@ -483,12 +483,13 @@ inline int angles(const char* who, Args& a, const int32_t* positions, int64_t ld
     const int ax = axis_of ? axis_of[i] : 0;
     RB_CHECK_ARG(ax >= 0 && ax < n_axes, "%s: axis_of[%d] = %d is not in [0, %d)", who, i, ax,
                  n_axes);
-    long double t = (long double)freq[i] * 0.159154943091895335768883763373L;  // / (2 pi)
-    if (t > -1 && t < 0) t += 1;
-    const long double f = t * 18446744073709551616.0L;
-    a.turns.f[i] = !(t > -1 && t < 1)              ? turns_of(freq[i])
-                   : f >= 18446744073709551615.0L ? 0
-                                                  : (uint64_t)f;
+    const long double t = (long double)freq[i] * 0.159154943091895335768883763373L;  // / (2 pi)
+    if (t <= -1 || t >= 1) {
+      a.turns.f[i] = turns_of(freq[i]);
+    } else {
+      const long double f = (t < 0 ? t + 1 : t) * 18446744073709551616.0L;
+      a.turns.f[i] = f >= 18446744073709551615.0L ? 0 : (uint64_t)f;
+    }
     a.turns.axis[i] = (uint8_t)ax;
   }
   return REMORA_B200_OK;

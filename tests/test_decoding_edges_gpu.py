@@ -298,3 +298,16 @@ def test_attention_values_that_cancel(rb, dtype, cache, Hq, D):
     o, l, mag, size = ref.attention(q[0], kc.float(), vc.float(), scale)
     assert float(o.abs().max()) < 2.0 ** -6 * float(mag.min())
     close(out[0], o, ref.attention_bound(o, l, mag, size, n, D, DT[dtype], 240.0)[0])
+
+
+def test_rope_frequencies_near_nothing(rb):
+    """Frequencies whose turns vanish beside one, of either sign: no angle at all, or next to."""
+    f = torch.tensor([0.0, -0.0, 1e-30, -1e-30, 5e-324, -5e-324, -1e-19, -2.0 ** -60] * 4,
+                     dtype=torch.float64)
+    pos = [0, 1, -7, 2 ** 31 - 1, -2 ** 31]
+    x = torch.randn(len(pos), 2, 64, generator=gen(8))
+    for inverse in (False, True):
+        # 2^31 times 2^-60, and one unit of the phase, 2^-32 of a turn; then the output's rounding
+        b = 2.0 ** -28 * (x[..., :32].abs() + x[..., 32:].abs()).double().repeat(1, 1, 2)
+        close(rb.rope(x.cuda(), i32(pos), f, inverse=inverse), x.double(),
+              ref.half_step(torch.float32) * (x.double().abs() + b) + b)
